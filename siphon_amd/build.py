@@ -15,11 +15,14 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 LIB_DIR = os.path.join(PKG, "lib")
 HIP_SO = os.path.join(LIB_DIR, "libsiphon_hip.so")
+# translation units of the library: csrc/<unit>.hip
+HIP_UNITS = ["sihip"]
 
 ARCH = "gfx950"
 HIPCC_FLAGS = [
@@ -52,9 +55,18 @@ def hipcc() -> str:
 
 
 def build_hip(verbose: bool = False) -> str:
+    """Compile the translation units side by side and link them."""
     os.makedirs(LIB_DIR, exist_ok=True)
+    objs = [os.path.join(LIB_DIR, u + ".hip.o") for u in HIP_UNITS]
+    flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+
+    def compile_unit(unit, obj):
+        _run([hipcc(), *flags, "-c", "-o", obj, os.path.join(PKG, "csrc", unit + ".hip")], verbose)
+
+    with ThreadPoolExecutor(len(HIP_UNITS)) as pool:
+        list(pool.map(compile_unit, HIP_UNITS, objs))
     tmp = HIP_SO + ".tmp"
-    _run([hipcc(), *HIPCC_FLAGS, "-o", tmp, os.path.join(PKG, "csrc", "sihip.hip")], verbose)
+    _run([hipcc(), *HIPCC_FLAGS, "-o", tmp, *objs], verbose)
     os.replace(tmp, HIP_SO)
     return HIP_SO
 
