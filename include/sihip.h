@@ -217,6 +217,143 @@ int sihip_attn_decode_dev(sihip_ctx *ctx, const float *q, const uint16_t *k_cach
                           int64_t head_dim, int64_t n_ctx, int64_t pos, float kq_scale,
                           float *out, float *scores, uint16_t *probs16, void *stream);
 
+/* ---- paged 8-bit KV cache ----------------------------------------------
+ * The cache of a host that serves several sequences from the device (the
+ * reference holds one sequence, engine.c:183-244): pages of `block` tokens
+ * that requests take from a common pool, keys and values in 8 bits. For each
+ * layer (device pointers, k and v 16-byte aligned):
+ *   k        int8 [n_pages][n_head_kv][block][head_dim]
+ *   v        int8 [n_pages][n_head_kv][head_dim][block]  (transposed, as the
+ *            f16 cache of sihip_attn_decode_dev)
+ *   k_scale, v_scale  f32 [n_pages][n_head_kv]
+ * A code times its page's and head's scale is the value it stands for.
+ * block: 16, 32, 64, 128 or 256; head_dim: a multiple of 16, at most 256.
+ * Memory that no token was written to may hold anything.
+ *
+ * A decode or prompt step is sihip_kv_plan_dev once, then for each layer
+ * sihip_kv_append_dev and sihip_attn_paged_dev. Lengths stay on the device
+ * between steps: the host passes bounds, nothing waits for it, and the calls
+ * may be captured into a graph. All are launched on the caller's stream
+ * and leave the caller's current device as it was. Struct pointers are
+ * read during the call only. */
+typedef struct sihip_kv_cache {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+    int64_t n_pages, n_head_kv, head_dim, block;
+} sihip_kv_cache;
+
+/* The requests of one step, as sihip_kv_plan_dev leaves them. Tokens of
+ * request r: rows q_start[r] .. q_start[r + 1] - 1 of the step's arrays; the
+ * last of them is at position kv_len[r] - 1. table[r][b] is the page of
+ * positions b * block .. A request whose numbers do not describe rows inside
+ * n_tok, or more new tokens than kv_len, takes part in nothing; a table
+ * entry outside 0 .. n_pages - 1 is a page that nothing is written to and
+ * whose keys no query sees. */
+typedef struct sihip_kv_batch {
+    const int32_t *q_start; /* [n_req + 1] */
+    const int32_t *kv_len;  /* [n_req] */
+    const int32_t *table;   /* [n_req][max_blocks] */
+    int64_t n_req, max_blocks;
+    int64_t n_tok;          /* rows of the step's arrays */
+    int64_t max_q, max_kv;  /* bounds on a request's new tokens and length, which
+                             * size the launches; what lies past them is not
+                             * written, or not seen */
+} sihip_kv_batch;
+
+/* Bookkeeping of a step. Request r has len[r] cached tokens and gets add[r]
+ * more (0: it waits), or has ended (add[r] = -1): then its pages go back to
+ * the free list and its length becomes 0 (its table row stays as it is).
+ * The free list is free_pages[0 .. *n_free - 1]; the pages of ended requests
+ * go behind it in the order of requests and blocks, then new blocks take
+ * pages from the end of that list in the order of requests and blocks.
+ *   table      entries of new blocks are written, all others left
+ *   q_start    exclusive prefix sums of the new tokens, the total last
+ *   kv_len     lengths after the step
+ *   slot, pos  of each new token in order: page * block + place in the page,
+ *              and its position; -1 in the rows behind the last token (and
+ *              a slot of -1 where its page is outside 0 .. n_pages - 1)
+ *   n_free_out length of the free list; entries past the shorter of the old
+ *              and the new list are left as they were
+ *   status     0, or the sum of: 1 a negative length or add < -1; 2 more
+ *              tokens than max_blocks holds; 4 more new tokens than n_tok;
+ *              8 too few pages; 16 a list longer than n_pages, before or
+ *              after. If not 0, nothing was taken or given back: kv_len is
+ *              len, the rest says that there are no tokens.
+ * kv_len and n_free_out must not be len and n_free (two sets of them take
+ * turns). n_req <= 4096; slot and pos may be NULL where n_tok is 0. */
+typedef struct sihip_kv_plan {
+    const int32_t *len, *add; /* [n_req] */
+    int32_t *free_pages;      /* [n_pages] */
+    const int32_t *n_free;    /* [1] */
+    int64_t n_req, n_tok, n_pages, max_blocks, block;
+    int32_t *table;           /* [n_req][max_blocks] */
+    int32_t *q_start;         /* [n_req + 1] */
+    int32_t *kv_len;          /* [n_req] */
+    int64_t *slot;            /* [n_tok] */
+    int32_t *pos;             /* [n_tok] */
+    int32_t *n_free_out;      /* [1] */
+    int32_t *status;          /* [1] */
+} sihip_kv_plan;
+
+int sihip_kv_plan_dev(sihip_ctx *ctx, const sihip_kv_plan *plan, void *stream);
+
+/* Write the step's keys and values: token t's rows are k + t * ldk and
+ * v + t * ldv, f32 [n_head_kv * head_dim]. For each page and head with new
+ * tokens the scale becomes max(scale, largest magnitude of the new values /
+ * 127), starting from 0 where the page's first token is new; new codes are
+ * value / scale, codes that were there code * old scale / new scale, rounded
+ * to the nearest, ties to even, exactly. Magnitudes below 2^-100 count as
+ * zero; infinities do not count for the scale and saturate, NaN becomes 0.
+ * Requests must not share a page that gets new tokens. */
+int sihip_kv_append_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch *batch,
+                        const float *k, int64_t ldk, const float *v, int64_t ldv, void *stream);
+
+/* Rows back as f32: row i of k and v (f32 [n_head_kv * head_dim] at i * ldk
+ * and i * ldv) receives the values of slot slots[i] (page * block + place); a
+ * slot outside the cache leaves its rows as they were. To move a sequence
+ * off the device, and to check one. */
+int sihip_kv_read_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const int64_t *slots, int64_t n,
+                      float *k, int64_t ldk, float *v, int64_t ldv, void *stream);
+
+/* Attention of the step's tokens over the cache (which holds their own keys
+ * already). For the token at position p and head h, KV head h / (n_head /
+ * n_head_kv):
+ *   s_j = kq_scale * <q, k_j>;  softcap > 0: softcap * tanh(s_j / softcap);
+ *         slopes: s_j - slopes[h] * |p - j|
+ *   out = sum_j softmax(s)_j v_j over the keys j < kv_len with j <= p and,
+ *         window > 0, p - j < window; prefix: or j < prefix[r], later ones
+ *         included. No such key: zeros.
+ * q and out: f32 rows [n_head * head_dim] at token * ldq and token * ldo; rows
+ * behind the last token are left as they were. Products are of f32 accuracy
+ * (22 bits of q and of the probabilities), sums are f32; results do not
+ * depend on the order in which workgroups run.
+ * workspace: NULL, or device memory of sihip_attn_paged_workspace bytes
+ * (256-byte aligned, zeroed once before its first use, then left alone) for
+ * callers whose launches may overlap those of other streams or graphs.
+ * With NULL the context's own is used: eager calls are ordered by the
+ * library; a graph that was captured with it must not run beside other work
+ * of the context. */
+typedef struct sihip_attn_paged {
+    const float *q;
+    int64_t ldq;
+    float *out;
+    int64_t ldo;
+    int64_t n_head;
+    float kq_scale, softcap;
+    const float *slopes;   /* [n_head] or NULL */
+    const int32_t *prefix; /* [n_req] or NULL */
+    int64_t window;        /* 0: none */
+    void *workspace;
+    uint64_t workspace_bytes;
+} sihip_attn_paged;
+
+int sihip_attn_paged_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch *batch,
+                         const sihip_attn_paged *args, void *stream);
+/* Bytes of workspace that a call with these arguments uses (0: none). */
+int sihip_attn_paged_workspace(sihip_ctx *ctx, const sihip_kv_cache *cache,
+                               const sihip_kv_batch *batch, const sihip_attn_paged *args,
+                               uint64_t *bytes);
+
 /* ---- device memory for hosts without a HIP runtime of their own -------
  * The reference host is plain C17 and never links HIP; these let it (and
  * tests) hold activations and outputs on the device for the *_dev entry

@@ -48,6 +48,42 @@ _u32 = ctypes.c_uint32
 _lib = None
 
 
+class _Args(ctypes.Structure):
+    """An argument structure of the C ABI (include/sihip.h), built from
+    keywords. Pointers are device addresses as ints; fields left out are 0."""
+
+    def __init__(self, **fields):
+        super().__init__(**fields)
+        self.ref = ctypes.byref(self)
+
+
+class KvCache(_Args):
+    """sihip_kv_cache: one layer's paged 8-bit cache."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp),
+                ("n_pages", _i64), ("n_head_kv", _i64), ("head_dim", _i64), ("block", _i64)]
+
+
+class KvBatch(_Args):
+    """sihip_kv_batch: the requests of one step."""
+    _fields_ = [("q_start", _vp), ("kv_len", _vp), ("table", _vp), ("n_req", _i64),
+                ("max_blocks", _i64), ("n_tok", _i64), ("max_q", _i64), ("max_kv", _i64)]
+
+
+class KvPlan(_Args):
+    """sihip_kv_plan: a step's bookkeeping."""
+    _fields_ = [("len", _vp), ("add", _vp), ("free_pages", _vp), ("n_free", _vp), ("n_req", _i64),
+                ("n_tok", _i64), ("n_pages", _i64), ("max_blocks", _i64), ("block", _i64),
+                ("table", _vp), ("q_start", _vp), ("kv_len", _vp), ("slot", _vp), ("pos", _vp),
+                ("n_free_out", _vp), ("status", _vp)]
+
+
+class AttnPaged(_Args):
+    """sihip_attn_paged: attention of a step's tokens over a KvCache."""
+    _fields_ = [("q", _vp), ("ldq", _i64), ("out", _vp), ("ldo", _i64), ("n_head", _i64),
+                ("kq_scale", ctypes.c_float), ("softcap", ctypes.c_float), ("slopes", _vp),
+                ("prefix", _vp), ("window", _i64), ("workspace", _vp), ("workspace_bytes", _u64)]
+
+
 def load_library(path: str = HIP_SO) -> ctypes.CDLL:
     """Load libsiphon_hip.so; raises if it has not been built."""
     global _lib
@@ -80,6 +116,11 @@ def load_library(path: str = HIP_SO) -> ctypes.CDLL:
     L.sihip_probe_read_dev.argtypes = [_vp, _vp, _u64, _vp, _vp]
     L.sihip_attn_decode_dev.argtypes = [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                                         ctypes.c_float, _vp, _vp, _vp, _vp]
+    L.sihip_kv_plan_dev.argtypes = [_vp, _vp, _vp]
+    L.sihip_kv_append_dev.argtypes = [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp]
+    L.sihip_kv_read_dev.argtypes = [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]
+    L.sihip_attn_paged_dev.argtypes = [_vp, _vp, _vp, _vp, _vp]
+    L.sihip_attn_paged_workspace.argtypes = [_vp, _vp, _vp, _vp, ctypes.POINTER(_u64)]
     L.sihip_gemm_dev.argtypes = [_vp, _vp, _vp, _i64, _vp, _vp]
     L.sihip_gemm_dev_noalloc.argtypes = [_vp, _vp, _vp, _i64, _vp, _vp]
     L.sihip_gemv_multi_dev.argtypes = [_vp, ctypes.c_int, ctypes.POINTER(_vp), _vp,
@@ -216,6 +257,30 @@ class Device:
         self._check(self.L.sihip_attn_decode_dev(self.ctx, q_ptr, k_ptr, v_ptr, n_head, n_head_kv,
                                                  head_dim, n_ctx, pos, kq_scale, out_ptr,
                                                  scores_ptr, probs_ptr, stream))
+
+    # the paged 8-bit KV cache
+    def kv_plan_dev(self, plan: KvPlan, stream: int | None = None):
+        self._check(self.L.sihip_kv_plan_dev(self.ctx, plan.ref, stream))
+
+    def kv_append_dev(self, cache: KvCache, batch: KvBatch, k_ptr: int, ldk: int, v_ptr: int,
+                      ldv: int, stream: int | None = None):
+        self._check(self.L.sihip_kv_append_dev(self.ctx, cache.ref, batch.ref, k_ptr, ldk, v_ptr,
+                                               ldv, stream))
+
+    def kv_read_dev(self, cache: KvCache, slots_ptr: int, n: int, k_ptr: int, ldk: int, v_ptr: int,
+                    ldv: int, stream: int | None = None):
+        self._check(self.L.sihip_kv_read_dev(self.ctx, cache.ref, slots_ptr, n, k_ptr, ldk, v_ptr,
+                                             ldv, stream))
+
+    def attn_paged_dev(self, cache: KvCache, batch: KvBatch, args: AttnPaged,
+                       stream: int | None = None):
+        self._check(self.L.sihip_attn_paged_dev(self.ctx, cache.ref, batch.ref, args.ref, stream))
+
+    def attn_paged_workspace(self, cache: KvCache, batch: KvBatch, args: AttnPaged) -> int:
+        n = _u64()
+        self._check(self.L.sihip_attn_paged_workspace(self.ctx, cache.ref, batch.ref, args.ref,
+                                                      ctypes.byref(n)))
+        return n.value
 
     def gemm_dev(self, w: Weight, X_ptr: int, M: int, Y_ptr: int, stream: int | None = None):
         self._check(self.L.sihip_gemm_dev(self.ctx, w.handle, X_ptr, M, Y_ptr, stream))

@@ -1,0 +1,280 @@
+// Entry points of the paged 8-bit KV cache (declarations in include/sihip.h):
+// argument checks, launch sizes, workspaces. Every array is the caller's and
+// every length is a device number, so the host checks what it can see (sizes,
+// alignment, pointers) and the kernels check what they read (requests, table
+// entries, slots) before they use it.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "attnp.h"
+#include "context.h"
+#include "kvcache.h"
+
+using namespace sihip;
+
+namespace {
+
+// The calls run on the context's device and give the caller's back.
+struct OnDevice {
+    int before = -1, device;
+    explicit OnDevice(int d) : device(d) {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        if (before != d) (void)hipSetDevice(d);
+    }
+    ~OnDevice() {
+        if (before >= 0 && before != device) (void)hipSetDevice(before);
+    }
+};
+
+bool aligned(const void *p, uintptr_t n) { return (uintptr_t)p % n == 0; }
+
+// log2 of a supported block, or -1
+int block_shift(int64_t block) {
+    for (int s = 4; s <= 8; s++)
+        if (block == (int64_t)1 << s) return s;
+    return -1;
+}
+
+int launched(sihip_ctx *ctx, const char *what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? SIHIP_OK : set_err(ctx, SIHIP_EDEVICE, "%s launch: %s", what, hipGetErrorString(e));
+}
+
+int check_cache(sihip_ctx *ctx, const char *fn, const sihip_kv_cache *c, CacheArgs &C) {
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale)
+        return set_err(ctx, SIHIP_EINVAL, "%s: NULL cache", fn);
+    const int shift = block_shift(c->block);
+    if (shift < 0)
+        return set_err(ctx, SIHIP_EINVAL, "%s: block %lld is not 16, 32, 64, 128 or 256", fn, (long long)c->block);
+    if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16)
+        return set_err(ctx, SIHIP_EINVAL, "%s: head_dim %lld is not a multiple of 16 up to 256", fn,
+                       (long long)c->head_dim);
+    if (c->n_head_kv < 1 || c->n_head_kv > 4096)
+        return set_err(ctx, SIHIP_EINVAL, "%s: n_head_kv %lld outside 1..4096", fn, (long long)c->n_head_kv);
+    if (c->n_pages < 1 || c->n_pages > INT32_MAX)
+        return set_err(ctx, SIHIP_EINVAL, "%s: n_pages %lld outside 1..2^31-1", fn, (long long)c->n_pages);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
+        return set_err(ctx, SIHIP_EINVAL, "%s: k and v must be 16-byte aligned, scales 4-byte", fn);
+    C = {c->k, c->v, c->k_scale, c->v_scale, c->n_pages, (int)c->n_head_kv, (int)c->head_dim, shift};
+    return SIHIP_OK;
+}
+
+int check_batch(sihip_ctx *ctx, const char *fn, const sihip_kv_batch *b, int64_t block, BatchArgs &R) {
+    if (!b || !b->q_start || !b->kv_len || !b->table) return set_err(ctx, SIHIP_EINVAL, "%s: NULL batch", fn);
+    if (b->n_req < 1 || b->n_req > kMaxRequests)
+        return set_err(ctx, SIHIP_EINVAL, "%s: n_req %lld outside 1..%lld", fn, (long long)b->n_req,
+                       (long long)kMaxRequests);
+    if (b->max_blocks < 1 || b->max_blocks > INT32_MAX / block)
+        return set_err(ctx, SIHIP_EINVAL, "%s: max_blocks %lld of %lld tokens pass 2^31 positions", fn,
+                       (long long)b->max_blocks, (long long)block);
+    if (b->n_tok < 0 || b->n_tok > INT32_MAX || b->max_q < 0 || b->max_q > INT32_MAX || b->max_kv < 0 ||
+        b->max_kv > INT32_MAX)
+        return set_err(ctx, SIHIP_EINVAL, "%s: n_tok %lld, max_q %lld or max_kv %lld outside 0..2^31-1", fn,
+                       (long long)b->n_tok, (long long)b->max_q, (long long)b->max_kv);
+    R = {b->q_start, b->kv_len, b->table, b->n_tok, (int)b->max_blocks,
+         (int)std::min(b->max_q, b->n_tok), (int)std::min(b->max_kv, b->max_blocks * block)};
+    return SIHIP_OK;
+}
+
+}  // namespace
+
+extern "C" int sihip_kv_plan_dev(sihip_ctx *ctx, const sihip_kv_plan *p, void *stream) {
+    if (!ctx || !p) return set_err(ctx, SIHIP_EINVAL, "kv_plan_dev: NULL argument");
+    if (!p->len || !p->add || !p->free_pages || !p->n_free || !p->table || !p->q_start || !p->kv_len ||
+        !p->n_free_out || !p->status || (p->n_tok > 0 && (!p->slot || !p->pos)))
+        return set_err(ctx, SIHIP_EINVAL, "kv_plan_dev: NULL array");
+    if (p->n_req < 1 || p->n_req > kMaxRequests)
+        return set_err(ctx, SIHIP_EINVAL, "kv_plan_dev: n_req %lld outside 1..%lld", (long long)p->n_req,
+                       (long long)kMaxRequests);
+    const int shift = block_shift(p->block);
+    if (shift < 0)
+        return set_err(ctx, SIHIP_EINVAL, "kv_plan_dev: block %lld is not 16, 32, 64, 128 or 256",
+                       (long long)p->block);
+    if (p->n_tok < 0 || p->n_tok > INT32_MAX || p->n_pages < 1 || p->n_pages > INT32_MAX)
+        return set_err(ctx, SIHIP_EINVAL, "kv_plan_dev: n_tok %lld or n_pages %lld out of range",
+                       (long long)p->n_tok, (long long)p->n_pages);
+    if (p->max_blocks < 1 || p->max_blocks > INT32_MAX / p->block)
+        return set_err(ctx, SIHIP_EINVAL, "kv_plan_dev: max_blocks %lld of %lld tokens pass 2^31 positions",
+                       (long long)p->max_blocks, (long long)p->block);
+    if (p->kv_len == p->len || p->kv_len == p->add || p->n_free_out == p->n_free)
+        return set_err(ctx, SIHIP_EINVAL, "kv_plan_dev: kv_len and n_free_out must not be inputs of the call");
+    const OnDevice on(ctx->device);
+    const PlanArgs A = {p->len, p->add, p->n_free, p->free_pages, p->table, p->q_start, p->kv_len, p->pos,
+                        p->n_free_out, p->status, p->slot, p->n_tok, (int)p->n_req, (int)p->n_pages,
+                        (int)p->max_blocks, shift};
+    const int64_t wgs = std::min<int64_t>(std::max<int64_t>(1, (p->n_tok + kPlanThreads - 1) / kPlanThreads), ctx->n_cu);
+    hipLaunchKernelGGL(kv_plan_kernel, dim3((unsigned)wgs), dim3(kPlanThreads), (size_t)p->n_req * 12,
+                       (hipStream_t)stream, A);
+    return launched(ctx, "kv_plan");
+}
+
+extern "C" int sihip_kv_append_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch *batch,
+                                   const float *k, int64_t ldk, const float *v, int64_t ldv, void *stream) {
+    if (!ctx) return set_err(ctx, SIHIP_EINVAL, "kv_append_dev: NULL argument");
+    AppendArgs A;
+    int rc = check_cache(ctx, "kv_append_dev", cache, A.C);
+    if (!rc) rc = check_batch(ctx, "kv_append_dev", batch, cache->block, A.R);
+    if (rc) return rc;
+    const int64_t width = (int64_t)A.C.n_kv * A.C.hd;
+    if (ldk < width || ldv < width)
+        return set_err(ctx, SIHIP_EINVAL, "kv_append_dev: rows of %lld values at ldk %lld, ldv %lld",
+                       (long long)width, (long long)ldk, (long long)ldv);
+    if (A.R.max_q == 0) return SIHIP_OK;
+    if (!k || !v || !aligned(k, 4) || !aligned(v, 4))
+        return set_err(ctx, SIHIP_EINVAL, "kv_append_dev: k and v must be f32 arrays");
+    A.k = k;
+    A.v = v;
+    A.ldk = ldk;
+    A.ldv = ldv;
+    const int64_t blocks = ((int64_t)A.R.max_q + cache->block - 2) / cache->block + 1;
+    A.blocks = (int)std::min<int64_t>(blocks, A.R.max_blocks);
+    const int64_t gx = (int64_t)A.blocks * A.C.n_kv;
+    if (gx * kAppendThreads > UINT32_MAX)
+        return set_err(ctx, SIHIP_EINVAL, "kv_append_dev: max_q %d of %d heads has no grid", A.R.max_q, A.C.n_kv);
+    const OnDevice on(ctx->device);
+    hipLaunchKernelGGL(kv_append_kernel, dim3((unsigned)gx, (unsigned)batch->n_req, 2), dim3(kAppendThreads), 0,
+                       (hipStream_t)stream, A);
+    return launched(ctx, "kv_append");
+}
+
+extern "C" int sihip_kv_read_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const int64_t *slots, int64_t n,
+                                 float *k, int64_t ldk, float *v, int64_t ldv, void *stream) {
+    if (!ctx) return set_err(ctx, SIHIP_EINVAL, "kv_read_dev: NULL argument");
+    ReadArgs A;
+    const int rc = check_cache(ctx, "kv_read_dev", cache, A.C);
+    if (rc) return rc;
+    const int64_t width = (int64_t)A.C.n_kv * A.C.hd;
+    if (n < 0 || n > INT32_MAX || ldk < width || ldv < width)
+        return set_err(ctx, SIHIP_EINVAL, "kv_read_dev: %lld rows of %lld values at ldk %lld, ldv %lld", (long long)n,
+                       (long long)width, (long long)ldk, (long long)ldv);
+    if (n == 0) return SIHIP_OK;
+    if (!slots || !k || !v || !aligned(slots, 8) || !aligned(k, 4) || !aligned(v, 4))
+        return set_err(ctx, SIHIP_EINVAL, "kv_read_dev: slots must be an int64 array, k and v f32 arrays");
+    A.slots = slots;
+    A.k = k;
+    A.v = v;
+    A.n = n;
+    A.ldk = ldk;
+    A.ldv = ldv;
+    const int64_t gx = (n + kReadRows - 1) / kReadRows;
+    if (gx * kReadThreads > UINT32_MAX)
+        return set_err(ctx, SIHIP_EINVAL, "kv_read_dev: %lld rows have no grid", (long long)n);
+    const OnDevice on(ctx->device);
+    hipLaunchKernelGGL(kv_read_kernel, dim3((unsigned)gx, (unsigned)A.C.n_kv), dim3(kReadThreads), 0,
+                       (hipStream_t)stream, A);
+    return launched(ctx, "kv_read");
+}
+
+// ---- attention ------------------------------------------------------------------
+
+namespace {
+
+struct AttnPPlan {
+    AttnPArgs A;
+    int64_t items;
+    size_t cnt_bytes, ws_bytes;
+};
+
+int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch *batch, const sihip_attn_paged *a,
+              AttnPPlan &P) {
+    const char *fn = "attn_paged_dev";
+    if (!ctx || !a) return set_err(ctx, SIHIP_EINVAL, "%s: NULL argument", fn);
+    AttnPArgs &A = P.A;
+    int rc = check_cache(ctx, fn, cache, A.C);
+    if (!rc) rc = check_batch(ctx, fn, batch, cache->block, A.R);
+    if (rc) return rc;
+    if (a->n_head < 1 || a->n_head > 4096 || a->n_head % A.C.n_kv)
+        return set_err(ctx, SIHIP_EINVAL, "%s: n_head %lld must be a multiple of n_head_kv %d (<= 4096)", fn,
+                       (long long)a->n_head, A.C.n_kv);
+    const int64_t width = a->n_head * A.C.hd;
+    if (a->ldq < width || a->ldo < width)
+        return set_err(ctx, SIHIP_EINVAL, "%s: rows of %lld values at ldq %lld, ldo %lld", fn, (long long)width,
+                       (long long)a->ldq, (long long)a->ldo);
+    if (!std::isfinite(a->kq_scale) || !std::isfinite(a->softcap) || a->softcap < 0)
+        return set_err(ctx, SIHIP_EINVAL, "%s: kq_scale %g or softcap %g", fn, (double)a->kq_scale,
+                       (double)a->softcap);
+    if (a->window < 0) return set_err(ctx, SIHIP_EINVAL, "%s: window %lld", fn, (long long)a->window);
+    if (A.R.max_q > 0 && (!a->q || !a->out || !aligned(a->q, 4) || !aligned(a->out, 4)))
+        return set_err(ctx, SIHIP_EINVAL, "%s: q and out must be f32 arrays", fn);
+    A.q = a->q;
+    A.out = a->out;
+    A.ldq = a->ldq;
+    A.ldo = a->ldo;
+    A.slopes = a->slopes;
+    A.prefix = a->prefix;
+    A.n_req = (int)batch->n_req;
+    A.G = (int)(a->n_head / A.C.n_kv);
+    A.window = (int)std::min<int64_t>(a->window, INT32_MAX);
+    A.scale2 = (float)((double)a->kq_scale * 1.4426950408889634);
+    A.cap = (float)((double)a->softcap * 1.4426950408889634);
+    A.cap_in = a->softcap > 0 ? (float)(2.0 * a->kq_scale / a->softcap * 1.4426950408889634) : 0.0f;
+    A.n_tiles = (int)(((int64_t)A.R.max_q * A.G + 15) / 16);
+    P.items = (int64_t)A.n_req * A.C.n_kv * A.n_tiles;
+    // splits of a row block's keys: until every CU has four workgroups, none
+    // shorter than a chunk per wave, as many as have counters
+    const int64_t chunks = ((int64_t)A.R.max_kv + 63) / 64;
+    int64_t n = (4 * (int64_t)ctx->n_cu + P.items - 1) / std::max<int64_t>(P.items, 1);
+    n = std::min<int64_t>(n, (chunks + kApWaves - 1) / kApWaves);
+    n = std::max<int64_t>(1, std::min<int64_t>(n, 64));
+    if (P.items > kGemmCounters) n = 1;
+    A.n_split = (int)n;
+    P.cnt_bytes = n > 1 ? ((size_t)P.items * 4 + 255) / 256 * 256 : 0;
+    P.ws_bytes = n > 1 ? (size_t)P.items * n * 16 * (A.C.hd + 2) * 4 : 0;
+    A.part = nullptr;
+    A.cnt = nullptr;
+    if ((int64_t)A.n_tiles * n * kApWaves * 64 > UINT32_MAX)
+        return set_err(ctx, SIHIP_EINVAL, "%s: max_q %d of %lld heads has no grid", fn, A.R.max_q,
+                       (long long)a->n_head);
+    return SIHIP_OK;
+}
+
+}  // namespace
+
+extern "C" int sihip_attn_paged_workspace(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch *batch,
+                                          const sihip_attn_paged *args, uint64_t *bytes) {
+    if (!bytes) return set_err(ctx, SIHIP_EINVAL, "attn_paged_workspace: NULL argument");
+    AttnPPlan P;
+    const int rc = plan_attn(ctx, cache, batch, args, P);
+    if (rc) return rc;
+    *bytes = P.cnt_bytes + P.ws_bytes;
+    return SIHIP_OK;
+}
+
+extern "C" int sihip_attn_paged_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch *batch,
+                                    const sihip_attn_paged *args, void *stream) {
+    AttnPPlan P;
+    int rc = plan_attn(ctx, cache, batch, args, P);
+    if (rc) return rc;
+    AttnPArgs &A = P.A;
+    if (A.R.max_q == 0) return SIHIP_OK;
+    const OnDevice on(ctx->device);
+    const hipStream_t st = (hipStream_t)stream;
+    const bool shared = A.n_split > 1 && !args->workspace;
+    if (A.n_split > 1 && args->workspace) {
+        if (args->workspace_bytes < P.cnt_bytes + P.ws_bytes || !aligned(args->workspace, 256))
+            return set_err(ctx, SIHIP_EINVAL, "attn_paged_dev: a workspace of %zu bytes, 256-byte aligned, is needed",
+                           P.cnt_bytes + P.ws_bytes);
+        A.cnt = (uint32_t *)args->workspace;
+        A.part = (float *)((uint8_t *)args->workspace + P.cnt_bytes);
+    } else if (shared) {
+        try {
+            rc = ensure(ctx, &ctx->d_attn, &ctx->d_attn_cap, P.ws_bytes, st);
+        } catch (...) {
+            rc = set_err(ctx, SIHIP_ENOMEM, "attn_paged_dev: out of host memory");
+        }
+        if (!rc) rc = order_before(ctx, ctx->order, st);
+        if (rc) return rc;
+        A.cnt = ctx->d_gcnt;
+        A.part = (float *)ctx->d_attn;
+    }
+    const dim3 grid((unsigned)(A.n_tiles * A.n_split), (unsigned)A.C.n_kv, (unsigned)A.n_req), t(kApWaves * 64);
+    if (A.C.hd <= 64) hipLaunchKernelGGL(attnp_rows_kernel<1>, grid, t, 0, st, A);
+    else if (A.C.hd <= 128) hipLaunchKernelGGL(attnp_rows_kernel<2>, grid, t, 0, st, A);
+    else if (A.C.hd <= 192) hipLaunchKernelGGL(attnp_rows_kernel<3>, grid, t, 0, st, A);
+    else hipLaunchKernelGGL(attnp_rows_kernel<4>, grid, t, 0, st, A);
+    rc = launched(ctx, "attn_paged");
+    if (rc) return rc;
+    return shared ? order_after(ctx, ctx->order, st) : SIHIP_OK;
+}
