@@ -226,8 +226,8 @@ int sihip_attn_decode_dev(sihip_ctx *ctx, const float *q, const uint16_t *k_cach
  *   v        int8 [n_pages][n_head_kv][head_dim][block]  (transposed, as the
  *            f16 cache of sihip_attn_decode_dev)
  *   k_scale, v_scale  f32 [n_pages][n_head_kv]
- * A code times its page's and head's scale is the value it stands for.
- * block: 16, 32, 64, 128 or 256; head_dim: a multiple of 16, at most 256.
+ * A code times its page's and head's scale, which is not negative, is the
+ * value it stands for. block: 16, 32, 64, 128 or 256; head_dim: a multiple of 16, at most 256.
  * Memory that no token was written to may hold anything.
  *
  * A decode or prompt step is sihip_kv_plan_dev once, then for each layer

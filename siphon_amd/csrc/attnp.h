@@ -45,8 +45,9 @@ struct AttnPArgs {
     float *out;
     int64_t ldq, ldo;
     int n_req, G, window;
-    float scale2;    // kq_scale * log2 e
-    float cap, cap_in;  // softcap * log2 e (0: none), 2 kq_scale / softcap * log2 e
+    float sign;      // of kq_scale: queries are multiplied by it,
+    float scale2;    // |kq_scale| * log2 e, so that factors of scores are not negative
+    float cap, cap_in;  // softcap * log2 e (0: none), 2 |kq_scale| / softcap * log2 e
     int n_tiles, n_split;
     float *part;     // [item][split][rows][hd + 2]: out^T sums, m, l
     uint32_t *cnt;   // [item]
@@ -86,6 +87,17 @@ __device__ inline void ap_split8(float *x, ap_h8 &hi, ap_h8 &lo) {
     }
 }
 
+// p w = hi + lo in f16 (p w up to 2^14). lo is taken from the product before
+// it is rounded; the empty statement makes the hi of the difference the one
+// that is multiplied.
+__device__ inline void ap_split8w(const float *p, float w, ap_h8 &hi, ap_h8 &lo) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) hi[j] = (_Float16)(p[j] * w);
+    asm("" : "+v"(hi));
+#pragma unroll
+    for (int j = 0; j < 8; j++) lo[j] = (_Float16)fmaf(p[j], w, -(float)hi[j]);
+}
+
 // What a block of rows of one request sees: positions p_lo .. p_hi of its
 // first and last row, the keys [0, keys), of which the first `prefix` are
 // visible to every row. In 64-key chunks: chunks [0, np) hold the prefix,
@@ -121,15 +133,26 @@ __device__ inline bool ap_visible(const AttnPArgs &A, const Sight &g, int p, int
     return j < g.keys && (j < g.prefix || (j <= p && (!A.window || j > p - A.window)));
 }
 
+// cap tanh(s / cap), s and cap in log2 units, x2 = 2 s / cap * log2 e. tanh x =
+// 1 - 2 / (e^2x + 1) is off by 2^-23 of 1, which near zero is much of a small
+// score: there (|x| < 0.32) the series up to x^11, off by 2^-24 of the score.
+__device__ inline float ap_capped(const AttnPArgs &A, float s, float x2) {
+    const float e = __builtin_amdgcn_exp2f(x2);
+    const float far = A.cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f));
+    const float x = x2 * (0.5f / kLog2e), z = x * x;
+    float y = fmaf(z, -1382.0f / 155925.0f, 62.0f / 2835.0f);
+    y = fmaf(z, y, -17.0f / 315.0f);
+    y = fmaf(z, y, 2.0f / 15.0f);
+    y = fmaf(z, y, -1.0f / 3.0f);
+    const float near = fmaf(s * z, y, s);
+    return z < 0.1f ? near : far;
+}
+
 // The score of a raw product: `f` is the factor to log2 units, fc the one of
-// the tanh's argument where scores are capped; tanh x = 1 - 2 / (e^2x + 1)
-// is off by 2^-23 of 1, that of the score by 2^-23 of the cap.
+// the tanh's argument where scores are capped.
 __device__ inline float ap_score(const AttnPArgs &A, float raw, float f, float fc, float slope, int p, int j) {
     float s = raw * f;
-    if (A.cap != 0.0f) {
-        const float e = __builtin_amdgcn_exp2f(raw * fc);
-        s = A.cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f));
-    }
+    if (A.cap != 0.0f) s = ap_capped(A, s, raw * fc);
     return fmaf(-slope, fabsf((float)(p - j)), s);
 }
 
@@ -137,6 +160,49 @@ __device__ inline float ap_score(const AttnPArgs &A, float raw, float f, float f
 __device__ inline int ap_row_exponent(float amax) {
     if (!(amax > 0.0f) || !(amax < INFINITY)) return 0;
     return max(-126, min(126, 13 - ilogbf(amax)));
+}
+
+// sums over total, 0 where no key was seen
+__device__ inline float ap_quotient(float o, float l) { return l > 0.0f || l != l ? o / l : 0.0f; }
+
+__device__ inline void ap_store(float *p, float v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The end of a row block whose keys were split over workgroups, after each
+// has stored its sums (agent-scope stores; agent.h says what their order rests
+// on): the last to arrive adds them up in the order of the splits, so the
+// result does not depend on the order of arrival, and leaves the counter zero.
+template <int ROWS, int THREADS>
+__device__ inline void ap_join(const AttnPArgs &A, const Span &s, int h, int tile, int64_t item, int rows, int n_split) {
+    __shared__ uint32_t last;
+    const int tid = threadIdx.x, hd = A.C.hd, stride = ROWS * (hd + 2);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (tid == 0)
+        last = __hip_atomic_fetch_add(A.cnt + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)n_split - 1;
+    __syncthreads();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    if (!last) return;
+    const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
+        A.part + item * A.n_split * stride, (short)0, n_split * stride * 4, 0x00020000);
+    for (int i = tid; i < rows * hd; i += THREADS) {
+        const int c = i / hd, d = i % hd;
+        float mm = kApNone, ll = 0.0f, oo = 0.0f;
+        for (int k = 0; k < n_split; k++) {
+            const uint32_t at = (uint32_t)(k * stride + c * (hd + 2)) * 4;
+            const float mk = load_agent_f32(pr, at + hd * 4), lk = load_agent_f32(pr, at + hd * 4 + 4);
+            const float vk = load_agent_f32(pr, at + d * 4);
+            const float m2 = fmaxf(mm, mk), ea = __builtin_amdgcn_exp2f(mm - m2), eb = __builtin_amdgcn_exp2f(mk - m2);
+            ll = fmaf(ll, ea, lk * eb);
+            oo = fmaf(oo, ea, vk * eb);
+            mm = m2;
+        }
+        const int rw = tile * ROWS + c;
+        A.out[(s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + d] = ap_quotient(oo, ll);
+    }
+    if (tid == 0) __hip_atomic_store(A.cnt + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ---- few rows ----------------------------------------------------------------------
@@ -147,7 +213,7 @@ __device__ inline int ap_row_exponent(float amax) {
 // of the matrix operand is token 16 (m / 4) + 4 t + m % 4) and 16 tokens of a
 // value row, converts them in registers and feeds the matrix cores.
 
-constexpr int kApWaves = 4;
+constexpr int kApWaves = 4, kApRows = 16;
 
 // hd rounded up to 64 NK dims
 template <int NK>
@@ -155,7 +221,6 @@ __global__ __launch_bounds__(kApWaves * 64) void attnp_rows_kernel(AttnPArgs A) 
     constexpr int ND = NK * 4;  // 16-dim tiles
     __shared__ float o_lds[kApWaves][16][NK * 64 + 1];
     __shared__ float m_lds[kApWaves][16], l_lds[kApWaves][16];
-    __shared__ uint32_t last;
     const int r = blockIdx.z, h = blockIdx.y;
     const int tile = blockIdx.x / A.n_split, split = blockIdx.x % A.n_split;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
@@ -197,7 +262,7 @@ __global__ __launch_bounds__(kApWaves * 64) void attnp_rows_kernel(AttnPArgs A) 
 #pragma unroll
             for (int e = 0; e < 2; e++) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[c][e][j] = ldexpf(x[c][e][j], e2);
+                for (int j = 0; j < 8; j++) x[c][e][j] = ldexpf(x[c][e][j] * A.sign, e2);
                 ap_split8(x[c][e], qh[c][e], ql[c][e]);
             }
         amax = ldexpf(1.0f, -e2);
@@ -343,45 +408,280 @@ __global__ __launch_bounds__(kApWaves * 64) void attnp_rows_kernel(AttnPArgs A) 
         }
         if (n_split == 1) {
             const int rw = tile * 16 + c;
-            A.out[(s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + d] = ll > 0.0f || ll != ll ? oo / ll : 0.0f;
+            A.out[(s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + d] = ap_quotient(oo, ll);
         } else {
-            __hip_atomic_store(part + c * (hd + 2) + d, oo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            ap_store(part + c * (hd + 2) + d, oo);
             if (d == 0) {
-                __hip_atomic_store(part + c * (hd + 2) + hd, mm, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(part + c * (hd + 2) + hd + 1, ll, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                ap_store(part + c * (hd + 2) + hd, mm);
+                ap_store(part + c * (hd + 2) + hd + 1, ll);
             }
         }
     }
     if (n_split == 1) return;
 
-    // the last split of the item to arrive joins them all, in their order
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __syncthreads();
-    if (tid == 0)
-        last = __hip_atomic_fetch_add(A.cnt + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)n_split - 1;
-    __syncthreads();
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    if (!last) return;
-    part = A.part + item * A.n_split * 16 * (hd + 2);
-    const int stride = 16 * (hd + 2);
-    const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(part, (short)0, n_split * stride * 4, 0x00020000);
-    for (int i = tid; i < rows * hd; i += kApWaves * 64) {
-        const int c = i / hd, d = i % hd;
-        float mm = kApNone, ll = 0.0f, oo = 0.0f;
-        for (int k = 0; k < n_split; k++) {
-            const uint32_t at = (uint32_t)(k * stride + c * (hd + 2)) * 4;
-            const float mk = load_agent_f32(pr, at + hd * 4), lk = load_agent_f32(pr, at + hd * 4 + 4);
-            const float vk = load_agent_f32(pr, at + d * 4);
-            const float m2 = fmaxf(mm, mk), ea = __builtin_amdgcn_exp2f(mm - m2), eb = __builtin_amdgcn_exp2f(mk - m2);
-            ll = fmaf(ll, ea, lk * eb);
-            oo = fmaf(oo, ea, vk * eb);
-            mm = m2;
+    ap_join<kApRows, kApWaves * 64>(A, s, h, tile, item, rows, n_split);
+}
+
+// ---- many rows ---------------------------------------------------------------------
+//
+// One workgroup: 128 rows of one request and KV head, 32 for each of its four
+// waves, one split of its 64-key chunks. A chunk's codes are loaded as they
+// lie, two chunks ahead, converted to f16 once for all waves and put into
+// LDS, two chunks in turn with one barrier each: converting in every wave
+// would cost as many vector instructions as the softmax. Rows of 16-byte
+// granules are permuted by an exclusive or so that eight lanes that read the
+// same column of eight rows reach all banks.
+//
+// A wave's 32x32 tile of S^T has its key rows in the order that gives lane
+// (row c, half e) the scores of keys 32 u + 16 e + i in register i: row m of
+// the operand is key 16 (m / 4 % 2) + 4 (m / 8) + m % 4.
+
+constexpr int kApTileRows = 128, kApTileThreads = 256;
+
+// hd rounded up to 16 NS dims
+template <int NS>
+__global__ __launch_bounds__(kApTileThreads, NS <= 8 ? 2 : 1) void attnp_tiles_kernel(AttnPArgs A) {
+    constexpr int ND = (NS + 1) / 2;             // 32-dim tiles of the output
+    constexpr int KC = (2 * NS + 7) / 8 * 8;     // granules of a key row in LDS
+    constexpr int NU = (64 * NS + kApTileThreads - 1) / kApTileThreads;  // 16-byte loads of a chunk, each
+    __shared__ uint4 k_lds[2][64][KC];
+    __shared__ uint4 v_lds[2][ND * 32][8];
+    const int h = blockIdx.x % A.C.n_kv, tile = A.n_tiles - 1 - blockIdx.x / A.C.n_kv, split = blockIdx.y, r = blockIdx.z;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
+    const Span s = request_span(A.R, r);
+    const int n_tok = min(s.n, A.R.max_q), n_rows = n_tok * A.G;
+    if (tile * kApTileRows >= n_rows) return;
+    const Sight S = ap_sight(A, r, s, tile * kApTileRows / A.G, min((tile * kApTileRows + kApTileRows - 1) / A.G, n_tok - 1));
+    const int n_split = max(1, min(A.n_split, S.n));
+    if (split >= n_split) return;
+    const int u0 = (int)((int64_t)S.n * split / n_split), u1 = (int)((int64_t)S.n * (split + 1) / n_split);
+
+    // the wave's rows and this lane's
+    const int row0 = tile * kApTileRows + wave * 32;
+    const bool idle = row0 >= n_rows;
+    const int row = min(row0 + col, n_rows - 1), tok = row / A.G, head = h * A.G + row % A.G, p = s.p0 + tok;
+    Sight W = S;
+    W.p_lo = s.p0 + min(row0, n_rows - 1) / A.G;
+    W.p_hi = s.p0 + min(row0 + 31, n_rows - 1) / A.G;
+    const float slope = A.slopes ? A.slopes[head] * kLog2e : 0.0f;
+    ap_h8 qh[NS], ql[NS];
+    float f_row;
+    {
+        const float *qrow = A.q + (s.q0 + tok) * A.ldq + (int64_t)head * hd + 8 * half;
+        float amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NS; c++)
+            if (16 * c < hd)
+#pragma unroll
+                for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(qrow[16 * c + j]));
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        const int e2 = ap_row_exponent(amax);
+#pragma unroll
+        for (int c = 0; c < NS; c++) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = 16 * c < hd ? ldexpf(qrow[16 * c + j] * A.sign, e2) : 0.0f;
+            ap_split8(x, qh[c], ql[c]);
         }
-        const int rw = tile * 16 + c;
-        A.out[(s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + d] = ll > 0.0f || ll != ll ? oo / ll : 0.0f;
+        f_row = ldexpf(1.0f, -e2);
     }
-    if (tid == 0) __hip_atomic_store(A.cnt + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const float fc_row = f_row * A.cap_in;
+    f_row *= A.scale2;
+
+    const int32_t *table = A.R.table + (int64_t)r * A.R.max_blocks;
+    const int64_t page_bytes = (int64_t)hd << shift;
+    auto page_of = [&](int j) {
+        const int b = j >> shift;
+        const int pg = j < S.keys && b < A.R.max_blocks ? table[b] : -1;
+        return pg >= 0 && pg < A.C.n_pages ? pg : -1;
+    };
+    // this thread's parts of a chunk: 16 dims of a key, 16 keys of a dim
+    uint4 kr[NU], vr[NU];
+    int kpg[NU], vpg, spg[2];
+    float ksc[2], vsc[2];
+    auto load_pages = [&](int u) {
+        const int j0 = ap_chunk(S, u) * 64;
+#pragma unroll
+        for (int i = 0; i < NU; i++) kpg[i] = page_of(j0 + (tid + kApTileThreads * i) / NS);
+        vpg = page_of(j0 + 16 * (tid & 3));
+    };
+    auto load_chunk = [&](int u) {
+        const int j0 = ap_chunk(S, u) * 64;
+#pragma unroll
+        for (int i = 0; i < NU; i++) {
+            const int un = tid + kApTileThreads * i;
+            const int key = un / NS, d16 = un % NS, dim = un >> 2;
+            const int64_t kb = ((int64_t)max(kpg[i], 0) * A.C.n_kv + h) * page_bytes + (int64_t)((j0 + key) & (B - 1)) * hd;
+            const int64_t vb = ((int64_t)max(vpg, 0) * A.C.n_kv + h) * page_bytes + ((j0 + 16 * (un & 3)) & (B - 1));
+            if (un < 64 * NS && d16 * 16 < hd) kr[i] = *(const uint4 *)(A.C.k + kb + d16 * 16);
+            if (dim < hd) vr[i] = *(const uint4 *)(A.C.v + vb + ((int64_t)dim << shift));
+        }
+    };
+    auto put_chunk = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NU; i++) {
+            const int un = tid + kApTileThreads * i;
+            const int key = un / NS, d16 = un % NS, dim = un >> 2;
+            if (un < 64 * NS && d16 * 16 < hd) {
+                const int x = (key & 3) | ((key >> 2) & 4);
+                k_lds[buf][key][(2 * d16) ^ x] = __builtin_bit_cast(uint4, ap_cvt8(kr[i].x, kr[i].y));
+                k_lds[buf][key][(2 * d16 + 1) ^ x] = __builtin_bit_cast(uint4, ap_cvt8(kr[i].z, kr[i].w));
+            }
+            if (dim < hd) {
+                const int c = 2 * (un & 3), x = dim & 7;
+                v_lds[buf][dim][c ^ x] = __builtin_bit_cast(uint4, ap_cvt8(vr[i].x, vr[i].y));
+                v_lds[buf][dim][(c + 1) ^ x] = __builtin_bit_cast(uint4, ap_cvt8(vr[i].z, vr[i].w));
+            }
+        }
+    };
+    auto load_scales = [&](int u) {
+        const int j0 = ap_chunk(S, u) * 64;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            spg[i] = page_of(j0 + 32 * i + 16 * half);
+            const int64_t at = (int64_t)max(spg[i], 0) * A.C.n_kv + h;
+            ksc[i] = A.C.ks[at];
+            vsc[i] = A.C.vs[at];
+        }
+    };
+
+    ap_f16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    float m = kApNone, l = 0.0f, ref = 0.0f;
+    // dims past hd meet zeros of q: keys must not hold NaN there
+    if (16 * NS > hd) {
+        for (int i = tid; i < 2 * 64 * KC; i += kApTileThreads) (&k_lds[0][0][0])[i] = uint4{0, 0, 0, 0};
+        __syncthreads();
+    }
+    if (u0 < u1) {
+        load_pages(u0);
+        load_chunk(u0);
+        load_pages(min(u0 + 1, u1 - 1));
+        put_chunk(0);
+        load_chunk(min(u0 + 1, u1 - 1));
+        load_pages(min(u0 + 2, u1 - 1));
+    }
+    for (int u = u0; u < u1; u++) {
+        const int buf = (u - u0) & 1;
+        load_scales(u);
+        __syncthreads();
+        if (u + 1 < u1) {
+            put_chunk(buf ^ 1);
+            load_chunk(min(u + 2, u1 - 1));
+            load_pages(min(u + 3, u1 - 1));
+        }
+        const int j0 = ap_chunk(S, u) * 64;
+        // nothing here for this wave's rows
+        if (idle || (j0 >= S.prefix && (j0 > W.p_hi || (A.window && j0 + 63 <= W.p_lo - A.window)))) continue;
+
+        ap_f16 sc[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[i][e] = 0.0f;
+        const int key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3), x = col & 7;
+#pragma unroll
+        for (int c = 0; c < NS; c++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const ap_h8 a = __builtin_bit_cast(ap_h8, k_lds[buf][32 * i + key][(2 * c + half) ^ x]);
+                sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], sc[i], 0, 0, 0);
+                sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], sc[i], 0, 0, 0);
+            }
+        float f[2] = {f_row * ksc[0], f_row * ksc[1]};
+        bool seen[2] = {spg[0] >= 0, spg[1] >= 0};
+        const bool mask = !ap_whole(A, W, j0 >> 6) || __any(!seen[0] || !seen[1]);
+        if (mask || A.cap != 0.0f || A.slopes) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float fc = fc_row * ksc[i];
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int j = j0 + 32 * i + 16 * half + e;
+                    const bool see = seen[i] && ap_visible(A, S, p, j);
+                    const float v = ap_score(A, sc[i][e], f[i], fc, slope, p, j);
+                    any |= see;
+                    sc[i][e] = see ? v : -INFINITY;
+                }
+                seen[i] = any;
+                f[i] = 1.0f;
+            }
+        }
+        float mx = kApNone, top = 0x1p-100f;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float y = sc[i][0];
+#pragma unroll
+            for (int e = 1; e < 16; e++) y = fmaxf(y, sc[i][e]);
+            mx = fmaxf(mx, y * f[i]);
+            vsc[i] = seen[i] ? vsc[i] : 0.0f;
+            top = fmaxf(top, vsc[i] >= 0x1p-100f && vsc[i] < INFINITY ? ldexpf(1.0f, ilogbf(vsc[i])) : 0.0f);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any(mx > m || top > ref)) {
+            // a row's own scale: columns of one tile see other segments
+            const float m2 = fmaxf(m, mx), r2 = fmaxf(ref, top), am = __builtin_amdgcn_exp2f(m - m2), ao = am * (ref / r2);
+            l *= am;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= ao;
+            m = m2;
+            ref = r2;
+        }
+        float sum = 0.0f;
+        const float unit = 0x1p13f / ref;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float w = vsc[i] * unit;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                ap_h8 ph, pl;
+                float pr[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    pr[j] = __builtin_amdgcn_exp2f(fmaf(sc[i][8 * e + j], f[i], -m));
+                    sum += pr[j];
+                }
+                ap_split8w(pr, w, ph, pl);
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const ap_h8 a = __builtin_bit_cast(ap_h8, v_lds[buf][32 * d + col][(4 * i + 2 * half + e) ^ x]);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl, o[d], 0, 0, 0);
+                }
+            }
+        }
+        l += sum;
+    }
+    l += __shfl_xor(l, 32);
+
+    const int64_t item = ((int64_t)r * A.C.n_kv + h) * A.n_tiles + tile;
+    const int rows = min(kApTileRows, n_rows - tile * kApTileRows);
+    const float back = ref * 0x1p-13f;
+    if (row0 + col < n_rows) {
+        float *to = n_split == 1 ? A.out + (s.q0 + tok) * A.ldo + (int64_t)head * hd
+                                 : A.part + ((item * A.n_split + split) * kApTileRows + wave * 32 + col) * (hd + 2);
+        const float over = n_split == 1 ? (l > 0.0f || l != l ? back / l : 0.0f) : back;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int dim = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
+                if (dim >= hd) continue;
+                if (n_split == 1) to[dim] = o[d][i] * over;
+                else ap_store(to + dim, o[d][i] * over);
+            }
+        if (n_split > 1 && half == 0) {
+            ap_store(to + hd, m);
+            ap_store(to + hd + 1, l);
+        }
+    }
+    if (n_split > 1) ap_join<kApTileRows, kApTileThreads>(A, s, h, tile, item, rows, n_split);
 }
 
 }  // namespace sihip

@@ -98,6 +98,15 @@ def test_masks_and_scores(dev, change, heads, n_kv, hd, block, steps):
     check(dev, cache, table, q_start, kv_len, queries(rng, sum(adds), heads, hd, 2.0), 1 / np.sqrt(hd), **o)
 
 
+@pytest.mark.parametrize("kq", [-0.25, 0.0, 1e-30, 3.0])
+@pytest.mark.parametrize("cap", [0.0, 10.0])
+def test_score_factors(dev, kq, cap):
+    rng = np.random.default_rng(17)
+    cache, table, q_start, kv_len = ko.requests(rng, [400, 0, 90], [1, 60, 3], 32, 2, 64)
+    check(dev, cache, table, q_start, kv_len, queries(rng, 64, 4, 64), kq, cap=cap)
+    check(dev, cache, table, [0, 1, 1, 4], kv_len, queries(rng, 4, 4, 64), kq, cap=cap)
+
+
 @pytest.mark.parametrize("adds", [[2, 3, 8], [4] * 5, [5, 1, 16, 2]])
 def test_a_few_tokens_each(dev, adds):
     """Drafted tokens: more rows than a 16-row block, fewer than a prompt's."""
