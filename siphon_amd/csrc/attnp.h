@@ -45,6 +45,7 @@ struct AttnPArgs {
     float *out;
     int64_t ldq, ldo;
     int n_req, G, window;
+    bool out_vec;    // rows of out and their heads are 16-byte aligned
     float sign;      // of kq_scale: queries are multiplied by it,
     float scale2;    // |kq_scale| * log2 e, so that factors of scores are not negative
     float cap, cap_in;  // softcap * log2 e (0: none), 2 |kq_scale| / softcap * log2 e
@@ -133,6 +134,22 @@ __device__ inline bool ap_visible(const AttnPArgs &A, const Sight &g, int p, int
     return j < g.keys && (j < g.prefix || (j <= p && (!A.window || j > p - A.window)));
 }
 
+// bits 0 .. n - 1 of 16
+__device__ inline uint32_t ap_below(int n) { return (1u << max(0, min(n, 16))) - 1u; }
+
+// the keys j0 .. j0 + 15 that the row at position p does not see, as bits
+__device__ inline uint32_t ap_hidden(const AttnPArgs &A, const Sight &g, int p, int j0) {
+    uint32_t see = ap_below(min(p + 1, g.keys) - j0);
+    if (A.window) see &= ~ap_below(p + 1 - A.window - j0);
+    return 0xffffu & ~(see | ap_below(g.prefix - j0));
+}
+
+// -inf where bit e is set
+__device__ inline float ap_hide(float x, uint32_t hidden, int e) {
+    const uint32_t h = (uint32_t)((int32_t)(hidden << (31 - e)) >> 31);
+    return __builtin_bit_cast(float, (h & 0xff800000u) | (~h & __builtin_bit_cast(uint32_t, x)));
+}
+
 // cap tanh(s / cap), s and cap in log2 units, x2 = 2 s / cap * log2 e. tanh x =
 // 1 - 2 / (e^2x + 1) is off by 2^-23 of 1, which near zero is much of a small
 // score: there (|x| < 0.32) the series up to x^11, off by 2^-24 of the score.
@@ -164,6 +181,18 @@ __device__ inline int ap_row_exponent(float amax) {
 
 // sums over total, 0 where no key was seen
 __device__ inline float ap_quotient(float o, float l) { return l > 0.0f || l != l ? o / l : 0.0f; }
+
+// four values in a row; wide: p is 16-byte aligned
+__device__ inline void ap_put4(float *p, float a, float b, float c, float d, bool wide) {
+    if (wide) {
+        *(float4 *)p = float4{a, b, c, d};
+    } else {
+        p[0] = a;
+        p[1] = b;
+        p[2] = c;
+        p[3] = d;
+    }
+}
 
 __device__ inline void ap_store(float *p, float v) {
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -428,24 +457,42 @@ __global__ __launch_bounds__(kApWaves * 64) void attnp_rows_kernel(AttnPArgs A) 
 // waves, one split of its 64-key chunks. A chunk's codes are loaded as they
 // lie, two chunks ahead, converted to f16 once for all waves and put into
 // LDS, two chunks in turn with one barrier each: converting in every wave
-// would cost as many vector instructions as the softmax. Rows of 16-byte
-// granules are permuted by an exclusive or so that eight lanes that read the
-// same column of eight rows reach all banks.
+// would cost as many vector instructions as the softmax. The 16-byte granules
+// of a row are permuted by an exclusive or, so that 16 lanes that read the same
+// column of 16 rows reach all 64 banks: by four bits of the row where a row
+// is a multiple of 256 bytes, by three where it is an odd multiple of 128 and
+// neighbouring rows lie in the two halves.
 //
 // A wave's 32x32 tile of S^T has its key rows in the order that gives lane
 // (row c, half e) the scores of keys 32 u + 16 e + i in register i: row m of
 // the operand is key 16 (m / 4 % 2) + 4 (m / 8) + m % 4.
 
-constexpr int kApTileRows = 128, kApTileThreads = 256;
+// A row's maximum follows the scores when they pass it by 2^4, so that most
+// chunks leave the sums alone: weights reach 2^4 and are held times 2^9.
+constexpr float kApLate = 4.0f, kApUnit = 0x1p9f;
+
+// the power of two below x (x is 0 or more), at least 2^-100
+__device__ inline float ap_power(float x) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, fmaxf(x, 0x1p-100f)) & 0x7f800000u);
+}
+
+// the larger of lane i's and lane i + 32's
+__device__ inline float ap_max_halves(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
 
 // hd rounded up to 16 NS dims
-template <int NS>
-__global__ __launch_bounds__(kApTileThreads, NS <= 8 ? 2 : 1) void attnp_tiles_kernel(AttnPArgs A) {
+template <int NS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kernel(AttnPArgs A) {
+    constexpr int kApTileRows = 32 * WAVES, kApTileThreads = 64 * WAVES;
     constexpr int ND = (NS + 1) / 2;             // 32-dim tiles of the output
     constexpr int KC = (2 * NS + 7) / 8 * 8;     // granules of a key row in LDS
     constexpr int NU = (64 * NS + kApTileThreads - 1) / kApTileThreads;  // 16-byte loads of a chunk, each
     __shared__ uint4 k_lds[2][64][KC];
     __shared__ uint4 v_lds[2][ND * 32][8];
+    __shared__ float s_lds[2][8];
     const int h = blockIdx.x % A.C.n_kv, tile = A.n_tiles - 1 - blockIdx.x / A.C.n_kv, split = blockIdx.y, r = blockIdx.z;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
@@ -489,61 +536,61 @@ __global__ __launch_bounds__(kApTileThreads, NS <= 8 ? 2 : 1) void attnp_tiles_k
     const float fc_row = f_row * A.cap_in;
     f_row *= A.scale2;
 
+    // loads without branches: what is not there is read from elsewhere in the
+    // table or the page and replaced
     const int32_t *table = A.R.table + (int64_t)r * A.R.max_blocks;
-    const int64_t page_bytes = (int64_t)hd << shift;
+    const int last_block = max(S.keys - 1, 0) >> shift, n_pages = (int)A.C.n_pages;
     auto page_of = [&](int j) {
-        const int b = j >> shift;
-        const int pg = j < S.keys && b < A.R.max_blocks ? table[b] : -1;
-        return pg >= 0 && pg < A.C.n_pages ? pg : -1;
+        const int pg = table[min(j >> shift, last_block)];
+        return j < S.keys && pg >= 0 && pg < n_pages ? pg : -1;
     };
-    // this thread's parts of a chunk: 16 dims of a key, 16 keys of a dim
+    // this thread's parts of a chunk: 16 dims of a key, 16 keys of a dim. A
+    // chunk starts at a multiple of 64, so a part's place in its page is the
+    // thread's own and, in pages of more than 64, the chunk's.
+    constexpr bool kWhole = 64 * NS % kApTileThreads == 0;
     uint4 kr[NU], vr[NU];
-    int kpg[NU], vpg, spg[2];
-    float ksc[2], vsc[2];
+    int kpg[NU], vpg;
+    float scale;  // of threads 0 .. 7: a key or value scale of segment tid % 4, -1 where it has no page
+    auto unit = [&](int i) { return kWhole ? tid + kApTileThreads * i : min(tid + kApTileThreads * i, 64 * NS - 1); };
+    const uint32_t head_bytes = (uint32_t)hd << shift, page_bytes = head_bytes * (uint32_t)A.C.n_kv;
+    const int8_t *kb[NU], *vb[NU];
+#pragma unroll
+    for (int i = 0; i < NU; i++) {
+        const int key = unit(i) / NS, d16 = unit(i) % NS, dim = unit(i) >> 2;
+        kb[i] = A.C.k + h * (int64_t)head_bytes + (key & (B - 1)) * hd + (d16 * 16 < hd ? d16 * 16 : 0);
+        vb[i] = A.C.v + h * (int64_t)head_bytes + ((dim < hd ? dim : 0) << shift) + ((16 * (tid & 3)) & (B - 1));
+    }
     auto load_pages = [&](int u) {
         const int j0 = ap_chunk(S, u) * 64;
 #pragma unroll
-        for (int i = 0; i < NU; i++) kpg[i] = page_of(j0 + (tid + kApTileThreads * i) / NS);
+        for (int i = 0; i < NU; i++) kpg[i] = page_of(j0 + unit(i) / NS);
         vpg = page_of(j0 + 16 * (tid & 3));
     };
     auto load_chunk = [&](int u) {
-        const int j0 = ap_chunk(S, u) * 64;
+        const int at = ap_chunk(S, u) * 64 & (B - 1);
+        const uint64_t vp = (uint64_t)(uint32_t)max(vpg, 0) * page_bytes + at;
 #pragma unroll
         for (int i = 0; i < NU; i++) {
-            const int un = tid + kApTileThreads * i;
-            const int key = un / NS, d16 = un % NS, dim = un >> 2;
-            const int64_t kb = ((int64_t)max(kpg[i], 0) * A.C.n_kv + h) * page_bytes + (int64_t)((j0 + key) & (B - 1)) * hd;
-            const int64_t vb = ((int64_t)max(vpg, 0) * A.C.n_kv + h) * page_bytes + ((j0 + 16 * (un & 3)) & (B - 1));
-            if (un < 64 * NS && d16 * 16 < hd) kr[i] = *(const uint4 *)(A.C.k + kb + d16 * 16);
-            if (dim < hd) vr[i] = *(const uint4 *)(A.C.v + vb + ((int64_t)dim << shift));
+            kr[i] = *(const uint4 *)(kb[i] + ((uint64_t)(uint32_t)max(kpg[i], 0) * page_bytes + at * hd));
+            vr[i] = *(const uint4 *)(vb[i] + vp);
         }
+        if (tid < 8) scale = vpg >= 0 ? (tid < 4 ? A.C.ks : A.C.vs)[(int64_t)vpg * A.C.n_kv + h] : -1.0f;
     };
     auto put_chunk = [&](int buf) {
+        const uint4 zero = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NU; i++) {
-            const int un = tid + kApTileThreads * i;
-            const int key = un / NS, d16 = un % NS, dim = un >> 2;
-            if (un < 64 * NS && d16 * 16 < hd) {
-                const int x = (key & 3) | ((key >> 2) & 4);
-                k_lds[buf][key][(2 * d16) ^ x] = __builtin_bit_cast(uint4, ap_cvt8(kr[i].x, kr[i].y));
-                k_lds[buf][key][(2 * d16 + 1) ^ x] = __builtin_bit_cast(uint4, ap_cvt8(kr[i].z, kr[i].w));
-            }
-            if (dim < hd) {
-                const int c = 2 * (un & 3), x = dim & 7;
-                v_lds[buf][dim][c ^ x] = __builtin_bit_cast(uint4, ap_cvt8(vr[i].x, vr[i].y));
-                v_lds[buf][dim][(c + 1) ^ x] = __builtin_bit_cast(uint4, ap_cvt8(vr[i].z, vr[i].w));
-            }
+            const int key = unit(i) / NS, d16 = unit(i) % NS, dim = unit(i) >> 2;
+            // dims past hd meet zeros of q: they must be numbers
+            const uint4 a = d16 * 16 < hd ? kr[i] : zero;
+            const int kx = (key & 3) | ((key >> 2) & 4) | ((key << 1) & 8), x = KC % 16 ? kx >> 1 : kx;
+            const int c = 2 * (tid & 3), y = (dim >> 1) & 7;
+            k_lds[buf][key][(2 * d16) ^ x] = __builtin_bit_cast(uint4, ap_cvt8(a.x, a.y));
+            k_lds[buf][key][(2 * d16 + 1) ^ x] = __builtin_bit_cast(uint4, ap_cvt8(a.z, a.w));
+            v_lds[buf][dim][c ^ y] = __builtin_bit_cast(uint4, ap_cvt8(vr[i].x, vr[i].y));
+            v_lds[buf][dim][(c + 1) ^ y] = __builtin_bit_cast(uint4, ap_cvt8(vr[i].z, vr[i].w));
         }
-    };
-    auto load_scales = [&](int u) {
-        const int j0 = ap_chunk(S, u) * 64;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            spg[i] = page_of(j0 + 32 * i + 16 * half);
-            const int64_t at = (int64_t)max(spg[i], 0) * A.C.n_kv + h;
-            ksc[i] = A.C.ks[at];
-            vsc[i] = A.C.vs[at];
-        }
+        if (tid < 8) s_lds[buf][tid] = scale;
     };
 
     ap_f16 o[ND];
@@ -551,12 +598,7 @@ __global__ __launch_bounds__(kApTileThreads, NS <= 8 ? 2 : 1) void attnp_tiles_k
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    float m = kApNone, l = 0.0f, ref = 0.0f;
-    // dims past hd meet zeros of q: keys must not hold NaN there
-    if (16 * NS > hd) {
-        for (int i = tid; i < 2 * 64 * KC; i += kApTileThreads) (&k_lds[0][0][0])[i] = uint4{0, 0, 0, 0};
-        __syncthreads();
-    }
+    float m = kApNone, l = 0.0f, ref = 0.0f, over = 0.0f;
     if (u0 < u1) {
         load_pages(u0);
         load_chunk(u0);
@@ -567,7 +609,6 @@ __global__ __launch_bounds__(kApTileThreads, NS <= 8 ? 2 : 1) void attnp_tiles_k
     }
     for (int u = u0; u < u1; u++) {
         const int buf = (u - u0) & 1;
-        load_scales(u);
         __syncthreads();
         if (u + 1 < u1) {
             put_chunk(buf ^ 1);
@@ -578,107 +619,112 @@ __global__ __launch_bounds__(kApTileThreads, NS <= 8 ? 2 : 1) void attnp_tiles_k
         // nothing here for this wave's rows
         if (idle || (j0 >= S.prefix && (j0 > W.p_hi || (A.window && j0 + 63 <= W.p_lo - A.window)))) continue;
 
-        ap_f16 sc[2];
+        const bool whole = ap_whole(A, W, j0 >> 6);
+        const int key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
+        const int x = KC % 16 ? (col >> 1) & 7 : col & 15, y = (col >> 1) & 7;
+#pragma unroll 1
+        for (int i = 0; i < 2; i++) {
+            const uint4 *kl = k_lds[buf][32 * i + key];
+            ap_f16 sc;
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+            for (int e = 0; e < 16; e++) sc[e] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 16; e++) sc[i][e] = 0.0f;
-        const int key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3), x = col & 7;
-#pragma unroll
-        for (int c = 0; c < NS; c++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const ap_h8 a = __builtin_bit_cast(ap_h8, k_lds[buf][32 * i + key][(2 * c + half) ^ x]);
-                sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], sc[i], 0, 0, 0);
-                sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], sc[i], 0, 0, 0);
+            for (int c = 0; c < NS; c++) {
+                const ap_h8 a = __builtin_bit_cast(ap_h8, kl[(2 * c + half) ^ x]);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], sc, 0, 0, 0);
             }
-        float f[2] = {f_row * ksc[0], f_row * ksc[1]};
-        bool seen[2] = {spg[0] >= 0, spg[1] >= 0};
-        const bool mask = !ap_whole(A, W, j0 >> 6) || __any(!seen[0] || !seen[1]);
-        if (mask || A.cap != 0.0f || A.slopes) {
+            // scores in log2 units are sc * f; the factor is kept above zero, so
+            // that it leaves -inf as it is, and is a number where no key is seen
+            const float ksc = s_lds[buf][2 * i + half];
+            float vsc = s_lds[buf][4 + 2 * i + half], f = fmaxf(f_row * ksc, 0x1p-120f);
+            if (A.cap != 0.0f) {
+                const float fc = fc_row * ksc;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float fc = fc_row * ksc[i];
-                bool any = false;
+                for (int e = 0; e < 16; e++) sc[e] = ap_capped(A, sc[e] * f, sc[e] * fc);
+                f = 1.0f;
+            }
+            const int j1 = j0 + 32 * i + 16 * half;
+            if (A.slopes) {
+                const float far = (float)(j1 - p), base = slope * far;
+                if (j0 + 63 <= W.p_lo) {  // no key behind a row's own
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int j = j0 + 32 * i + 16 * half + e;
-                    const bool see = seen[i] && ap_visible(A, S, p, j);
-                    const float v = ap_score(A, sc[i][e], f[i], fc, slope, p, j);
-                    any |= see;
-                    sc[i][e] = see ? v : -INFINITY;
+                    for (int e = 0; e < 16; e++) sc[e] = fmaf(sc[e], f, fmaf(slope, (float)e, base));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sc[e] = fmaf(sc[e], f, -slope * fabsf(far + (float)e));
                 }
-                seen[i] = any;
-                f[i] = 1.0f;
+                f = 1.0f;
             }
-        }
-        float mx = kApNone, top = 0x1p-100f;
+            if (!whole || __any(vsc < 0.0f)) {
+                const uint32_t hidden = vsc < 0.0f ? 0xffffu : ap_hidden(A, S, p, j1);
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            float y = sc[i][0];
+                for (int e = 0; e < 16; e++) sc[e] = ap_hide(sc[e], hidden, e);
+                vsc = hidden != 0xffffu ? vsc : 0.0f;
+            }
+            float mx = sc[0];
 #pragma unroll
-            for (int e = 1; e < 16; e++) y = fmaxf(y, sc[i][e]);
-            mx = fmaxf(mx, y * f[i]);
-            vsc[i] = seen[i] ? vsc[i] : 0.0f;
-            top = fmaxf(top, vsc[i] >= 0x1p-100f && vsc[i] < INFINITY ? ldexpf(1.0f, ilogbf(vsc[i])) : 0.0f);
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__any(mx > m || top > ref)) {
-            // a row's own scale: columns of one tile see other segments
-            const float m2 = fmaxf(m, mx), r2 = fmaxf(ref, top), am = __builtin_amdgcn_exp2f(m - m2), ao = am * (ref / r2);
-            l *= am;
+            for (int e = 1; e < 16; e++) mx = fmaxf(mx, sc[e]);
+            mx = ap_max_halves(mx * f);
+            const float top = ap_max_halves(ap_power(vsc));
+            if (__any(mx > m + kApLate || top > ref)) {
+                const float m2 = fmaxf(m, mx), r2 = fmaxf(ref, top), am = __builtin_amdgcn_exp2f(m - m2), ao = am * (ref / r2);
+                l *= am;
 #pragma unroll
-            for (int d = 0; d < ND; d++) o[d] *= ao;
-            m = m2;
-            ref = r2;
-        }
-        float sum = 0.0f;
-        const float unit = 0x1p13f / ref;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const float w = vsc[i] * unit;
+                for (int d = 0; d < ND; d++) o[d] *= ao;
+                m = m2;
+                ref = r2;
+                over = kApUnit / ref;
+            }
+            const float w = vsc * over;
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 ap_h8 ph, pl;
                 float pr[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    pr[j] = __builtin_amdgcn_exp2f(fmaf(sc[i][8 * e + j], f[i], -m));
-                    sum += pr[j];
+                    pr[j] = __builtin_amdgcn_exp2f(fmaf(sc[8 * e + j], f, -m));
+                    l += pr[j];
                 }
                 ap_split8w(pr, w, ph, pl);
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
-                    const ap_h8 a = __builtin_bit_cast(ap_h8, v_lds[buf][32 * d + col][(4 * i + 2 * half + e) ^ x]);
+                    const ap_h8 a = __builtin_bit_cast(ap_h8, v_lds[buf][32 * d + col][(4 * i + 2 * half + e) ^ y]);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl, o[d], 0, 0, 0);
                 }
             }
         }
-        l += sum;
     }
     l += __shfl_xor(l, 32);
 
     const int64_t item = ((int64_t)r * A.C.n_kv + h) * A.n_tiles + tile;
     const int rows = min(kApTileRows, n_rows - tile * kApTileRows);
-    const float back = ref * 0x1p-13f;
+    const float back = ref * (1.0f / kApUnit);
     if (row0 + col < n_rows) {
-        float *to = n_split == 1 ? A.out + (s.q0 + tok) * A.ldo + (int64_t)head * hd
-                                 : A.part + ((item * A.n_split + split) * kApTileRows + wave * 32 + col) * (hd + 2);
-        const float over = n_split == 1 ? (l > 0.0f || l != l ? back / l : 0.0f) : back;
+        // four dims in a row a register group: 32 d + 8 a + 4 half ..
+        if (n_split == 1) {
+            float *to = A.out + (s.q0 + tok) * A.ldo + (int64_t)head * hd + 4 * half;
+            const float z = l > 0.0f || l != l ? back / l : 0.0f;
 #pragma unroll
-        for (int d = 0; d < ND; d++)
+            for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int dim = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
-                if (dim >= hd) continue;
-                if (n_split == 1) to[dim] = o[d][i] * over;
-                else ap_store(to + dim, o[d][i] * over);
+                for (int a = 0; a < 4; a++)
+                    if (32 * d + 8 * a < hd) ap_put4(to + 32 * d + 8 * a, o[d][4 * a] * z, o[d][4 * a + 1] * z,
+                                o[d][4 * a + 2] * z, o[d][4 * a + 3] * z, A.out_vec);
+        } else {
+            float *to = A.part + ((item * A.n_split + split) * kApTileRows + wave * 32 + col) * (hd + 2);
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int a = 0; a < 4; a++)
+                    if (32 * d + 8 * a < hd)
+#pragma unroll
+                        for (int b = 0; b < 4; b++) ap_store(to + 32 * d + 8 * a + 4 * half + b, o[d][4 * a + b] * back);
+            if (half == 0) {
+                ap_store(to + hd, m);
+                ap_store(to + hd + 1, l);
             }
-        if (n_split > 1 && half == 0) {
-            ap_store(to + hd, m);
-            ap_store(to + hd + 1, l);
         }
     }
     if (n_split > 1) ap_join<kApTileRows, kApTileThreads>(A, s, h, tile, item, rows, n_split);

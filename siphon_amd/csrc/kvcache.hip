@@ -173,7 +173,7 @@ namespace {
 
 struct AttnPPlan {
     AttnPArgs A;
-    bool tiles;  // 128-row blocks
+    int waves;  // of 32 rows in a large row block, 0: 16-row blocks
     int64_t items;
     size_t cnt_bytes, ws_bytes;
 };
@@ -203,6 +203,7 @@ int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch 
     A.out = a->out;
     A.ldq = a->ldq;
     A.ldo = a->ldo;
+    A.out_vec = aligned(a->out, 16) && a->ldo % 4 == 0;
     A.slopes = a->slopes;
     A.prefix = a->prefix;
     A.n_req = (int)batch->n_req;
@@ -214,16 +215,16 @@ int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch 
     A.cap = (float)((double)a->softcap * 1.4426950408889634);
     A.cap_in = a->softcap > 0 ? (float)(2.0 * scale / a->softcap * 1.4426950408889634) : 0.0f;
     const int64_t rows = (int64_t)A.R.max_q * A.G;
-    P.tiles = rows > 32;
-    const int block_rows = P.tiles ? kApTileRows : kApRows;
+    P.waves = rows <= 32 ? 0 : rows <= 1024 || A.C.hd > 128 ? 4 : 8;
+    const int block_rows = P.waves ? 32 * P.waves : kApRows;
     A.n_tiles = (int)((rows + block_rows - 1) / block_rows);
     P.items = (int64_t)A.n_req * A.C.n_kv * A.n_tiles;
     // splits of a row block's keys: until every CU has four workgroups (two of
     // the large ones), none shorter than a chunk per wave (eight chunks), as
     // many as have counters
     const int64_t chunks = ((int64_t)A.R.max_kv + 63) / 64;
-    int64_t n = ((P.tiles ? 2 : 4) * (int64_t)ctx->n_cu + P.items - 1) / std::max<int64_t>(P.items, 1);
-    n = std::min<int64_t>(n, P.tiles ? (chunks + 7) / 8 : (chunks + kApWaves - 1) / kApWaves);
+    int64_t n = ((P.waves ? 8 / P.waves : 4) * (int64_t)ctx->n_cu + P.items - 1) / std::max<int64_t>(P.items, 1);
+    n = std::min<int64_t>(n, P.waves ? (chunks + 7) / 8 : (chunks + kApWaves - 1) / kApWaves);
     n = std::max<int64_t>(1, std::min<int64_t>(n, 64));
     if (P.items > kGemmCounters) n = 1;
     A.n_split = (int)n;
@@ -231,7 +232,7 @@ int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch 
     P.ws_bytes = n > 1 ? (size_t)P.items * n * block_rows * (A.C.hd + 2) * 4 : 0;
     A.part = nullptr;
     A.cnt = nullptr;
-    if ((int64_t)A.n_tiles * (P.tiles ? A.C.n_kv : n) * 256 > UINT32_MAX)
+    if ((int64_t)A.n_tiles * (P.waves ? A.C.n_kv : n) * 512 > UINT32_MAX)
         return set_err(ctx, SIHIP_EINVAL, "%s: max_q %d of %lld heads has no grid", fn, A.R.max_q,
                        (long long)a->n_head);
     return SIHIP_OK;
@@ -277,13 +278,17 @@ extern "C" int sihip_attn_paged_dev(sihip_ctx *ctx, const sihip_kv_cache *cache,
         A.part = (float *)ctx->d_attn;
     }
     const int hd = A.C.hd;
-    if (P.tiles) {
-        const dim3 grid((unsigned)(A.n_tiles * A.C.n_kv), (unsigned)A.n_split, (unsigned)A.n_req), t(kApTileThreads);
-        if (hd <= 64) hipLaunchKernelGGL(attnp_tiles_kernel<4>, grid, t, 0, st, A);
-        else if (hd <= 96) hipLaunchKernelGGL(attnp_tiles_kernel<6>, grid, t, 0, st, A);
-        else if (hd <= 128) hipLaunchKernelGGL(attnp_tiles_kernel<8>, grid, t, 0, st, A);
-        else if (hd <= 192) hipLaunchKernelGGL(attnp_tiles_kernel<12>, grid, t, 0, st, A);
-        else hipLaunchKernelGGL(attnp_tiles_kernel<16>, grid, t, 0, st, A);
+    if (P.waves) {
+        const dim3 grid((unsigned)(A.n_tiles * A.C.n_kv), (unsigned)A.n_split, (unsigned)A.n_req), t(P.waves * 64);
+#define SIHIP_APT(NS)                                                                         \
+    if (P.waves == 4) hipLaunchKernelGGL((attnp_tiles_kernel<NS, 4>), grid, t, 0, st, A);     \
+    else hipLaunchKernelGGL((attnp_tiles_kernel<NS, 8>), grid, t, 0, st, A);
+        if (hd <= 64) { SIHIP_APT(4) }
+        else if (hd <= 96) { SIHIP_APT(6) }
+        else if (hd <= 128) { SIHIP_APT(8) }
+        else if (hd <= 192) hipLaunchKernelGGL((attnp_tiles_kernel<12, 4>), grid, t, 0, st, A);
+        else hipLaunchKernelGGL((attnp_tiles_kernel<16, 4>), grid, t, 0, st, A);
+#undef SIHIP_APT
     } else {
         const dim3 grid((unsigned)(A.n_tiles * A.n_split), (unsigned)A.C.n_kv, (unsigned)A.n_req), t(kApWaves * 64);
         if (hd <= 64) hipLaunchKernelGGL(attnp_rows_kernel<1>, grid, t, 0, st, A);

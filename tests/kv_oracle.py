@@ -122,10 +122,11 @@ def attention(cache, table, q_start, kv_len, q, kq_scale, cap=0.0, slopes=None, 
     twice the largest of them for a quotient of sums of exponentials, plus
     2^-20 for the exponentials and their split, and 2^-24 for each of the
     2 n + 64 additions of an output's chain: relative to sum p |v|. A key's
-    weight times its value scale is held in f16 halves of a number below 2^14,
-    the largest weight of a row being 1 and the power of two below the largest
-    scale 2^13, so its last half is a multiple of 2^-24: half of that, 2^-38 of
-    the largest scale, times codes up to 128, for each key (the sum of weights is at least 1)."""
+    weight times its value scale is held in f16 halves in units of 2^-9 of the
+    power of two below the largest scale (2^-13 where the maximum is never
+    late), so its last half is a multiple of 2^-24 there: half of that, 2^-34
+    of the largest scale, times codes up to 128, for each key (the weight of
+    a row's largest score is at least 1)."""
     T, H, hd = q.shape
     G = H // cache.n_kv
     out, err = np.zeros((T, H, hd)), np.zeros((T, H, hd))
@@ -136,7 +137,7 @@ def attention(cache, table, q_start, kv_len, q, kq_scale, cap=0.0, slopes=None, 
             continue
         k, v = cache.rows(table[r], end)
         vs = np.array([cache.vs[p] for p in table[r, :blocks_of(end, cache.block)]], np.float64)
-        step = end * 2.0 ** -38 * 128 * np.max(vs[np.isfinite(vs)], initial=0.0)
+        step = end * 2.0 ** -34 * 128 * np.max(vs[np.isfinite(vs)], initial=0.0)
         n = q1 - q0
         p = np.arange(end - n, end)[:, None]
         j = np.arange(end)[None, :]
