@@ -80,7 +80,10 @@ const char *sihip_last_error(const sihip_ctx *ctx);
  * GEMMD_MIN_M (the smallest M on the prompt GEMMs of the K-quants and of the
  * other formats, 0: never), RING_MT and RING_SBK (m tiles and K-slice length of
  * these two), ATTN_FUSE (k: decode attention in one launch up to 512 k
- * positions, at most 1536, 0: never), and
+ * positions, at most 1536, 0: never), ATTNP_WAVES (paged attention: 2, 4 or 8
+ * waves of 32 rows in a row block, 0: blocks of 16 rows; values that have no
+ * kernel for the head_dim fall back to the rule), ATTNP_SPLITS (the most
+ * splits of a row block's keys), and
  * Q80_SCALAR: 1 quantizes Q8_0-pair
  * activations with the reference's portable scalar routine (reference
  * kernels.c:542-558), as the reference does when SI_SCALAR is set or the
@@ -328,8 +331,8 @@ int sihip_kv_read_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const int64_t
  * (22 bits of q and of the probabilities), sums are f32; results do not
  * depend on the order in which workgroups run.
  * workspace: NULL, or device memory of sihip_attn_paged_workspace bytes
- * (256-byte aligned, zeroed once before its first use, then left alone) for
- * callers whose launches may overlap those of other streams or graphs.
+ * (16-byte aligned, its contents do not matter) of their own for calls that
+ * may overlap other work of the context, on other streams or in graphs.
  * With NULL the context's own is used: eager calls are ordered by the
  * library; a graph that was captured with it must not run beside other work
  * of the context. */

@@ -27,7 +27,6 @@
 #include <math.h>
 #include <stdint.h>
 
-#include "agent.h"
 #include "kvcache.h"
 
 namespace sihip {
@@ -49,9 +48,10 @@ struct AttnPArgs {
     float sign;      // of kq_scale: queries are multiplied by it,
     float scale2;    // |kq_scale| * log2 e, so that factors of scores are not negative
     float cap, cap_in;  // softcap * log2 e (0: none), 2 |kq_scale| / softcap * log2 e
-    int n_tiles, n_split;
-    float *part;     // [item][split][rows][hd + 2]: out^T sums, m, l
-    uint32_t *cnt;   // [item]
+    int n_tiles;     // most row blocks of a request
+    int n_split, per_split;  // most splits of a row block's keys, least chunks of one
+    int placed;      // large row blocks: 1 if the grid is their list (ap_place)
+    float *part;     // [item][split][hd / 4 + 1][rows] of four: sums by dims, then m, l
 };
 
 constexpr float kApNone = -3.4e38f;  // running maximum before any key
@@ -194,45 +194,38 @@ __device__ inline void ap_put4(float *p, float a, float b, float c, float d, boo
     }
 }
 
-__device__ inline void ap_store(float *p, float v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Splits of a row block with n chunks.
+__device__ inline int ap_splits(const AttnPArgs &A, int n) {
+    return max(1, min(A.n_split, (n + A.per_split - 1) / A.per_split));
 }
 
-// The end of a row block whose keys were split over workgroups, after each
-// has stored its sums (agent-scope stores; agent.h says what their order rests
-// on): the last to arrive adds them up in the order of the splits, so the
-// result does not depend on the order of arrival, and leaves the counter zero.
-template <int ROWS, int THREADS>
-__device__ inline void ap_join(const AttnPArgs &A, const Span &s, int h, int tile, int64_t item, int rows, int n_split) {
-    __shared__ uint32_t last;
-    const int tid = threadIdx.x, hd = A.C.hd, stride = ROWS * (hd + 2);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __syncthreads();
-    if (tid == 0)
-        last = __hip_atomic_fetch_add(A.cnt + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)n_split - 1;
-    __syncthreads();
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    if (!last) return;
-    const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
-        A.part + item * A.n_split * stride, (short)0, n_split * stride * 4, 0x00020000);
-    for (int i = tid; i < rows * hd; i += THREADS) {
-        const int c = i / hd, d = i % hd;
-        float mm = kApNone, ll = 0.0f, oo = 0.0f;
-        for (int k = 0; k < n_split; k++) {
-            const uint32_t at = (uint32_t)(k * stride + c * (hd + 2)) * 4;
-            const float mk = load_agent_f32(pr, at + hd * 4), lk = load_agent_f32(pr, at + hd * 4 + 4);
-            const float vk = load_agent_f32(pr, at + d * 4);
-            const float m2 = fmaxf(mm, mk), ea = __builtin_amdgcn_exp2f(mm - m2), eb = __builtin_amdgcn_exp2f(mk - m2);
-            ll = fmaf(ll, ea, lk * eb);
-            oo = fmaf(oo, ea, vk * eb);
-            mm = m2;
-        }
-        const int rw = tile * ROWS + c;
-        A.out[(s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + d] = ap_quotient(oo, ll);
-    }
-    if (tid == 0) __hip_atomic_store(A.cnt + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Sums, maximum and total of a row's split, in four-byte units of A.part
+__device__ inline int64_t ap_part(const AttnPArgs &A, int64_t item, int split, int rows) {
+    return (item * A.n_split + split) * (A.C.hd / 4 + 1) * rows * 4;
 }
+
+// the power of two below x (x is 0 or more), at least 2^-100
+__device__ inline float ap_power(float x) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, fmaxf(x, 0x1p-100f)) & 0x7f800000u);
+}
+
+// the larger of lane i's and lane i + 32's
+__device__ inline float ap_max_halves(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+// the largest of lanes i, i + 16, i + 32 and i + 48
+__device__ inline float ap_max_quarters(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, ap_max_halves(x));
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+// A row's maximum follows the scores when they pass it by 2^4, so that most
+// chunks leave the sums alone: weights reach 2^4 and are held times 2^9.
+constexpr float kApLate = 4.0f, kApUnit = 0x1p9f;
 
 // ---- few rows ----------------------------------------------------------------------
 //
@@ -240,28 +233,45 @@ __device__ inline void ap_join(const AttnPArgs &A, const Span &s, int h, int til
 // chunks; the waves take chunks in turn and join through LDS at the end.
 // Nothing is staged: a lane loads 16 bytes of a key row (key tile t, row m
 // of the matrix operand is token 16 (m / 4) + 4 t + m % 4) and 16 tokens of a
-// value row, converts them in registers and feeds the matrix cores.
+// value row, converts them in registers and feeds the matrix cores. The next
+// chunk's keys are loaded once this one's are converted, its values after
+// this one's, so that each has half an iteration to arrive and two waves of a
+// SIMD keep the memory busy.
 
-constexpr int kApWaves = 4, kApRows = 16;
+constexpr int kApRows = 16;
 
 // hd rounded up to 64 NK dims
-template <int NK>
-__global__ __launch_bounds__(kApWaves * 64) void attnp_rows_kernel(AttnPArgs A) {
+template <int NK, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, NK <= 2 ? 2 : 1) void attnp_rows_kernel(AttnPArgs A) {
     constexpr int ND = NK * 4;  // 16-dim tiles
-    __shared__ float o_lds[kApWaves][16][NK * 64 + 1];
-    __shared__ float m_lds[kApWaves][16], l_lds[kApWaves][16];
+    __shared__ float4 o_lds[WAVES][ND * 4][17];
+    __shared__ float m_lds[WAVES][16], l_lds[WAVES][16];
     const int r = blockIdx.z, h = blockIdx.y;
     const int tile = blockIdx.x / A.n_split, split = blockIdx.x % A.n_split;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
     const Span s = request_span(A.R, r);
-    const int n_rows = min(s.n, A.R.max_q) * A.G;
+    const int n_tok = min(s.n, A.R.max_q), n_rows = n_tok * A.G;
     if (tile * 16 >= n_rows) return;
-    const int t0 = tile * 16 / A.G, t1 = min((tile * 16 + 15) / A.G, min(s.n, A.R.max_q) - 1);
+    const int t0 = tile * 16 / A.G, t1 = min((tile * 16 + 15) / A.G, n_tok - 1);
     const Sight S = ap_sight(A, r, s, t0, t1);
-    const int n_split = max(1, min(A.n_split, (S.n + kApWaves - 1) / kApWaves));
+    const int n_split = ap_splits(A, S.n);
     if (split >= n_split) return;
     const int u0 = (int)((int64_t)S.n * split / n_split), u1 = (int)((int64_t)S.n * (split + 1) / n_split);
+
+    // pages of a chunk's 16-token segments: of this lane's key rows (segment
+    // col / 4), and of its values and scores (segment g)
+    const int32_t *table = A.R.table + (int64_t)r * A.R.max_blocks;
+    const int last_block = max(S.keys - 1, 0) >> shift, n_pages = (int)A.C.n_pages;
+    auto page_of = [&](int u, int seg) {
+        const int j = ap_chunk(S, u) * 64 + seg * 16, pg = table[min(j >> shift, last_block)];
+        return j < S.keys && pg >= 0 && pg < n_pages ? pg : -1;
+    };
+    int u = u0 + wave, pk = 0, pv = 0;
+    if (u < u1) {
+        pk = page_of(u, col >> 2);
+        pv = page_of(u, g);
+    }
 
     // this lane's row
     const int row = min(tile * 16 + col, n_rows - 1);
@@ -270,9 +280,9 @@ __global__ __launch_bounds__(kApWaves * 64) void attnp_rows_kernel(AttnPArgs A) 
     const float slope = A.slopes ? A.slopes[head] * kLog2e : 0.0f;
     const float *qrow = A.q + (s.q0 + tok) * A.ldq + (int64_t)head * hd;
     ap_h8 qh[NK][2], ql[NK][2];
-    float amax = 0.0f;
+    float f_row;
     {
-        float x[NK][2][8];
+        float x[NK][2][8], amax = 0.0f;
 #pragma unroll
         for (int c = 0; c < NK; c++)
 #pragma unroll
@@ -280,175 +290,177 @@ __global__ __launch_bounds__(kApWaves * 64) void attnp_rows_kernel(AttnPArgs A) 
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int d = 64 * c + 16 * g + 8 * e + j;
-                    x[c][e][j] = d < hd ? qrow[d] : 0.0f;
+                    x[c][e][j] = d < hd ? qrow[d] * A.sign : 0.0f;
                     amax = fmaxf(amax, fabsf(x[c][e][j]));
                 }
-        amax = fmaxf(amax, __shfl_xor(amax, 16));
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
-        const int e2 = ap_row_exponent(amax);
+        const int e2 = ap_row_exponent(ap_max_quarters(amax));
 #pragma unroll
         for (int c = 0; c < NK; c++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[c][e][j] = ldexpf(x[c][e][j] * A.sign, e2);
+                for (int j = 0; j < 8; j++) x[c][e][j] = ldexpf(x[c][e][j], e2);
                 ap_split8(x[c][e], qh[c][e], ql[c][e]);
             }
-        amax = ldexpf(1.0f, -e2);
+        f_row = ldexpf(1.0f, -e2);
     }
-    const float f_row = amax * A.scale2, fc_row = amax * A.cap_in;
+    const float fc_row = f_row * A.cap_in;
+    f_row *= A.scale2;
 
-    float m = kApNone, l = 0.0f, ref = 0.0f;  // ref: power of two of the value scales
+    float m = kApNone, l = 0.0f, ref = 0.0f, over = 0.0f;
     ap_f4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = ap_f4{0, 0, 0, 0};
-    const int32_t *table = A.R.table + (int64_t)r * A.R.max_blocks;
-    const int64_t page_bytes = (int64_t)hd << shift;
-
-    for (int u = u0 + wave; u < u1; u += kApWaves) {
-        const int c = ap_chunk(S, u);
-        // the pages of the 16-token segments: of this lane's key rows
-        // (segment col / 4) and of its values and scores (segment g)
-        auto page_of = [&](int seg, bool &ok) {
-            const int j = c * 64 + seg * 16, b = j >> shift;
-            const int pg = j < S.keys && b < A.R.max_blocks ? table[b] : -1;
-            ok = pg >= 0 && pg < A.C.n_pages;
-            return (int64_t)(ok ? pg : 0) * A.C.n_kv + h;
-        };
-        bool okk, ok;
-        const int64_t pk = page_of(col >> 2, okk), pv = page_of(g, ok);
-        const int koff = (c * 64 + (col >> 2) * 16) & (B - 1), voff = (c * 64 + g * 16) & (B - 1);
-        const int8_t *kp = A.C.k + pk * page_bytes + (int64_t)(koff + (col & 3)) * hd;
-        const int8_t *vp = A.C.v + pv * page_bytes + voff;
-        uint4 kr[4][NK], vr[ND];
+    // a chunk starts at a multiple of 64: a lane's place in a page is its own
+    // and, in pages of more than 64, the chunk's
+    const uint32_t head_bytes = (uint32_t)hd << shift, page_bytes = head_bytes * (uint32_t)A.C.n_kv;
+    const int8_t *kb = A.C.k + h * (int64_t)head_bytes + (((col >> 2) * 16 & (B - 1)) + (col & 3)) * hd;
+    const int8_t *vb = A.C.v + h * (int64_t)head_bytes + (col << shift) + (g * 16 & (B - 1));
+    int dim[NK];  // this lane's dims of a key row; those past hd meet zeros of q
+#pragma unroll
+    for (int e = 0; e < NK; e++) dim[e] = 64 * e + 16 * g < hd ? 64 * e + 16 * g : 0;
+    uint4 kr[4][NK], vr[ND];
+    float ksc = 0.0f, vsc = 0.0f;
+    auto load_keys = [&](int u) {
+        const int8_t *kp = kb + ((uint64_t)(uint32_t)max(pk, 0) * page_bytes + (ap_chunk(S, u) * 64 & (B - 1)) * hd);
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int e = 0; e < NK; e++) {
-                const int d = 64 * e + 16 * g;
-                kr[t][e] = *(const uint4 *)(kp + 4 * t * hd + (d < hd ? d : 0));
-            }
-        const float ksc = A.C.ks[pv], vsc = A.C.vs[pv];
+            for (int e = 0; e < NK; e++) kr[t][e] = *(const uint4 *)(kp + (4 * t * hd + dim[e]));
+        const int64_t at = (int64_t)max(pv, 0) * A.C.n_kv + h;
+        ksc = A.C.ks[at];
+        vsc = pv < 0 ? -1.0f : A.C.vs[at];  // -1: no page
+    };
+    auto load_values = [&](int u, int page) {
+        const int8_t *vp = vb + ((uint64_t)(uint32_t)max(page, 0) * page_bytes + (ap_chunk(S, u) * 64 & (B - 1)));
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            const int dim = 16 * d + col;
-            vr[d] = *(const uint4 *)(vp + ((int64_t)(dim < hd ? dim : 0) << shift));
-        }
+        for (int d = 0; d < ND; d++) vr[d] = *(const uint4 *)(vp + ((min(16 * d, hd - 16)) << shift));
+    };
+    int pv_next = 0;
+    if (u < u1) {
+        load_keys(u);
+        load_values(u, pv);
+        const int next = min(u + WAVES, u1 - 1);
+        pk = page_of(next, col >> 2);
+        pv = page_of(next, g);
+    }
+    for (; u < u1; u += WAVES) {
+        const int next = min(u + WAVES, u1 - 1), c = ap_chunk(S, u);
         ap_f4 sc[4];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            sc[t] = ap_f4{0, 0, 0, 0};
+        for (int t = 0; t < 4; t++) sc[t] = ap_f4{0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < NK; e++) {
+        for (int e = 0; e < NK; e++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
                 const ap_h8 a = ap_cvt8(kr[t][e].x, kr[t][e].y), b = ap_cvt8(kr[t][e].z, kr[t][e].w);
                 sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[e][0], sc[t], 0, 0, 0);
                 sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[e][1], sc[t], 0, 0, 0);
                 sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[e][0], sc[t], 0, 0, 0);
                 sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ql[e][1], sc[t], 0, 0, 0);
             }
+        // scores in log2 units are sc * f; the factor is kept above zero, so
+        // that it leaves -inf as it is, and is a number where no key is seen
+        const int j0 = c * 64 + g * 16;  // key of register (t, i): j0 + 4 t + i
+        float f = fmaxf(f_row * ksc, 0x1p-120f), vs = vsc;
+        const float fc = fc_row * ksc;
+        load_keys(next);
+        pv_next = pv;
+        if (A.cap != 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) sc[i >> 2][i & 3] = ap_capped(A, sc[i >> 2][i & 3] * f, sc[i >> 2][i & 3] * fc);
+            f = 1.0f;
         }
-        // scores, in log2 units; tokens of this lane: j0 + 4 t + i
-        const int j0 = c * 64 + g * 16;
-        const float f = f_row * ksc, fc = fc_row * ksc;
-        const bool mask = !ap_whole(A, S, c) || __any(!ok);
-        float mx = kApNone;
-        bool any_seen = false;
+        if (A.slopes) {
+            const float far = (float)(j0 - p);
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int i = 0; i < 16; i++) sc[i >> 2][i & 3] = fmaf(sc[i >> 2][i & 3], f, -slope * fabsf(far + (float)i));
+            f = 1.0f;
+        }
+        if (!ap_whole(A, S, c) || __any(vs < 0.0f)) {
+            const uint32_t hidden = vs < 0.0f ? 0xffffu : ap_hidden(A, S, p, j0);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int j = j0 + 4 * t + i;
-                float v = ap_score(A, sc[t][i], f, fc, slope, p, j);
-                if (mask) {
-                    const bool see = ok && ap_visible(A, S, p, j);
-                    any_seen |= see;
-                    v = see ? v : -INFINITY;
-                }
-                sc[t][i] = v;
-                mx = fmaxf(mx, v);
-            }
-        const bool seen = ok && (!mask || any_seen);
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        // the value scales' power of two: the largest so far. A segment that
-        // this row does not see counts nothing, whatever its page holds.
-        const float vs = seen ? vsc : 0.0f;
-        float top = vs >= 0x1p-100f && vs < INFINITY ? ldexpf(1.0f, ilogbf(vs)) : 0x1p-100f;
-        for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-        const float ref2 = fmaxf(ref, top), m2 = fmaxf(m, mx);
-        const float am = __builtin_amdgcn_exp2f(m - m2);
-        const float ao = am * (ref / ref2);
-        m = m2;
-        ref = ref2;
-        const float w = vs * (0x1p13f / ref);
-        float sum = 0.0f;
+            for (int i = 0; i < 16; i++) sc[i >> 2][i & 3] = ap_hide(sc[i >> 2][i & 3], hidden, i);
+            vs = hidden != 0xffffu ? vs : 0.0f;
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) mx = fmaxf(mx, sc[i >> 2][i & 3]);
+        mx = ap_max_quarters(mx * f);
+        const float top = ap_max_quarters(ap_power(vs));
+        if (__any(mx > m + kApLate || top > ref)) {
+            const float m2 = fmaxf(m, mx), r2 = fmaxf(ref, top), am = __builtin_amdgcn_exp2f(m - m2), ao = am * (ref / r2);
+            l *= am;
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= ao;
+            m = m2;
+            ref = r2;
+            over = kApUnit / ref;
+        }
+        const float w = vs * over;
         ap_h8 ph[2], pl[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            float x[8];
+            float pr[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float pr = __builtin_amdgcn_exp2f(sc[2 * e + (j >> 2)][j & 3] - m);
-                sum += pr;
-                x[j] = pr * w;
+                pr[j] = __builtin_amdgcn_exp2f(fmaf(sc[2 * e + (j >> 2)][j & 3], f, -m));
+                l += pr[j];
             }
-            ap_split8(x, ph[e], pl[e]);
+            ap_split8w(pr, w, ph[e], pl[e]);
         }
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        l = fmaf(l, am, sum);
 #pragma unroll
         for (int d = 0; d < ND; d++) {
-            if (16 * d >= hd) continue;
             const ap_h8 a = ap_cvt8(vr[d].x, vr[d].y), b = ap_cvt8(vr[d].z, vr[d].w);
-            o[d] *= ao;
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[0], o[d], 0, 0, 0);
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ph[1], o[d], 0, 0, 0);
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[0], o[d], 0, 0, 0);
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, pl[1], o[d], 0, 0, 0);
         }
+        load_values(next, pv_next);
+        pk = page_of(min(next + WAVES, u1 - 1), col >> 2);
+        pv = page_of(min(next + WAVES, u1 - 1), g);
     }
 
-    // join the waves: all lanes of a column hold the same m and l
-    const float back = ref * 0x1p-13f;
+    // join the waves: all lanes of a column hold the same m and parts of l
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const float back = ref * (1.0f / kApUnit);
     if (g == 0) {
         m_lds[wave][col] = m;
         l_lds[wave][col] = l;
     }
 #pragma unroll
     for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) o_lds[wave][col][16 * d + 4 * g + i] = o[d][i] * back;
+        o_lds[wave][4 * d + g][col] = float4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back};
     __syncthreads();
     const int rows = min(16, n_rows - tile * 16);
-    const int64_t item = ((int64_t)r * A.C.n_kv + h) * A.n_tiles + tile;
-    float *part = A.part + (item * A.n_split + split) * 16 * (hd + 2);
-    for (int i = tid; i < rows * hd; i += kApWaves * 64) {
-        const int c = i / hd, d = i % hd;
-        float mm = kApNone;
+    const int64_t item = ((int64_t)r * A.n_tiles + tile) * A.C.n_kv + h;
+    float *part = A.part + ap_part(A, item, split, 16);
+    for (int i = tid; i < 4 * hd; i += WAVES * 64) {
+        // whole rows to out, the sums of a dim for all rows to the splits
+        const int c = n_split == 1 ? i / (hd / 4) : i % 16, d4 = n_split == 1 ? i % (hd / 4) : i / 16;
+        if (c >= rows) continue;
+        float mm = kApNone, ll = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kApWaves; w++) mm = fmaxf(mm, m_lds[w][c]);
-        float ll = 0.0f, oo = 0.0f;
+        for (int w = 0; w < WAVES; w++) mm = fmaxf(mm, m_lds[w][c]);
+        float4 oo = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < kApWaves; w++) {
+        for (int w = 0; w < WAVES; w++) {
             const float e = __builtin_amdgcn_exp2f(m_lds[w][c] - mm);
+            const float4 v = o_lds[w][d4][c];
             ll = fmaf(l_lds[w][c], e, ll);
-            oo = fmaf(o_lds[w][c][d], e, oo);
+            oo = float4{fmaf(v.x, e, oo.x), fmaf(v.y, e, oo.y), fmaf(v.z, e, oo.z), fmaf(v.w, e, oo.w)};
         }
         if (n_split == 1) {
             const int rw = tile * 16 + c;
-            A.out[(s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + d] = ap_quotient(oo, ll);
+            ap_put4(A.out + (s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + 4 * d4, ap_quotient(oo.x, ll),
+                    ap_quotient(oo.y, ll), ap_quotient(oo.z, ll), ap_quotient(oo.w, ll), A.out_vec);
         } else {
-            ap_store(part + c * (hd + 2) + d, oo);
-            if (d == 0) {
-                ap_store(part + c * (hd + 2) + hd, mm);
-                ap_store(part + c * (hd + 2) + hd + 1, ll);
-            }
+            ((float4 *)part)[i] = oo;
+            if (d4 == 0) ((float4 *)part)[4 * hd + c] = float4{mm, ll, 0, 0};
         }
     }
-    if (n_split == 1) return;
-
-    ap_join<kApRows, kApWaves * 64>(A, s, h, tile, item, rows, n_split);
 }
 
 // ---- many rows ---------------------------------------------------------------------
@@ -467,20 +479,54 @@ __global__ __launch_bounds__(kApWaves * 64) void attnp_rows_kernel(AttnPArgs A) 
 // (row c, half e) the scores of keys 32 u + 16 e + i in register i: row m of
 // the operand is key 16 (m / 4 % 2) + 4 (m / 8) + m % 4.
 
-// A row's maximum follows the scores when they pass it by 2^4, so that most
-// chunks leave the sums alone: weights reach 2^4 and are held times 2^9.
-constexpr float kApLate = 4.0f, kApUnit = 0x1p9f;
+// Large row blocks lie in the grid by their number in their request, high
+// ones first, whatever the request: those see the most keys, and a launch that
+// starts them last would end with them alone. Block i of that order: with F(t)
+// = sum over requests of max(0, blocks - t), its number t has F(t + 1) <= i <
+// F(t), and it is the i - F(t + 1)th of the requests with more than t blocks.
+// The lanes try 64 numbers at once; up to 64 kPlaceRegs requests.
+constexpr int kPlaceRegs = 4;
 
-// the power of two below x (x is 0 or more), at least 2^-100
-__device__ inline float ap_power(float x) {
-    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, fmaxf(x, 0x1p-100f)) & 0x7f800000u);
-}
-
-// the larger of lane i's and lane i + 32's
-__device__ inline float ap_max_halves(float x) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, x);
-    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+__device__ inline bool ap_place(const AttnPArgs &A, int rows, int64_t i, int &r, int &tile) {
+    const int lane = threadIdx.x & 63;
+    int blocks[kPlaceRegs];
+#pragma unroll
+    for (int k = 0; k < kPlaceRegs; k++) {
+        const int q = lane + 64 * k;
+        blocks[k] = q < A.n_req ? (min(request_span(A.R, q).n, A.R.max_q) * A.G + rows - 1) / rows : 0;
+    }
+    int lo = 0, span = A.n_tiles;
+    int64_t f = 0;
+    for (;;) {
+        const int step = (span + 63) / 64, t = lo + lane * step;
+        f = 0;
+#pragma unroll
+        for (int k = 0; k < kPlaceRegs; k++)
+            for (int q = 0; q < min(64, A.n_req - 64 * k); q++) f += max(0, __builtin_amdgcn_readlane(blocks[k], q) - t);
+        const int c = __popcll(__ballot(f > i));
+        if (c == 0) return false;  // (of the first round only: past the last block)
+        lo += (c - 1) * step;
+        f = __shfl(f, c - 1);
+        if (step == 1) break;
+        span = step;
+    }
+    int more = 0;
+#pragma unroll
+    for (int k = 0; k < kPlaceRegs; k++) more += __popcll(__ballot(blocks[k] > lo));
+    int rank = (int)(i - (f - more));
+#pragma unroll
+    for (int k = 0; k < kPlaceRegs; k++) {
+        uint64_t has = __ballot(blocks[k] > lo);
+        const int n = __popcll(has);
+        if (rank >= 0 && rank < n) {
+            for (; rank; rank--) has &= has - 1;
+            r = 64 * k + __ffsll((unsigned long long)has) - 1;
+        }
+        rank -= n;
+    }
+    r = __builtin_amdgcn_readfirstlane(r);
+    tile = lo;
+    return true;
 }
 
 // hd rounded up to 16 NS dims
@@ -493,14 +539,18 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
     __shared__ uint4 k_lds[2][64][KC];
     __shared__ uint4 v_lds[2][ND * 32][8];
     __shared__ float s_lds[2][8];
-    const int h = blockIdx.x % A.C.n_kv, tile = A.n_tiles - 1 - blockIdx.x / A.C.n_kv, split = blockIdx.y, r = blockIdx.z;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
+    const int h = blockIdx.x % A.C.n_kv, split = blockIdx.y;
+    const int64_t place = blockIdx.x / A.C.n_kv;
+    int r = blockIdx.z, tile = (int)(A.n_tiles - 1 - place);
+    if (A.placed && !ap_place(A, kApTileRows, place, r, tile)) return;
+    const int64_t item = (A.placed ? place : (int64_t)r * A.n_tiles + tile) * A.C.n_kv + h;
     const Span s = request_span(A.R, r);
     const int n_tok = min(s.n, A.R.max_q), n_rows = n_tok * A.G;
     if (tile * kApTileRows >= n_rows) return;
     const Sight S = ap_sight(A, r, s, tile * kApTileRows / A.G, min((tile * kApTileRows + kApTileRows - 1) / A.G, n_tok - 1));
-    const int n_split = max(1, min(A.n_split, S.n));
+    const int n_split = ap_splits(A, S.n);
     if (split >= n_split) return;
     const int u0 = (int)((int64_t)S.n * split / n_split), u1 = (int)((int64_t)S.n * (split + 1) / n_split);
 
@@ -698,8 +748,6 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
     }
     l += __shfl_xor(l, 32);
 
-    const int64_t item = ((int64_t)r * A.C.n_kv + h) * A.n_tiles + tile;
-    const int rows = min(kApTileRows, n_rows - tile * kApTileRows);
     const float back = ref * (1.0f / kApUnit);
     if (row0 + col < n_rows) {
         // four dims in a row a register group: 32 d + 8 a + 4 half ..
@@ -713,21 +761,56 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
                     if (32 * d + 8 * a < hd) ap_put4(to + 32 * d + 8 * a, o[d][4 * a] * z, o[d][4 * a + 1] * z,
                                 o[d][4 * a + 2] * z, o[d][4 * a + 3] * z, A.out_vec);
         } else {
-            float *to = A.part + ((item * A.n_split + split) * kApTileRows + wave * 32 + col) * (hd + 2);
+            float4 *to = (float4 *)(A.part + ap_part(A, item, split, kApTileRows)) + wave * 32 + col;
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
                 for (int a = 0; a < 4; a++)
                     if (32 * d + 8 * a < hd)
-#pragma unroll
-                        for (int b = 0; b < 4; b++) ap_store(to + 32 * d + 8 * a + 4 * half + b, o[d][4 * a + b] * back);
-            if (half == 0) {
-                ap_store(to + hd, m);
-                ap_store(to + hd + 1, l);
-            }
+                        to[(8 * d + 2 * a + half) * kApTileRows] = float4{o[d][4 * a] * back, o[d][4 * a + 1] * back,
+                                                                          o[d][4 * a + 2] * back, o[d][4 * a + 3] * back};
+            if (half == 0) to[hd / 4 * kApTileRows] = float4{m, l, 0, 0};
         }
     }
-    if (n_split > 1) ap_join<kApTileRows, kApTileThreads>(A, s, h, tile, item, rows, n_split);
+}
+
+// ---- row blocks whose keys were split -----------------------------------------------
+//
+// A second launch adds up a row block's splits, in their order: a thread has
+// four dims of a row. (One workgroup, the last of a block to arrive, would
+// have to read all of it: 66 KB a split for 128 rows of 128 dims.)
+
+constexpr int kApJoinThreads = 256;
+
+template <int ROWS>
+__global__ __launch_bounds__(kApJoinThreads) void attnp_join_kernel(AttnPArgs A) {
+    const int h = blockIdx.x % A.C.n_kv, hd = A.C.hd;
+    const int64_t place = blockIdx.x / A.C.n_kv;
+    int r = blockIdx.z, tile = (int)place;
+    if (A.placed && !ap_place(A, ROWS, place, r, tile)) return;
+    const int64_t item = (A.placed ? place : (int64_t)r * A.n_tiles + tile) * A.C.n_kv + h;
+    const Span s = request_span(A.R, r);
+    const int n_tok = min(s.n, A.R.max_q), n_rows = n_tok * A.G;
+    const int c = threadIdx.x % ROWS, d4 = blockIdx.y * (kApJoinThreads / ROWS) + threadIdx.x / ROWS, row = tile * ROWS + c;
+    if (tile * ROWS >= n_rows) return;
+    const int t0 = tile * ROWS / A.G, t1 = min((tile * ROWS + ROWS - 1) / A.G, n_tok - 1);
+    const int n_split = ap_splits(A, ap_sight(A, r, s, t0, t1).n);
+    if (n_split == 1 || row >= n_rows || 4 * d4 >= hd) return;
+    const float4 *part = (const float4 *)(A.part + ap_part(A, item, 0, ROWS)) + c;
+    const int64_t step = (int64_t)(hd / 4 + 1) * ROWS;
+    float m = kApNone, l = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < n_split; k++) m = fmaxf(m, part[k * step + hd / 4 * ROWS].x);
+    float4 o = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int k = 0; k < n_split; k++) {
+        const float4 ml = part[k * step + hd / 4 * ROWS], v = part[k * step + d4 * ROWS];
+        const float e = __builtin_amdgcn_exp2f(ml.x - m);
+        l = fmaf(ml.y, e, l);
+        o = float4{fmaf(v.x, e, o.x), fmaf(v.y, e, o.y), fmaf(v.z, e, o.z), fmaf(v.w, e, o.w)};
+    }
+    ap_put4(A.out + (s.q0 + row / A.G) * A.ldo + (int64_t)(h * A.G + row % A.G) * hd + 4 * d4, ap_quotient(o.x, l),
+            ap_quotient(o.y, l), ap_quotient(o.z, l), ap_quotient(o.w, l), A.out_vec);
 }
 
 }  // namespace sihip

@@ -171,12 +171,24 @@ extern "C" int sihip_kv_read_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, co
 
 namespace {
 
+constexpr int kApRowWaves = 4;  // of a 16-row block
+
 struct AttnPPlan {
     AttnPArgs A;
     int waves;  // of 32 rows in a large row block, 0: 16-row blocks
-    int64_t items;
-    size_t cnt_bytes, ws_bytes;
+    int64_t blocks, items;  // row blocks, and those times the KV heads
+    int64_t gx;             // of the grid
+    int block_rows;
+    size_t ws_bytes;
 };
+
+// Waves of 32 rows in a row block of the prompt kernel, 0: 16-row blocks.
+int attn_waves(const sihip_ctx *ctx, const AttnPArgs &A, int64_t rows) {
+    const int64_t o = ctx->opt.attnp_waves;
+    if (o == 0 || ((o == 2 || o == 4 || o == 8) && (A.C.hd <= 128 || o == 4))) return (int)o;
+    if (rows <= 32) return 0;
+    return rows <= 1024 || A.C.hd > 128 ? 4 : 8;
+}
 
 int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch *batch, const sihip_attn_paged *a,
               AttnPPlan &P) {
@@ -215,24 +227,29 @@ int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch 
     A.cap = (float)((double)a->softcap * 1.4426950408889634);
     A.cap_in = a->softcap > 0 ? (float)(2.0 * scale / a->softcap * 1.4426950408889634) : 0.0f;
     const int64_t rows = (int64_t)A.R.max_q * A.G;
-    P.waves = rows <= 32 ? 0 : rows <= 1024 || A.C.hd > 128 ? 4 : 8;
+    P.waves = attn_waves(ctx, A, rows);
     const int block_rows = P.waves ? 32 * P.waves : kApRows;
     A.n_tiles = (int)((rows + block_rows - 1) / block_rows);
-    P.items = (int64_t)A.n_req * A.C.n_kv * A.n_tiles;
-    // splits of a row block's keys: until every CU has four workgroups (two of
-    // the large ones), none shorter than a chunk per wave (eight chunks), as
-    // many as have counters
-    const int64_t chunks = ((int64_t)A.R.max_kv + 63) / 64;
-    int64_t n = ((P.waves ? 8 / P.waves : 4) * (int64_t)ctx->n_cu + P.items - 1) / std::max<int64_t>(P.items, 1);
-    n = std::min<int64_t>(n, P.waves ? (chunks + 7) / 8 : (chunks + kApWaves - 1) / kApWaves);
+    // row blocks of all requests: as many as the longest has each, or, listed
+    // (ap_place), no more than the step's rows fill
+    P.blocks = (int64_t)A.n_req * A.n_tiles;
+    A.placed = P.waves && A.n_req <= 64 * kPlaceRegs;
+    if (A.placed) P.blocks = std::min(P.blocks, A.R.n_tok * A.G / block_rows + A.n_req);
+    P.items = P.blocks * A.C.n_kv;
+    // splits of a row block's keys: until every CU has its workgroups, none
+    // shorter than a chunk per wave
+    const int64_t chunks = std::max<int64_t>(1, ((int64_t)A.R.max_kv + 63) / 64);
+    const int64_t per_cu = P.waves ? std::max(1, 8 / P.waves) : 4, least = P.waves ? 4 : kApRowWaves;
+    int64_t n = (per_cu * ctx->n_cu + P.items - 1) / std::max<int64_t>(P.items, 1);
+    if (ctx->opt.attnp_splits > 0) n = ctx->opt.attnp_splits;
     n = std::max<int64_t>(1, std::min<int64_t>(n, 64));
-    if (P.items > kGemmCounters) n = 1;
-    A.n_split = (int)n;
-    P.cnt_bytes = n > 1 ? ((size_t)P.items * 4 + 255) / 256 * 256 : 0;
-    P.ws_bytes = n > 1 ? (size_t)P.items * n * block_rows * (A.C.hd + 2) * 4 : 0;
+    A.per_split = (int)std::max<int64_t>((chunks + n - 1) / n, ctx->opt.attnp_splits > 0 ? 1 : least);
+    A.n_split = (int)((chunks + A.per_split - 1) / A.per_split);
+    P.block_rows = block_rows;
+    P.ws_bytes = A.n_split > 1 ? (size_t)P.items * A.n_split * block_rows * (A.C.hd / 4 + 1) * 16 : 0;
     A.part = nullptr;
-    A.cnt = nullptr;
-    if ((int64_t)A.n_tiles * (P.waves ? A.C.n_kv : n) * 512 > UINT32_MAX)
+    P.gx = P.waves ? (A.placed ? P.blocks : A.n_tiles) * A.C.n_kv : A.n_tiles * A.n_split;
+    if (P.gx * 512 > UINT32_MAX)
         return set_err(ctx, SIHIP_EINVAL, "%s: max_q %d of %lld heads has no grid", fn, A.R.max_q,
                        (long long)a->n_head);
     return SIHIP_OK;
@@ -246,7 +263,7 @@ extern "C" int sihip_attn_paged_workspace(sihip_ctx *ctx, const sihip_kv_cache *
     AttnPPlan P;
     const int rc = plan_attn(ctx, cache, batch, args, P);
     if (rc) return rc;
-    *bytes = P.cnt_bytes + P.ws_bytes;
+    *bytes = P.ws_bytes;
     return SIHIP_OK;
 }
 
@@ -260,13 +277,7 @@ extern "C" int sihip_attn_paged_dev(sihip_ctx *ctx, const sihip_kv_cache *cache,
     const OnDevice on(ctx->device);
     const hipStream_t st = (hipStream_t)stream;
     const bool shared = A.n_split > 1 && !args->workspace;
-    if (A.n_split > 1 && args->workspace) {
-        if (args->workspace_bytes < P.cnt_bytes + P.ws_bytes || !aligned(args->workspace, 256))
-            return set_err(ctx, SIHIP_EINVAL, "attn_paged_dev: a workspace of %zu bytes, 256-byte aligned, is needed",
-                           P.cnt_bytes + P.ws_bytes);
-        A.cnt = (uint32_t *)args->workspace;
-        A.part = (float *)((uint8_t *)args->workspace + P.cnt_bytes);
-    } else if (shared) {
+    if (shared) {
         try {
             rc = ensure(ctx, &ctx->d_attn, &ctx->d_attn_cap, P.ws_bytes, st);
         } catch (...) {
@@ -274,14 +285,19 @@ extern "C" int sihip_attn_paged_dev(sihip_ctx *ctx, const sihip_kv_cache *cache,
         }
         if (!rc) rc = order_before(ctx, ctx->order, st);
         if (rc) return rc;
-        A.cnt = ctx->d_gcnt;
         A.part = (float *)ctx->d_attn;
+    } else if (A.n_split > 1) {
+        if (args->workspace_bytes < P.ws_bytes || !aligned(args->workspace, 16))
+            return set_err(ctx, SIHIP_EINVAL, "attn_paged_dev: a workspace of %zu bytes, 16-byte aligned, is needed",
+                           P.ws_bytes);
+        A.part = (float *)args->workspace;
     }
     const int hd = A.C.hd;
     if (P.waves) {
-        const dim3 grid((unsigned)(A.n_tiles * A.C.n_kv), (unsigned)A.n_split, (unsigned)A.n_req), t(P.waves * 64);
+        const dim3 grid((unsigned)P.gx, (unsigned)A.n_split, A.placed ? 1u : (unsigned)A.n_req), t(P.waves * 64);
 #define SIHIP_APT(NS)                                                                         \
-    if (P.waves == 4) hipLaunchKernelGGL((attnp_tiles_kernel<NS, 4>), grid, t, 0, st, A);     \
+    if (P.waves == 2) hipLaunchKernelGGL((attnp_tiles_kernel<NS, 2>), grid, t, 0, st, A);     \
+    else if (P.waves == 4) hipLaunchKernelGGL((attnp_tiles_kernel<NS, 4>), grid, t, 0, st, A); \
     else hipLaunchKernelGGL((attnp_tiles_kernel<NS, 8>), grid, t, 0, st, A);
         if (hd <= 64) { SIHIP_APT(4) }
         else if (hd <= 96) { SIHIP_APT(6) }
@@ -290,11 +306,22 @@ extern "C" int sihip_attn_paged_dev(sihip_ctx *ctx, const sihip_kv_cache *cache,
         else hipLaunchKernelGGL((attnp_tiles_kernel<16, 4>), grid, t, 0, st, A);
 #undef SIHIP_APT
     } else {
-        const dim3 grid((unsigned)(A.n_tiles * A.n_split), (unsigned)A.C.n_kv, (unsigned)A.n_req), t(kApWaves * 64);
-        if (hd <= 64) hipLaunchKernelGGL(attnp_rows_kernel<1>, grid, t, 0, st, A);
-        else if (hd <= 128) hipLaunchKernelGGL(attnp_rows_kernel<2>, grid, t, 0, st, A);
-        else if (hd <= 192) hipLaunchKernelGGL(attnp_rows_kernel<3>, grid, t, 0, st, A);
-        else hipLaunchKernelGGL(attnp_rows_kernel<4>, grid, t, 0, st, A);
+        const dim3 grid((unsigned)P.gx, (unsigned)A.C.n_kv, (unsigned)A.n_req), t(kApRowWaves * 64);
+        if (hd <= 64) hipLaunchKernelGGL((attnp_rows_kernel<1, kApRowWaves>), grid, t, 0, st, A);
+        else if (hd <= 128) hipLaunchKernelGGL((attnp_rows_kernel<2, kApRowWaves>), grid, t, 0, st, A);
+        else if (hd <= 192) hipLaunchKernelGGL((attnp_rows_kernel<3, kApRowWaves>), grid, t, 0, st, A);
+        else hipLaunchKernelGGL((attnp_rows_kernel<4, kApRowWaves>), grid, t, 0, st, A);
+    }
+    if (A.n_split > 1) {
+        const int per_wg = kApJoinThreads / P.block_rows;  // four-dim columns
+        const dim3 grid((unsigned)((A.placed ? P.blocks : A.n_tiles) * A.C.n_kv), (unsigned)((hd / 4 + per_wg - 1) / per_wg),
+                        A.placed ? 1u : (unsigned)A.n_req), t(kApJoinThreads);
+        switch (P.block_rows) {
+            case kApRows: hipLaunchKernelGGL(attnp_join_kernel<kApRows>, grid, t, 0, st, A); break;
+            case 64: hipLaunchKernelGGL(attnp_join_kernel<64>, grid, t, 0, st, A); break;
+            case 128: hipLaunchKernelGGL(attnp_join_kernel<128>, grid, t, 0, st, A); break;
+            default: hipLaunchKernelGGL(attnp_join_kernel<256>, grid, t, 0, st, A); break;
+        }
     }
     rc = launched(ctx, "attn_paged");
     if (rc) return rc;

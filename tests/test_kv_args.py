@@ -110,7 +110,7 @@ if what == "capture":
     fake.fake_capture(1)
     result = [n, first, said(dev.attn_paged_dev, c, b, a, 5)]
 else:
-    size, at = dict(small=(n - 1, X), exact=(n, X), aligned=(n + 512, X + 16))[what]
+    size, at = dict(small=(n - 1, X), exact=(n, X), aligned=(n + 512, X + 8))[what]
     result = [n, said(dev.attn_paged_dev, c, b, attn(workspace=at, workspace_bytes=size))]
 """)
     assert got[0] > 0
