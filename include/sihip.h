@@ -331,8 +331,9 @@ int sihip_kv_read_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const int64_t
  * (22 bits of q and of the probabilities), sums are f32; results do not
  * depend on the order in which workgroups run.
  * workspace: NULL, or device memory of sihip_attn_paged_workspace bytes
- * (16-byte aligned, its contents do not matter) of their own for calls that
- * may overlap other work of the context, on other streams or in graphs.
+ * (16-byte aligned) of its own for calls that may overlap other work of the
+ * context, on other streams or in graphs: zeroed once, before its first use,
+ * then left to calls of any size that do not overlap each other.
  * With NULL the context's own is used: eager calls are ordered by the
  * library; a graph that was captured with it must not run beside other work
  * of the context. */

@@ -27,6 +27,9 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
+#include "agent.h"
 #include "kvcache.h"
 
 namespace sihip {
@@ -44,14 +47,18 @@ struct AttnPArgs {
     float *out;
     int64_t ldq, ldo;
     int n_req, G, window;
-    bool out_vec;    // rows of out and their heads are 16-byte aligned
+    bool q_vec, out_vec;  // rows of q or out and their heads are 16-byte aligned
     float sign;      // of kq_scale: queries are multiplied by it,
     float scale2;    // |kq_scale| * log2 e, so that factors of scores are not negative
     float cap, cap_in;  // softcap * log2 e (0: none), 2 |kq_scale| / softcap * log2 e
     int n_tiles;     // most row blocks of a request
     int n_split, per_split;  // most splits of a row block's keys, least chunks of one
-    int placed;      // large row blocks: 1 if the grid is their list (ap_place)
-    float *part;     // [item][split][hd / 4 + 1][rows] of four: sums by dims, then m, l
+    int whole;       // chunks that are not split
+    int slots;       // placed 16-row blocks: workgroups that share the chunks of all
+    int chunk;       // log2 of the keys of a chunk
+    int placed;      // 1: the grid is a list made on the device (ap_place, ap_deal)
+    float *part;     // [piece][hd / 4 + 1][rows] of four: sums by dims, then m, l
+    uint32_t *cnt;   // 16-row blocks: pieces that have arrived, zero between launches
 };
 
 constexpr float kApNone = -3.4e38f;  // running maximum before any key
@@ -99,10 +106,22 @@ __device__ inline void ap_split8w(const float *p, float w, ap_h8 &hi, ap_h8 &lo)
     for (int j = 0; j < 8; j++) lo[j] = (_Float16)fmaf(p[j], w, -(float)hi[j]);
 }
 
+// eight values of a query row; wide: rows of q and their heads are 16-byte aligned
+__device__ inline void ap_load8(const float *q, bool wide, float *x) {
+    if (wide) {
+        const float4 a = ((const float4 *)q)[0], b = ((const float4 *)q)[1];
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+        x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = q[j];
+    }
+}
+
 // What a block of rows of one request sees: positions p_lo .. p_hi of its
 // first and last row, the keys [0, keys), of which the first `prefix` are
-// visible to every row. In 64-key chunks: chunks [0, np) hold the prefix,
-// [c0, c1) the rest; chunk u of n is u < np ? u : u - np + c0.
+// visible to every row. In chunks: [0, np) hold the prefix, [c0, c1) the rest;
+// chunk u of n is u < np ? u : u - np + c0.
 struct Sight {
     int p_lo, p_hi, keys, prefix, np, c0, n;
 };
@@ -115,17 +134,18 @@ __device__ inline Sight ap_sight(const AttnPArgs &A, int r, const Span &s, int t
     g.prefix = A.prefix ? max(0, min(A.prefix[r], g.keys)) : 0;
     const int end = min(max(g.p_hi + 1, g.prefix), g.keys);
     const int start = A.window ? max(0, g.p_lo - A.window + 1) : 0;
-    g.np = A.window ? (g.prefix + 63) / 64 : 0;
-    g.c0 = max(start / 64, g.np);
-    g.n = g.np + max(0, (end + 63) / 64 - g.c0);
+    const int up = (1 << A.chunk) - 1;
+    g.np = A.window ? (g.prefix + up) >> A.chunk : 0;
+    g.c0 = max(start >> A.chunk, g.np);
+    g.n = g.np + max(0, ((end + up) >> A.chunk) - g.c0);
     return g;
 }
 
 __device__ inline int ap_chunk(const Sight &g, int u) { return u < g.np ? u : u - g.np + g.c0; }
 
-// whether every row of the block sees all 64 keys of chunk c
-__device__ inline bool ap_whole(const AttnPArgs &A, const Sight &g, int c) {
-    const int j0 = c * 64, j1 = j0 + 63;
+// whether every row of the block sees the n keys from j0 on
+__device__ inline bool ap_whole(const AttnPArgs &A, const Sight &g, int j0, int n) {
+    const int j1 = j0 + n - 1;
     if (j1 >= g.keys) return false;
     return j1 < g.prefix || (j1 <= g.p_lo && (!A.window || j0 > g.p_hi - A.window));
 }
@@ -194,14 +214,32 @@ __device__ inline void ap_put4(float *p, float a, float b, float c, float d, boo
     }
 }
 
-// Splits of a row block with n chunks.
-__device__ inline int ap_splits(const AttnPArgs &A, int n) {
-    return max(1, min(A.n_split, (n + A.per_split - 1) / A.per_split));
+// Splits of a row block with n chunks, in pieces of `per`.
+__device__ inline int ap_splits(const AttnPArgs &A, int n, int per) {
+    return n <= max(per, A.whole) ? 1 : min(A.n_split, (n + per - 1) / per);
 }
 
-// Sums, maximum and total of a row's split, in four-byte units of A.part
-__device__ inline int64_t ap_part(const AttnPArgs &A, int64_t item, int split, int rows) {
-    return (item * A.n_split + split) * (A.C.hd / 4 + 1) * rows * 4;
+// Sums, maxima and totals of a piece (a row block's split)
+__device__ inline float4 *ap_part(const AttnPArgs &A, int64_t piece, int rows) {
+    return (float4 *)A.part + piece * (A.C.hd / 4 + 1) * rows;
+}
+
+// Adds up to 16 pieces' totals (ml: maximum, total) and sums to those of the
+// pieces before them.
+__device__ inline void ap_add16(int n, const float4 *ml, const float4 *v, float &m, float &l, float4 &o) {
+    float m2 = m;
+#pragma unroll
+    for (int k = 0; k < 16; k++) m2 = fmaxf(m2, ml[k].x);
+    const float a = __builtin_amdgcn_exp2f(m - m2);
+    l *= a;
+    o = float4{o.x * a, o.y * a, o.z * a, o.w * a};
+    m = m2;
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const float e = k < n ? __builtin_amdgcn_exp2f(ml[k].x - m) : 0.0f;
+        l = fmaf(ml[k].y, e, l);
+        o = float4{fmaf(v[k].x, e, o.x), fmaf(v[k].y, e, o.y), fmaf(v[k].z, e, o.z), fmaf(v[k].w, e, o.w)};
+    }
 }
 
 // the power of two below x (x is 0 or more), at least 2^-100
@@ -230,41 +268,214 @@ constexpr float kApLate = 4.0f, kApUnit = 0x1p9f;
 // ---- few rows ----------------------------------------------------------------------
 //
 // One workgroup: 16 rows of one request and KV head, one split of its
-// chunks; the waves take chunks in turn and join through LDS at the end.
-// Nothing is staged: a lane loads 16 bytes of a key row (key tile t, row m
-// of the matrix operand is token 16 (m / 4) + 4 t + m % 4) and 16 tokens of a
-// value row, converts them in registers and feeds the matrix cores. The next
-// chunk's keys are loaded once this one's are converted, its values after
-// this one's, so that each has half an iteration to arrive and two waves of a
-// SIMD keep the memory busy.
+// chunks; its waves take chunks in turn and join through LDS at the end.
+// Nothing is staged: a lane loads 16 bytes of a key row and 4 TT tokens of a
+// value row, converts them in registers and feeds the matrix cores. A chunk is
+// TT tiles of 16 keys: row m of key tile t is token 4 TT (m / 4) + 4 t + m % 4,
+// so that a lane's scores are of 4 TT tokens in a row. The next chunk's keys
+// are loaded once this one's are converted, its values after this one's:
+// each has half an iteration to arrive, and two waves of a SIMD keep the memory
+// busy. (Wide heads take half the keys a chunk, so that two waves fit.)
 
 constexpr int kApRows = 16;
+constexpr int kPlaceRegs = 4;  // requests a lane keeps in ap_deal and ap_place
+
+// The pieces of a ragged batch. The host knows bounds on the lengths only, so
+// the device deals: all chunks of all row blocks over the slots give the length
+// of a piece, a row block has as many as it needs, and the grid, slots plus row
+// blocks, holds them all. Every wave does the same sums over the requests, 64 at
+// a time. (Grids of the longest request's splits for everybody started
+// workgroups without work, 4 us each.)
+struct Deal {
+    int per;                 // chunks of a piece
+    Span s[kPlaceRegs];      // of request lane + 64 k: its tokens,
+    int n[kPlaceRegs];       // chunks,
+    int last[kPlaceRegs];    // and the pieces up to and with it
+
+    __device__ int splits(const AttnPArgs &A, int n) const { return n <= max(per, A.whole) ? 1 : (n + per - 1) / per; }
+};
+
+// x of this lane and all before it
+template <class T>
+__device__ inline T ap_scan(T x) {
+    static_assert(sizeof(T) == 4, "one register");
+    auto from = [&](auto ctrl, int rows) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, false) & rows);
+    };
+    const int lane = threadIdx.x & 63, in_row = lane & 15;
+    // shifts by 1, 2, 4 and 8 within rows of 16, then lanes 15 and 31 to the rows behind them
+    x += from(std::integral_constant<int, 0x111>(), in_row >= 1 ? -1 : 0);
+    x += from(std::integral_constant<int, 0x112>(), in_row >= 2 ? -1 : 0);
+    x += from(std::integral_constant<int, 0x114>(), in_row >= 4 ? -1 : 0);
+    x += from(std::integral_constant<int, 0x118>(), in_row >= 8 ? -1 : 0);
+    x += from(std::integral_constant<int, 0x142>(), lane & 16 ? -1 : 0);
+    x += from(std::integral_constant<int, 0x143>(), lane & 32 ? -1 : 0);
+    return x;
+}
+
+__device__ inline Deal ap_deal(const AttnPArgs &A) {
+    const int lane = threadIdx.x & 63;
+    Deal D;
+    int tiles[kPlaceRegs];
+    float all = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kPlaceRegs; k++) {
+        const int r = lane + 64 * k;
+        D.n[k] = tiles[k] = 0;
+        D.s[k] = Span{0, 0, 0, 0};
+        if (r < A.n_req) {
+            D.s[k] = request_span(A.R, r);
+            const int n = min(D.s[k].n, A.R.max_q);
+            if (n > 0) {
+                tiles[k] = (n * A.G + kApRows - 1) / kApRows;
+                D.n[k] = ap_sight(A, r, D.s[k], 0, n - 1).n;
+            }
+        }
+        all += (float)tiles[k] * (float)(A.C.n_kv * D.n[k]);
+    }
+    // rounded up by more than the sum can be off: a piece too long by that is
+    // harmless, one too short would make more pieces than the grid has
+    all = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ap_scan(all)), 63));
+    D.per = max(A.per_split, (int)fminf(ceilf(all * 1.0001f / (float)A.slots), 0x1p30f));
+    int before = 0;
+#pragma unroll
+    for (int k = 0; k < kPlaceRegs; k++) {
+        D.last[k] = tiles[k] * A.C.n_kv * D.splits(A, D.n[k]);
+        if (64 * k < A.n_req) D.last[k] = ap_scan(D.last[k]);
+        D.last[k] += before;
+        before = __builtin_amdgcn_readlane(D.last[k], 63);
+    }
+    return D;
+}
+
+// pieces before request r's, its chunks and its tokens
+__device__ inline int ap_dealt(const Deal &D, int r, int &n, Span &s) {
+    int before = 0;
+#pragma unroll
+    for (int k = 0; k < kPlaceRegs; k++) {
+        if (r >= 64 * k && r < 64 * k + 64) {
+            const int l = r - 64 * k;
+            n = __builtin_amdgcn_readlane(D.n[k], l);
+            s.q0 = __builtin_amdgcn_readlane((int)D.s[k].q0, l);  // (a row of at most 2^31)
+            s.n = __builtin_amdgcn_readlane(D.s[k].n, l);
+            s.p0 = __builtin_amdgcn_readlane(D.s[k].p0, l);
+            s.end = __builtin_amdgcn_readlane(D.s[k].end, l);
+            if (l > 0) before = __builtin_amdgcn_readlane(D.last[k], l - 1);
+        } else if (r >= 64 * k + 64) {
+            before = __builtin_amdgcn_readlane(D.last[k], 63);
+        }
+    }
+    return before;
+}
+
+// the request that piece i belongs to, or -1
+__device__ inline int ap_dealt_to(const Deal &D, int i) {
+    int r = -1;
+#pragma unroll
+    for (int k = kPlaceRegs - 1; k >= 0; k--) {
+        const uint64_t past = __ballot(D.last[k] > i);
+        if (past) r = 64 * k + __ffsll((unsigned long long)past) - 1;
+    }
+    return r;
+}
+
+// four values at agent scope (agent.h)
+__device__ inline void ap_store4(__amdgpu_buffer_rsrc_t r, uint32_t at, float4 v) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), r, (int)(at * 16), 0, 16);
+}
+__device__ inline float4 ap_fetch4(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    return __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(at * 16), 0, 16));
+}
+__device__ inline __amdgpu_buffer_rsrc_t ap_pieces(const AttnPArgs &A, int64_t piece, int n) {
+    return __builtin_amdgcn_make_buffer_rsrc(ap_part(A, piece, kApRows), (short)0, n * (A.C.hd / 4 + 1) * kApRows * 16, 0x00020000);
+}
+
+// The end of a 16-row block whose keys were split over n pieces, after each
+// workgroup has stored its own at agent scope (agent.h says what the order
+// rests on): the last to arrive adds them up in the order of the splits, so
+// that the result does not depend on the order of arrival, and leaves the counter
+// zero. (A second launch took 10 to 20 us: most of its workgroups had nothing to
+// join, and each had to find that out.)
+template <int THREADS>
+__device__ inline void ap_join_rows(const AttnPArgs &A, const Span &s, int h, int tile, int rows, int64_t first, int n) {
+    __shared__ uint32_t last;
+    const int tid = threadIdx.x, hd = A.C.hd;
+    uint32_t *cnt = A.cnt + first;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (tid == 0) last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)n - 1;
+    __syncthreads();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    if (!last) return;
+    const __amdgpu_buffer_rsrc_t part = ap_pieces(A, first, n);
+    const uint32_t step = (hd / 4 + 1) * kApRows;
+    for (int i = tid; i < rows * (hd / 4); i += THREADS) {
+        const int c = i % rows, d4 = i / rows;
+        float m = kApNone, l = 0.0f;
+        float4 o = {0, 0, 0, 0};
+        for (int k0 = 0; k0 < n; k0 += 16) {
+            float4 ml[16], v[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const uint32_t at = min(k0 + k, n - 1) * step + c;
+                ml[k] = ap_fetch4(part, at + hd / 4 * kApRows);
+                v[k] = ap_fetch4(part, at + d4 * kApRows);
+            }
+            ap_add16(n - k0, ml, v, m, l, o);
+        }
+        const int rw = tile * kApRows + c;
+        ap_put4(A.out + (s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + 4 * d4, ap_quotient(o.x, l),
+                ap_quotient(o.y, l), ap_quotient(o.z, l), ap_quotient(o.w, l), A.out_vec);
+    }
+    if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 
 // hd rounded up to 64 NK dims
-template <int NK, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, NK <= 2 ? 2 : 1) void attnp_rows_kernel(AttnPArgs A) {
+template <int NK, int TT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) {
     constexpr int ND = NK * 4;  // 16-dim tiles
-    __shared__ float4 o_lds[WAVES][ND * 4][17];
-    __shared__ float m_lds[WAVES][16], l_lds[WAVES][16];
-    const int r = blockIdx.z, h = blockIdx.y;
-    const int tile = blockIdx.x / A.n_split, split = blockIdx.x % A.n_split;
+    constexpr int CH = 16 * TT, SEG = 4 * TT;
+    constexpr uint32_t kAll = (1u << SEG) - 1;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
-    const Span s = request_span(A.R, r);
+    int r = blockIdx.z, h = blockIdx.y, tile, split, per = A.per_split;
+    int64_t piece;
+    Span s;
+    if (A.placed) {
+        const Deal D = ap_deal(A);
+        const int i = blockIdx.x;
+        r = ap_dealt_to(D, i);
+        if (r < 0) return;
+        int n;
+        const int before = ap_dealt(D, r, n, s), parts = D.splits(A, n);
+        split = (i - before) % parts;
+        h = (i - before) / parts % A.C.n_kv;
+        tile = (i - before) / parts / A.C.n_kv;
+        per = D.per;
+        piece = i;
+    } else {
+        s = request_span(A.R, r);
+        // workgroups go to the eight XCDs in turn, and of a ragged batch only the
+        // low splits have work: turned by request and head they reach all XCDs
+        tile = blockIdx.x / A.n_split;
+        split = (blockIdx.x % A.n_split + h + r) % A.n_split;
+        piece = (((int64_t)r * A.n_tiles + tile) * A.C.n_kv + h) * A.n_split + split;
+    }
+    const int32_t *table = A.R.table + (int64_t)r * A.R.max_blocks;
     const int n_tok = min(s.n, A.R.max_q), n_rows = n_tok * A.G;
     if (tile * 16 >= n_rows) return;
     const int t0 = tile * 16 / A.G, t1 = min((tile * 16 + 15) / A.G, n_tok - 1);
     const Sight S = ap_sight(A, r, s, t0, t1);
-    const int n_split = ap_splits(A, S.n);
+    const int n_split = ap_splits(A, S.n, per);
     if (split >= n_split) return;
-    const int u0 = (int)((int64_t)S.n * split / n_split), u1 = (int)((int64_t)S.n * (split + 1) / n_split);
+    const int u0 = split * per, u1 = split == n_split - 1 ? S.n : u0 + per;
 
-    // pages of a chunk's 16-token segments: of this lane's key rows (segment
-    // col / 4), and of its values and scores (segment g)
-    const int32_t *table = A.R.table + (int64_t)r * A.R.max_blocks;
+    // pages of this lane's key rows, and of its values and scores
     const int last_block = max(S.keys - 1, 0) >> shift, n_pages = (int)A.C.n_pages;
     auto page_of = [&](int u, int seg) {
-        const int j = ap_chunk(S, u) * 64 + seg * 16, pg = table[min(j >> shift, last_block)];
+        const int j = ap_chunk(S, u) * CH + seg * SEG, pg = table[min(j >> shift, last_block)];
         return j < S.keys && pg >= 0 && pg < n_pages ? pg : -1;
     };
     int u = u0 + wave, pk = 0, pv = 0;
@@ -279,18 +490,67 @@ __global__ __launch_bounds__(WAVES * 64, NK <= 2 ? 2 : 1) void attnp_rows_kernel
     const int p = s.p0 + tok;
     const float slope = A.slopes ? A.slopes[head] * kLog2e : 0.0f;
     const float *qrow = A.q + (s.q0 + tok) * A.ldq + (int64_t)head * hd;
+    float x[NK][2][8];
+#pragma unroll
+    for (int c = 0; c < NK; c++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) ap_load8(qrow + (64 * c + 16 * g < hd ? 64 * c + 16 * g : 0) + 8 * e, A.q_vec, x[c][e]);
+
+    // a chunk starts at a multiple of its length: a lane's place in a page is
+    // its own and, in longer pages, the chunk's
+    const uint32_t head_bytes = (uint32_t)hd << shift, page_bytes = head_bytes * (uint32_t)A.C.n_kv;
+    const int8_t *kb = A.C.k + h * (int64_t)head_bytes + (((col >> 2) * SEG & (B - 1)) + (col & 3)) * hd;
+    const int8_t *vb = A.C.v + h * (int64_t)head_bytes + (col << shift) + (g * SEG & (B - 1));
+    int dim[NK];  // this lane's dims of a key row; those past hd meet zeros of q
+#pragma unroll
+    for (int e = 0; e < NK; e++) dim[e] = 64 * e + 16 * g < hd ? 64 * e + 16 * g : 0;
+    uint4 kr[TT][NK];
+    uint32_t vr[ND][TT];
+    float ksc = 0.0f, vsc = 0.0f;
+    auto load_keys = [&](int u) {
+        const int8_t *kp = kb + ((uint64_t)(uint32_t)max(pk, 0) * page_bytes + (ap_chunk(S, u) * CH & (B - 1)) * hd);
+#pragma unroll
+        for (int t = 0; t < TT; t++)
+#pragma unroll
+            for (int e = 0; e < NK; e++) kr[t][e] = *(const uint4 *)(kp + (4 * t * hd + dim[e]));
+        const int64_t at = (int64_t)max(pv, 0) * A.C.n_kv + h;
+        ksc = A.C.ks[at];
+        vsc = pv < 0 ? -1.0f : A.C.vs[at];  // -1: no page
+    };
+    auto load_values = [&](int u, int page) {
+        const int8_t *vp = vb + ((uint64_t)(uint32_t)max(page, 0) * page_bytes + (ap_chunk(S, u) * CH & (B - 1)));
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            const int8_t *at = vp + (min(16 * d, hd - 16) << shift);
+            if constexpr (TT == 4) {
+                const uint4 v = *(const uint4 *)at;
+                vr[d][0] = v.x, vr[d][1] = v.y, vr[d][2] = v.z, vr[d][3] = v.w;
+            } else {
+                const uint2 v = *(const uint2 *)at;
+                vr[d][0] = v.x, vr[d][1] = v.y;
+            }
+        }
+    };
+    if (u < u1) {
+        load_keys(u);
+        load_values(u, pv);
+        const int next = min(u + WAVES, u1 - 1);
+        pk = page_of(next, col >> 2);
+        pv = page_of(next, g);
+    }
+
+    // the query, while the first keys are on their way
     ap_h8 qh[NK][2], ql[NK][2];
-    float f_row;
+    float f_row, fc_row;
     {
-        float x[NK][2][8], amax = 0.0f;
+        float amax = 0.0f;
 #pragma unroll
         for (int c = 0; c < NK; c++)
 #pragma unroll
             for (int e = 0; e < 2; e++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const int d = 64 * c + 16 * g + 8 * e + j;
-                    x[c][e][j] = d < hd ? qrow[d] * A.sign : 0.0f;
+                    x[c][e][j] = 64 * c + 16 * g < hd ? x[c][e][j] * A.sign : 0.0f;
                     amax = fmaxf(amax, fabsf(x[c][e][j]));
                 }
         const int e2 = ap_row_exponent(ap_max_quarters(amax));
@@ -303,56 +563,22 @@ __global__ __launch_bounds__(WAVES * 64, NK <= 2 ? 2 : 1) void attnp_rows_kernel
                 ap_split8(x[c][e], qh[c][e], ql[c][e]);
             }
         f_row = ldexpf(1.0f, -e2);
+        fc_row = f_row * A.cap_in;
+        f_row *= A.scale2;
     }
-    const float fc_row = f_row * A.cap_in;
-    f_row *= A.scale2;
-
     float m = kApNone, l = 0.0f, ref = 0.0f, over = 0.0f;
     ap_f4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = ap_f4{0, 0, 0, 0};
-    // a chunk starts at a multiple of 64: a lane's place in a page is its own
-    // and, in pages of more than 64, the chunk's
-    const uint32_t head_bytes = (uint32_t)hd << shift, page_bytes = head_bytes * (uint32_t)A.C.n_kv;
-    const int8_t *kb = A.C.k + h * (int64_t)head_bytes + (((col >> 2) * 16 & (B - 1)) + (col & 3)) * hd;
-    const int8_t *vb = A.C.v + h * (int64_t)head_bytes + (col << shift) + (g * 16 & (B - 1));
-    int dim[NK];  // this lane's dims of a key row; those past hd meet zeros of q
-#pragma unroll
-    for (int e = 0; e < NK; e++) dim[e] = 64 * e + 16 * g < hd ? 64 * e + 16 * g : 0;
-    uint4 kr[4][NK], vr[ND];
-    float ksc = 0.0f, vsc = 0.0f;
-    auto load_keys = [&](int u) {
-        const int8_t *kp = kb + ((uint64_t)(uint32_t)max(pk, 0) * page_bytes + (ap_chunk(S, u) * 64 & (B - 1)) * hd);
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int e = 0; e < NK; e++) kr[t][e] = *(const uint4 *)(kp + (4 * t * hd + dim[e]));
-        const int64_t at = (int64_t)max(pv, 0) * A.C.n_kv + h;
-        ksc = A.C.ks[at];
-        vsc = pv < 0 ? -1.0f : A.C.vs[at];  // -1: no page
-    };
-    auto load_values = [&](int u, int page) {
-        const int8_t *vp = vb + ((uint64_t)(uint32_t)max(page, 0) * page_bytes + (ap_chunk(S, u) * 64 & (B - 1)));
-#pragma unroll
-        for (int d = 0; d < ND; d++) vr[d] = *(const uint4 *)(vp + ((min(16 * d, hd - 16)) << shift));
-    };
-    int pv_next = 0;
-    if (u < u1) {
-        load_keys(u);
-        load_values(u, pv);
-        const int next = min(u + WAVES, u1 - 1);
-        pk = page_of(next, col >> 2);
-        pv = page_of(next, g);
-    }
     for (; u < u1; u += WAVES) {
         const int next = min(u + WAVES, u1 - 1), c = ap_chunk(S, u);
-        ap_f4 sc[4];
+        ap_f4 sc[TT];
 #pragma unroll
-        for (int t = 0; t < 4; t++) sc[t] = ap_f4{0, 0, 0, 0};
+        for (int t = 0; t < TT; t++) sc[t] = ap_f4{0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < NK; e++)
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
+            for (int t = 0; t < TT; t++) {
                 const ap_h8 a = ap_cvt8(kr[t][e].x, kr[t][e].y), b = ap_cvt8(kr[t][e].z, kr[t][e].w);
                 sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[e][0], sc[t], 0, 0, 0);
                 sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[e][1], sc[t], 0, 0, 0);
@@ -361,31 +587,31 @@ __global__ __launch_bounds__(WAVES * 64, NK <= 2 ? 2 : 1) void attnp_rows_kernel
             }
         // scores in log2 units are sc * f; the factor is kept above zero, so
         // that it leaves -inf as it is, and is a number where no key is seen
-        const int j0 = c * 64 + g * 16;  // key of register (t, i): j0 + 4 t + i
+        const int j0 = c * CH + g * SEG;  // key of register (t, i): j0 + 4 t + i
         float f = fmaxf(f_row * ksc, 0x1p-120f), vs = vsc;
         const float fc = fc_row * ksc;
+        const int pv_next = pv;
         load_keys(next);
-        pv_next = pv;
         if (A.cap != 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) sc[i >> 2][i & 3] = ap_capped(A, sc[i >> 2][i & 3] * f, sc[i >> 2][i & 3] * fc);
+            for (int i = 0; i < SEG; i++) sc[i >> 2][i & 3] = ap_capped(A, sc[i >> 2][i & 3] * f, sc[i >> 2][i & 3] * fc);
             f = 1.0f;
         }
         if (A.slopes) {
             const float far = (float)(j0 - p);
 #pragma unroll
-            for (int i = 0; i < 16; i++) sc[i >> 2][i & 3] = fmaf(sc[i >> 2][i & 3], f, -slope * fabsf(far + (float)i));
+            for (int i = 0; i < SEG; i++) sc[i >> 2][i & 3] = fmaf(sc[i >> 2][i & 3], f, -slope * fabsf(far + (float)i));
             f = 1.0f;
         }
-        if (!ap_whole(A, S, c) || __any(vs < 0.0f)) {
-            const uint32_t hidden = vs < 0.0f ? 0xffffu : ap_hidden(A, S, p, j0);
+        if (!ap_whole(A, S, c * CH, CH) || __any(vs < 0.0f)) {
+            const uint32_t hidden = vs < 0.0f ? kAll : ap_hidden(A, S, p, j0) & kAll;
 #pragma unroll
-            for (int i = 0; i < 16; i++) sc[i >> 2][i & 3] = ap_hide(sc[i >> 2][i & 3], hidden, i);
-            vs = hidden != 0xffffu ? vs : 0.0f;
+            for (int i = 0; i < SEG; i++) sc[i >> 2][i & 3] = ap_hide(sc[i >> 2][i & 3], hidden, i);
+            vs = hidden != kAll ? vs : 0.0f;
         }
         float mx = sc[0][0];
 #pragma unroll
-        for (int i = 1; i < 16; i++) mx = fmaxf(mx, sc[i >> 2][i & 3]);
+        for (int i = 1; i < SEG; i++) mx = fmaxf(mx, sc[i >> 2][i & 3]);
         mx = ap_max_quarters(mx * f);
         const float top = ap_max_quarters(ap_power(vs));
         if (__any(mx > m + kApLate || top > ref)) {
@@ -398,9 +624,9 @@ __global__ __launch_bounds__(WAVES * 64, NK <= 2 ? 2 : 1) void attnp_rows_kernel
             over = kApUnit / ref;
         }
         const float w = vs * over;
-        ap_h8 ph[2], pl[2];
+        ap_h8 ph[TT / 2], pl[TT / 2];
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int e = 0; e < TT / 2; e++) {
             float pr[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -410,57 +636,76 @@ __global__ __launch_bounds__(WAVES * 64, NK <= 2 ? 2 : 1) void attnp_rows_kernel
             ap_split8w(pr, w, ph[e], pl[e]);
         }
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            const ap_h8 a = ap_cvt8(vr[d].x, vr[d].y), b = ap_cvt8(vr[d].z, vr[d].w);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[0], o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ph[1], o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[0], o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, pl[1], o[d], 0, 0, 0);
-        }
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < TT / 2; e++) {
+                const ap_h8 a = ap_cvt8(vr[d][2 * e], vr[d][2 * e + 1]);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[e], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[e], o[d], 0, 0, 0);
+            }
         load_values(next, pv_next);
         pk = page_of(min(next + WAVES, u1 - 1), col >> 2);
         pv = page_of(min(next + WAVES, u1 - 1), g);
     }
 
-    // join the waves: all lanes of a column hold the same m and parts of l
+    // all lanes of a column hold the same m and parts of l
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     const float back = ref * (1.0f / kApUnit);
-    if (g == 0) {
-        m_lds[wave][col] = m;
-        l_lds[wave][col] = l;
-    }
-#pragma unroll
-    for (int d = 0; d < ND; d++)
-        o_lds[wave][4 * d + g][col] = float4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back};
-    __syncthreads();
     const int rows = min(16, n_rows - tile * 16);
-    const int64_t item = ((int64_t)r * A.n_tiles + tile) * A.C.n_kv + h;
-    float *part = A.part + ap_part(A, item, split, 16);
-    for (int i = tid; i < 4 * hd; i += WAVES * 64) {
-        // whole rows to out, the sums of a dim for all rows to the splits
-        const int c = n_split == 1 ? i / (hd / 4) : i % 16, d4 = n_split == 1 ? i % (hd / 4) : i / 16;
-        if (c >= rows) continue;
-        float mm = kApNone, ll = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) mm = fmaxf(mm, m_lds[w][c]);
-        float4 oo = {0, 0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const float e = __builtin_amdgcn_exp2f(m_lds[w][c] - mm);
-            const float4 v = o_lds[w][d4][c];
-            ll = fmaf(l_lds[w][c], e, ll);
-            oo = float4{fmaf(v.x, e, oo.x), fmaf(v.y, e, oo.y), fmaf(v.z, e, oo.z), fmaf(v.w, e, oo.w)};
-        }
+    const __amdgpu_buffer_rsrc_t part = ap_pieces(A, piece, 1);
+    if constexpr (WAVES == 1) {
         if (n_split == 1) {
-            const int rw = tile * 16 + c;
-            ap_put4(A.out + (s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + 4 * d4, ap_quotient(oo.x, ll),
-                    ap_quotient(oo.y, ll), ap_quotient(oo.z, ll), ap_quotient(oo.w, ll), A.out_vec);
-        } else {
-            ((float4 *)part)[i] = oo;
-            if (d4 == 0) ((float4 *)part)[4 * hd + c] = float4{mm, ll, 0, 0};
+            if (col >= rows) return;
+            const float z = l > 0.0f || l != l ? back / l : 0.0f;
+            float *to = A.out + (s.q0 + tok) * A.ldo + (int64_t)head * hd + 4 * g;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+                if (16 * d < hd) ap_put4(to + 16 * d, o[d][0] * z, o[d][1] * z, o[d][2] * z, o[d][3] * z, A.out_vec);
+        } else if (col < rows) {
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+                if (16 * d < hd)
+                    ap_store4(part, (4 * d + g) * 16 + col, float4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back});
+            if (g == 0) ap_store4(part, 4 * hd + col, float4{m, l, 0, 0});
+        }
+    } else {
+        __shared__ float4 o_lds[WAVES][ND * 4][17];
+        __shared__ float m_lds[WAVES][16], l_lds[WAVES][16];
+        if (g == 0) {
+            m_lds[wave][col] = m;
+            l_lds[wave][col] = l;
+        }
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+            o_lds[wave][4 * d + g][col] = float4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back};
+        __syncthreads();
+        for (int i = tid; i < 4 * hd; i += WAVES * 64) {
+            // whole rows to out, the sums of a dim for all rows to the splits
+            const int c = n_split == 1 ? i / (hd / 4) : i % 16, d4 = n_split == 1 ? i % (hd / 4) : i / 16;
+            if (c >= rows) continue;
+            float mm = kApNone, ll = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) mm = fmaxf(mm, m_lds[w][c]);
+            float4 oo = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float e = __builtin_amdgcn_exp2f(m_lds[w][c] - mm);
+                const float4 v = o_lds[w][d4][c];
+                ll = fmaf(l_lds[w][c], e, ll);
+                oo = float4{fmaf(v.x, e, oo.x), fmaf(v.y, e, oo.y), fmaf(v.z, e, oo.z), fmaf(v.w, e, oo.w)};
+            }
+            if (n_split == 1) {
+                const int rw = tile * 16 + c;
+                ap_put4(A.out + (s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + 4 * d4,
+                        ap_quotient(oo.x, ll), ap_quotient(oo.y, ll), ap_quotient(oo.z, ll), ap_quotient(oo.w, ll), A.out_vec);
+            } else {
+                ap_store4(part, i, oo);
+                if (d4 == 0) ap_store4(part, 4 * hd + c, float4{mm, ll, 0, 0});
+            }
         }
     }
+    if (n_split > 1) ap_join_rows<WAVES * 64>(A, s, h, tile, rows, piece - split, n_split);
 }
 
 // ---- many rows ---------------------------------------------------------------------
@@ -485,10 +730,13 @@ __global__ __launch_bounds__(WAVES * 64, NK <= 2 ? 2 : 1) void attnp_rows_kernel
 // = sum over requests of max(0, blocks - t), its number t has F(t + 1) <= i <
 // F(t), and it is the i - F(t + 1)th of the requests with more than t blocks.
 // The lanes try 64 numbers at once; up to 64 kPlaceRegs requests.
-constexpr int kPlaceRegs = 4;
-
 __device__ inline bool ap_place(const AttnPArgs &A, int rows, int64_t i, int &r, int &tile) {
     const int lane = threadIdx.x & 63;
+    if (A.n_req == 1) {
+        r = 0;
+        tile = (min(request_span(A.R, 0).n, A.R.max_q) * A.G + rows - 1) / rows - 1 - (int)i;
+        return tile >= 0;
+    }
     int blocks[kPlaceRegs];
 #pragma unroll
     for (int k = 0; k < kPlaceRegs; k++) {
@@ -550,7 +798,7 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
     const int n_tok = min(s.n, A.R.max_q), n_rows = n_tok * A.G;
     if (tile * kApTileRows >= n_rows) return;
     const Sight S = ap_sight(A, r, s, tile * kApTileRows / A.G, min((tile * kApTileRows + kApTileRows - 1) / A.G, n_tok - 1));
-    const int n_split = ap_splits(A, S.n);
+    const int n_split = ap_splits(A, S.n, A.per_split);
     if (split >= n_split) return;
     const int u0 = (int)((int64_t)S.n * split / n_split), u1 = (int)((int64_t)S.n * (split + 1) / n_split);
 
@@ -562,29 +810,7 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
     W.p_lo = s.p0 + min(row0, n_rows - 1) / A.G;
     W.p_hi = s.p0 + min(row0 + 31, n_rows - 1) / A.G;
     const float slope = A.slopes ? A.slopes[head] * kLog2e : 0.0f;
-    ap_h8 qh[NS], ql[NS];
-    float f_row;
-    {
-        const float *qrow = A.q + (s.q0 + tok) * A.ldq + (int64_t)head * hd + 8 * half;
-        float amax = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NS; c++)
-            if (16 * c < hd)
-#pragma unroll
-                for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(qrow[16 * c + j]));
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
-        const int e2 = ap_row_exponent(amax);
-#pragma unroll
-        for (int c = 0; c < NS; c++) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = 16 * c < hd ? ldexpf(qrow[16 * c + j] * A.sign, e2) : 0.0f;
-            ap_split8(x, qh[c], ql[c]);
-        }
-        f_row = ldexpf(1.0f, -e2);
-    }
-    const float fc_row = f_row * A.cap_in;
-    f_row *= A.scale2;
+    const float *qrow = A.q + (s.q0 + tok) * A.ldq + (int64_t)head * hd + 8 * half;
 
     // loads without branches: what is not there is read from elsewhere in the
     // table or the page and replaced
@@ -643,16 +869,43 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
         if (tid < 8) s_lds[buf][tid] = scale;
     };
 
-    ap_f16 o[ND];
-#pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     float m = kApNone, l = 0.0f, ref = 0.0f, over = 0.0f;
     if (u0 < u1) {
         load_pages(u0);
         load_chunk(u0);
         load_pages(min(u0 + 1, u1 - 1));
+    }
+    // the query, while the first chunk is on its way
+    ap_h8 qh[NS], ql[NS];
+    float f_row, fc_row;
+    {
+        float x[NS][8], amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NS; c++) ap_load8(qrow + (16 * c < hd ? 16 * c : 0), A.q_vec, x[c]);
+#pragma unroll
+        for (int c = 0; c < NS; c++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[c][j] = 16 * c < hd ? x[c][j] * A.sign : 0.0f;
+                amax = fmaxf(amax, fabsf(x[c][j]));
+            }
+        const int e2 = ap_row_exponent(ap_max_halves(amax));
+#pragma unroll
+        for (int c = 0; c < NS; c++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[c][j] = ldexpf(x[c][j], e2);
+            ap_split8(x[c], qh[c], ql[c]);
+        }
+        f_row = ldexpf(1.0f, -e2);
+        fc_row = f_row * A.cap_in;
+        f_row *= A.scale2;
+    }
+    ap_f16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    if (u0 < u1) {
         put_chunk(0);
         load_chunk(min(u0 + 1, u1 - 1));
         load_pages(min(u0 + 2, u1 - 1));
@@ -669,7 +922,7 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
         // nothing here for this wave's rows
         if (idle || (j0 >= S.prefix && (j0 > W.p_hi || (A.window && j0 + 63 <= W.p_lo - A.window)))) continue;
 
-        const bool whole = ap_whole(A, W, j0 >> 6);
+        const bool whole = ap_whole(A, W, j0, 64);
         const int key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
         const int x = KC % 16 ? (col >> 1) & 7 : col & 15, y = (col >> 1) & 7;
 #pragma unroll 1
@@ -761,7 +1014,7 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
                     if (32 * d + 8 * a < hd) ap_put4(to + 32 * d + 8 * a, o[d][4 * a] * z, o[d][4 * a + 1] * z,
                                 o[d][4 * a + 2] * z, o[d][4 * a + 3] * z, A.out_vec);
         } else {
-            float4 *to = (float4 *)(A.part + ap_part(A, item, split, kApTileRows)) + wave * 32 + col;
+            float4 *to = ap_part(A, item * A.n_split + split, kApTileRows) + wave * 32 + col;
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -776,7 +1029,7 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
 
 // ---- row blocks whose keys were split -----------------------------------------------
 //
-// A second launch adds up a row block's splits, in their order: a thread has
+// A second launch adds up a large row block's splits, in their order: a thread has
 // four dims of a row. (One workgroup, the last of a block to arrive, would
 // have to read all of it: 66 KB a split for 128 rows of 128 dims.)
 
@@ -788,26 +1041,28 @@ __global__ __launch_bounds__(kApJoinThreads) void attnp_join_kernel(AttnPArgs A)
     const int64_t place = blockIdx.x / A.C.n_kv;
     int r = blockIdx.z, tile = (int)place;
     if (A.placed && !ap_place(A, ROWS, place, r, tile)) return;
-    const int64_t item = (A.placed ? place : (int64_t)r * A.n_tiles + tile) * A.C.n_kv + h;
+    const int64_t piece = ((A.placed ? place : (int64_t)r * A.n_tiles + tile) * A.C.n_kv + h) * A.n_split;
     const Span s = request_span(A.R, r);
     const int n_tok = min(s.n, A.R.max_q), n_rows = n_tok * A.G;
     const int c = threadIdx.x % ROWS, d4 = blockIdx.y * (kApJoinThreads / ROWS) + threadIdx.x / ROWS, row = tile * ROWS + c;
     if (tile * ROWS >= n_rows) return;
     const int t0 = tile * ROWS / A.G, t1 = min((tile * ROWS + ROWS - 1) / A.G, n_tok - 1);
-    const int n_split = ap_splits(A, ap_sight(A, r, s, t0, t1).n);
+    const int n_split = ap_splits(A, ap_sight(A, r, s, t0, t1).n, A.per_split);
     if (n_split == 1 || row >= n_rows || 4 * d4 >= hd) return;
-    const float4 *part = (const float4 *)(A.part + ap_part(A, item, 0, ROWS)) + c;
+    const float4 *part = ap_part(A, piece, ROWS) + c;
     const int64_t step = (int64_t)(hd / 4 + 1) * ROWS;
+    // sixteen splits at once, all their loads in flight
     float m = kApNone, l = 0.0f;
-#pragma unroll 8
-    for (int k = 0; k < n_split; k++) m = fmaxf(m, part[k * step + hd / 4 * ROWS].x);
     float4 o = {0, 0, 0, 0};
-#pragma unroll 8
-    for (int k = 0; k < n_split; k++) {
-        const float4 ml = part[k * step + hd / 4 * ROWS], v = part[k * step + d4 * ROWS];
-        const float e = __builtin_amdgcn_exp2f(ml.x - m);
-        l = fmaf(ml.y, e, l);
-        o = float4{fmaf(v.x, e, o.x), fmaf(v.y, e, o.y), fmaf(v.z, e, o.z), fmaf(v.w, e, o.w)};
+    for (int k0 = 0; k0 < n_split; k0 += 16) {
+        float4 ml[16], v[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            const int64_t at = min(k0 + k, n_split - 1) * step;
+            ml[k] = part[at + hd / 4 * ROWS];
+            v[k] = part[at + d4 * ROWS];
+        }
+        ap_add16(n_split - k0, ml, v, m, l, o);
     }
     ap_put4(A.out + (s.q0 + row / A.G) * A.ldo + (int64_t)(h * A.G + row % A.G) * hd + 4 * d4, ap_quotient(o.x, l),
             ap_quotient(o.y, l), ap_quotient(o.z, l), ap_quotient(o.w, l), A.out_vec);

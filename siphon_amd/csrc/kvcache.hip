@@ -171,15 +171,17 @@ extern "C" int sihip_kv_read_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, co
 
 namespace {
 
-constexpr int kApRowWaves = 4;  // of a 16-row block
+// counters at the front of a caller's workspace, whatever the call's size
+constexpr size_t kCounterBytes = (size_t)kGemmCounters * 4;
 
 struct AttnPPlan {
     AttnPArgs A;
     int waves;  // of 32 rows in a large row block, 0: 16-row blocks
+    int row_waves;  // waves that share a 16-row block's chunks
     int64_t blocks, items;  // row blocks, and those times the KV heads
     int64_t gx;             // of the grid
     int block_rows;
-    size_t ws_bytes;
+    size_t part_bytes;
 };
 
 // Waves of 32 rows in a row block of the prompt kernel, 0: 16-row blocks.
@@ -215,6 +217,7 @@ int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch 
     A.out = a->out;
     A.ldq = a->ldq;
     A.ldo = a->ldo;
+    A.q_vec = aligned(a->q, 16) && a->ldq % 4 == 0;
     A.out_vec = aligned(a->out, 16) && a->ldo % 4 == 0;
     A.slopes = a->slopes;
     A.prefix = a->prefix;
@@ -233,22 +236,49 @@ int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch 
     // row blocks of all requests: as many as the longest has each, or, listed
     // (ap_place), no more than the step's rows fill
     P.blocks = (int64_t)A.n_req * A.n_tiles;
-    A.placed = P.waves && A.n_req <= 64 * kPlaceRegs;
-    if (A.placed) P.blocks = std::min(P.blocks, A.R.n_tok * A.G / block_rows + A.n_req);
+    A.placed = A.n_req <= 64 * kPlaceRegs;
+    if (A.placed && P.waves) P.blocks = std::min(P.blocks, A.R.n_tok * A.G / block_rows + A.n_req);
     P.items = P.blocks * A.C.n_kv;
-    // splits of a row block's keys: until every CU has its workgroups, none
-    // shorter than a chunk per wave
-    const int64_t chunks = std::max<int64_t>(1, ((int64_t)A.R.max_kv + 63) / 64);
-    const int64_t per_cu = P.waves ? std::max(1, 8 / P.waves) : 4, least = P.waves ? 4 : kApRowWaves;
-    int64_t n = (per_cu * ctx->n_cu + P.items - 1) / std::max<int64_t>(P.items, 1);
-    if (ctx->opt.attnp_splits > 0) n = ctx->opt.attnp_splits;
-    n = std::max<int64_t>(1, std::min<int64_t>(n, 64));
-    A.per_split = (int)std::max<int64_t>((chunks + n - 1) / n, ctx->opt.attnp_splits > 0 ? 1 : least);
-    A.n_split = (int)((chunks + A.per_split - 1) / A.per_split);
+    A.chunk = P.waves || A.C.hd <= 128 ? 6 : 5;
+    const int64_t chunks = std::max<int64_t>(1, ((int64_t)A.R.max_kv + (1 << A.chunk) - 1) >> A.chunk);
+    const int64_t forced = ctx->opt.attnp_splits;
+    int64_t pieces = 0;
+    if (P.waves || !A.placed) {
+        // splits of a row block's keys: until every CU has its workgroups, none
+        // shorter than a chunk per wave
+        P.row_waves = 4;
+        const int64_t per_cu = P.waves ? std::max(1, 8 / P.waves) : 4;
+        int64_t n = (per_cu * ctx->n_cu + P.items - 1) / std::max<int64_t>(P.items, 1);
+        if (forced > 0) n = forced;
+        n = std::max<int64_t>(1, std::min<int64_t>(n, 64));
+        A.per_split = (int)std::max<int64_t>((chunks + n - 1) / n, forced > 0 ? 1 : 4);
+        A.n_split = (int)((chunks + A.per_split - 1) / A.per_split);
+        A.whole = 0;
+        pieces = P.items * A.n_split;
+    } else {
+        // two workgroups of four waves a CU, or eight of one
+        const int64_t w = ctx->opt.attnp_row_waves;
+        P.row_waves = w == 1 || w == 4 || w == 8 ? (int)w : P.items >= 64 ? 1 : 4;
+        A.slots = 8 / P.row_waves * ctx->n_cu;
+        A.per_split = P.row_waves;
+        A.whole = 3 * P.row_waves;
+        if (forced > 0) {
+            A.slots = (int)std::min<int64_t>(forced * std::max<int64_t>(P.items, 1), 1 << 20);
+            A.per_split = 1;
+            A.whole = 0;
+        }
+        A.n_split = chunks > std::max(A.whole, A.per_split) ? INT32_MAX : 1;
+        pieces = P.items + A.slots;
+    }
+    // 16-row blocks join by counters, one for each piece at most
+    if (!P.waves && pieces > kGemmCounters) {
+        A.n_split = 1;
+        A.per_split = INT32_MAX;
+    }
     P.block_rows = block_rows;
-    P.ws_bytes = A.n_split > 1 ? (size_t)P.items * A.n_split * block_rows * (A.C.hd / 4 + 1) * 16 : 0;
+    P.part_bytes = A.n_split > 1 ? (size_t)pieces * block_rows * (A.C.hd / 4 + 1) * 16 : 0;
     A.part = nullptr;
-    P.gx = P.waves ? (A.placed ? P.blocks : A.n_tiles) * A.C.n_kv : A.n_tiles * A.n_split;
+    P.gx = P.waves ? (A.placed ? P.blocks : A.n_tiles) * A.C.n_kv : A.placed ? (A.n_split > 1 ? pieces : P.items) : (int64_t)A.n_tiles * A.n_split;
     if (P.gx * 512 > UINT32_MAX)
         return set_err(ctx, SIHIP_EINVAL, "%s: max_q %d of %lld heads has no grid", fn, A.R.max_q,
                        (long long)a->n_head);
@@ -263,7 +293,7 @@ extern "C" int sihip_attn_paged_workspace(sihip_ctx *ctx, const sihip_kv_cache *
     AttnPPlan P;
     const int rc = plan_attn(ctx, cache, batch, args, P);
     if (rc) return rc;
-    *bytes = P.ws_bytes;
+    *bytes = P.part_bytes ? kCounterBytes + P.part_bytes : 0;
     return SIHIP_OK;
 }
 
@@ -279,18 +309,20 @@ extern "C" int sihip_attn_paged_dev(sihip_ctx *ctx, const sihip_kv_cache *cache,
     const bool shared = A.n_split > 1 && !args->workspace;
     if (shared) {
         try {
-            rc = ensure(ctx, &ctx->d_attn, &ctx->d_attn_cap, P.ws_bytes, st);
+            rc = ensure(ctx, &ctx->d_attn, &ctx->d_attn_cap, P.part_bytes, st);
         } catch (...) {
             rc = set_err(ctx, SIHIP_ENOMEM, "attn_paged_dev: out of host memory");
         }
         if (!rc) rc = order_before(ctx, ctx->order, st);
         if (rc) return rc;
+        A.cnt = ctx->d_gcnt;
         A.part = (float *)ctx->d_attn;
     } else if (A.n_split > 1) {
-        if (args->workspace_bytes < P.ws_bytes || !aligned(args->workspace, 16))
+        if (args->workspace_bytes < kCounterBytes + P.part_bytes || !aligned(args->workspace, 16))
             return set_err(ctx, SIHIP_EINVAL, "attn_paged_dev: a workspace of %zu bytes, 16-byte aligned, is needed",
-                           P.ws_bytes);
-        A.part = (float *)args->workspace;
+                           kCounterBytes + P.part_bytes);
+        A.cnt = (uint32_t *)args->workspace;
+        A.part = (float *)((uint8_t *)args->workspace + kCounterBytes);
     }
     const int hd = A.C.hd;
     if (P.waves) {
@@ -306,22 +338,24 @@ extern "C" int sihip_attn_paged_dev(sihip_ctx *ctx, const sihip_kv_cache *cache,
         else hipLaunchKernelGGL((attnp_tiles_kernel<16, 4>), grid, t, 0, st, A);
 #undef SIHIP_APT
     } else {
-        const dim3 grid((unsigned)P.gx, (unsigned)A.C.n_kv, (unsigned)A.n_req), t(kApRowWaves * 64);
-        if (hd <= 64) hipLaunchKernelGGL((attnp_rows_kernel<1, kApRowWaves>), grid, t, 0, st, A);
-        else if (hd <= 128) hipLaunchKernelGGL((attnp_rows_kernel<2, kApRowWaves>), grid, t, 0, st, A);
-        else if (hd <= 192) hipLaunchKernelGGL((attnp_rows_kernel<3, kApRowWaves>), grid, t, 0, st, A);
-        else hipLaunchKernelGGL((attnp_rows_kernel<4, kApRowWaves>), grid, t, 0, st, A);
+        const dim3 grid((unsigned)P.gx, A.placed ? 1u : (unsigned)A.C.n_kv, A.placed ? 1u : (unsigned)A.n_req), t(P.row_waves * 64);
+#define SIHIP_APR(NK, TT)                                                                                  \
+    if (P.row_waves == 1) hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 1>), grid, t, 0, st, A);           \
+    else if (P.row_waves == 4) hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 4>), grid, t, 0, st, A);      \
+    else hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 8>), grid, t, 0, st, A);
+        if (hd <= 64) { SIHIP_APR(1, 4) }
+        else if (hd <= 128) { SIHIP_APR(2, 4) }
+        else if (hd <= 192) { SIHIP_APR(3, 2) }
+        else { SIHIP_APR(4, 2) }
+#undef SIHIP_APR
     }
-    if (A.n_split > 1) {
+    if (P.waves && A.n_split > 1) {
         const int per_wg = kApJoinThreads / P.block_rows;  // four-dim columns
         const dim3 grid((unsigned)((A.placed ? P.blocks : A.n_tiles) * A.C.n_kv), (unsigned)((hd / 4 + per_wg - 1) / per_wg),
                         A.placed ? 1u : (unsigned)A.n_req), t(kApJoinThreads);
-        switch (P.block_rows) {
-            case kApRows: hipLaunchKernelGGL(attnp_join_kernel<kApRows>, grid, t, 0, st, A); break;
-            case 64: hipLaunchKernelGGL(attnp_join_kernel<64>, grid, t, 0, st, A); break;
-            case 128: hipLaunchKernelGGL(attnp_join_kernel<128>, grid, t, 0, st, A); break;
-            default: hipLaunchKernelGGL(attnp_join_kernel<256>, grid, t, 0, st, A); break;
-        }
+        if (P.block_rows == 64) hipLaunchKernelGGL(attnp_join_kernel<64>, grid, t, 0, st, A);
+        else if (P.block_rows == 128) hipLaunchKernelGGL(attnp_join_kernel<128>, grid, t, 0, st, A);
+        else hipLaunchKernelGGL(attnp_join_kernel<256>, grid, t, 0, st, A);
     }
     rc = launched(ctx, "attn_paged");
     if (rc) return rc;

@@ -100,7 +100,7 @@ def test_workspaces(what):
     exist before a capture."""
     got = fake_hip.run(SETUP + f"""
 what = {what!r}
-c, b, a = cache(), batch(max_kv=640, n_tok=1, n_req=1), attn()
+c, b, a = cache(), batch(max_kv=2000, max_blocks=80, n_tok=1, n_req=1), attn()
 n = dev.attn_paged_workspace(c, b, a)
 if what == "capture":
     fake.fake_capture(1)
