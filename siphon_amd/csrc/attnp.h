@@ -323,6 +323,7 @@ __device__ inline Deal ap_deal(const AttnPArgs &A) {
         const int r = lane + 64 * k;
         D.n[k] = tiles[k] = 0;
         D.s[k] = Span{0, 0, 0, 0};
+        if (64 * k >= A.n_req) continue;  // (of the whole wave)
         if (r < A.n_req) {
             D.s[k] = request_span(A.R, r);
             const int n = min(D.s[k].n, A.R.max_q);
@@ -340,9 +341,9 @@ __device__ inline Deal ap_deal(const AttnPArgs &A) {
     int before = 0;
 #pragma unroll
     for (int k = 0; k < kPlaceRegs; k++) {
-        D.last[k] = tiles[k] * A.C.n_kv * D.splits(A, D.n[k]);
-        if (64 * k < A.n_req) D.last[k] = ap_scan(D.last[k]);
-        D.last[k] += before;
+        D.last[k] = before;
+        if (64 * k >= A.n_req) continue;
+        D.last[k] += ap_scan(tiles[k] * A.C.n_kv * D.splits(A, D.n[k]));
         before = __builtin_amdgcn_readlane(D.last[k], 63);
     }
     return D;
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
     const Sight S = ap_sight(A, r, s, t0, t1);
     const int n_split = ap_splits(A, S.n, per);
     if (split >= n_split) return;
-    const int u0 = split * per, u1 = split == n_split - 1 ? S.n : u0 + per;
+    const int u0 = (int)((int64_t)S.n * split / n_split), u1 = (int)((int64_t)S.n * (split + 1) / n_split);
 
     // pages of this lane's key rows, and of its values and scores
     const int last_block = max(S.keys - 1, 0) >> shift, n_pages = (int)A.C.n_pages;
@@ -575,15 +576,24 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
         ap_f4 sc[TT];
 #pragma unroll
         for (int t = 0; t < TT; t++) sc[t] = ap_f4{0, 0, 0, 0};
+        // (two tiles at a time: a product waits for the one before it of its sum)
 #pragma unroll
         for (int e = 0; e < NK; e++)
 #pragma unroll
-            for (int t = 0; t < TT; t++) {
-                const ap_h8 a = ap_cvt8(kr[t][e].x, kr[t][e].y), b = ap_cvt8(kr[t][e].z, kr[t][e].w);
-                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[e][0], sc[t], 0, 0, 0);
-                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[e][1], sc[t], 0, 0, 0);
-                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[e][0], sc[t], 0, 0, 0);
-                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ql[e][1], sc[t], 0, 0, 0);
+            for (int t = 0; t < TT; t += 2) {
+                ap_h8 a[2][2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    a[i][0] = ap_cvt8(kr[t + i][e].x, kr[t + i][e].y);
+                    a[i][1] = ap_cvt8(kr[t + i][e].z, kr[t + i][e].w);
+                }
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) sc[t + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i][y], qh[e][y], sc[t + i], 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) sc[t + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i][y], ql[e][y], sc[t + i], 0, 0, 0);
+                }
             }
         // scores in log2 units are sc * f; the factor is kept above zero, so
         // that it leaves -inf as it is, and is a number where no key is seen
@@ -636,12 +646,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
             ap_split8w(pr, w, ph[e], pl[e]);
         }
 #pragma unroll
-        for (int d = 0; d < ND; d++)
+        for (int d = 0; d < ND; d += 2)
 #pragma unroll
             for (int e = 0; e < TT / 2; e++) {
-                const ap_h8 a = ap_cvt8(vr[d][2 * e], vr[d][2 * e + 1]);
+                const ap_h8 a = ap_cvt8(vr[d][2 * e], vr[d][2 * e + 1]), b = ap_cvt8(vr[d + 1][2 * e], vr[d + 1][2 * e + 1]);
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[e], o[d], 0, 0, 0);
+                o[d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ph[e], o[d + 1], 0, 0, 0);
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[e], o[d], 0, 0, 0);
+                o[d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, pl[e], o[d + 1], 0, 0, 0);
             }
         load_values(next, pv_next);
         pk = page_of(min(next + WAVES, u1 - 1), col >> 2);

@@ -256,12 +256,16 @@ int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch 
         A.whole = 0;
         pieces = P.items * A.n_split;
     } else {
-        // two workgroups of four waves a CU, or eight of one
+        // Four waves share a piece, or, where there are row blocks enough, each
+        // has its own. Workgroups that the pieces are made for: one a CU for few
+        // long requests (32 heads of 128 over 131072 keys 55 us, 65 with 1.5 a
+        // CU), more where lengths differ (64 requests of up to 8192 keys 95 us with
+        // one, 90 with three; 16 of 16000 with 8 heads 71, 58 with 1.5).
         const int64_t w = ctx->opt.attnp_row_waves;
-        P.row_waves = w == 1 || w == 4 || w == 8 ? (int)w : P.items >= 64 ? 1 : 4;
-        A.slots = 8 / P.row_waves * ctx->n_cu;
+        P.row_waves = w == 1 || w == 4 || w == 8 ? (int)w : P.items >= 4 * ctx->n_cu ? 1 : 4;
+        A.slots = (P.row_waves == 1 ? 16 : P.items < 64 ? 2 : P.items < 256 ? 3 : 6) * ctx->n_cu / 2;
         A.per_split = P.row_waves;
-        A.whole = 3 * P.row_waves;
+        A.whole = 2 * P.row_waves;
         if (forced > 0) {
             A.slots = (int)std::min<int64_t>(forced * std::max<int64_t>(P.items, 1), 1 << 20);
             A.per_split = 1;
