@@ -57,6 +57,7 @@ struct AttnPArgs {
     int slots;       // placed 16-row blocks: workgroups that share the chunks of all
     int chunk;       // log2 of the keys of a chunk
     int placed;      // 1: the grid is a list made on the device (ap_place, ap_deal)
+    int least, most; // rows of the requests that are in it
     float *part;     // [piece][hd / 4 + 1][rows] of four: sums by dims, then m, l
     uint32_t *cnt;   // 16-row blocks: pieces that have arrived, zero between launches
 };
@@ -327,7 +328,7 @@ __device__ inline Deal ap_deal(const AttnPArgs &A) {
         if (r < A.n_req) {
             D.s[k] = request_span(A.R, r);
             const int n = min(D.s[k].n, A.R.max_q);
-            if (n > 0) {
+            if (n > 0 && n * A.G <= A.most) {
                 tiles[k] = (n * A.G + kApRows - 1) / kApRows;
                 D.n[k] = ap_sight(A, r, D.s[k], 0, n - 1).n;
             }
@@ -732,6 +733,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
 // is a multiple of 256 bytes, by three where it is an odd multiple of 128 and
 // neighbouring rows lie in the two halves.
 //
+// Each half of a chunk is two steps between barriers: vector work (weights from
+// scores, codes to f16) and matrix work (weights times values, the next half's
+// scores). Of eight waves four are a step behind the others, which leaves each
+// SIMD one wave of either kind at any time: kTurns.
+//
 // A wave's 32x32 tile of S^T has its key rows in the order that gives lane
 // (row c, half e) the scores of keys 32 u + 16 e + i in register i: row m of
 // the operand is key 16 (m / 4 % 2) + 4 (m / 8) + m % 4.
@@ -746,14 +752,16 @@ __device__ inline bool ap_place(const AttnPArgs &A, int rows, int64_t i, int &r,
     const int lane = threadIdx.x & 63;
     if (A.n_req == 1) {
         r = 0;
-        tile = (min(request_span(A.R, 0).n, A.R.max_q) * A.G + rows - 1) / rows - 1 - (int)i;
-        return tile >= 0;
+        const int n = min(request_span(A.R, 0).n, A.R.max_q) * A.G;
+        tile = (n + rows - 1) / rows - 1 - (int)i;
+        return n >= A.least && tile >= 0;
     }
     int blocks[kPlaceRegs];
 #pragma unroll
     for (int k = 0; k < kPlaceRegs; k++) {
         const int q = lane + 64 * k;
-        blocks[k] = q < A.n_req ? (min(request_span(A.R, q).n, A.R.max_q) * A.G + rows - 1) / rows : 0;
+        const int n = q < A.n_req ? min(request_span(A.R, q).n, A.R.max_q) * A.G : 0;
+        blocks[k] = n < A.least ? 0 : (n + rows - 1) / rows;
     }
     int lo = 0, span = A.n_tiles;
     int64_t f = 0;
@@ -791,8 +799,9 @@ __device__ inline bool ap_place(const AttnPArgs &A, int rows, int64_t i, int &r,
 
 // hd rounded up to 16 NS dims
 template <int NS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kernel(AttnPArgs A) {
+__global__ __launch_bounds__(64 * WAVES, NS <= 4 && WAVES == 4 ? 3 : 2) void attnp_tiles_kernel(AttnPArgs A) {
     constexpr int kApTileRows = 32 * WAVES, kApTileThreads = 64 * WAVES;
+    constexpr bool kTurns = WAVES == 8;
     constexpr int ND = (NS + 1) / 2;             // 32-dim tiles of the output
     constexpr int KC = (2 * NS + 7) / 8 * 8;     // granules of a key row in LDS
     constexpr int NU = (64 * NS + kApTileThreads - 1) / kApTileThreads;  // 16-byte loads of a chunk, each
@@ -854,37 +863,44 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
         for (int i = 0; i < NU; i++) kpg[i] = page_of(j0 + unit(i) / NS);
         vpg = page_of(j0 + 16 * (tid & 3));
     };
-    auto load_chunk = [&](int u) {
+    auto load_keys = [&](int u) {
         const int at = ap_chunk(S, u) * 64 & (B - 1);
-        const uint64_t vp = (uint64_t)(uint32_t)max(vpg, 0) * page_bytes + at;
 #pragma unroll
-        for (int i = 0; i < NU; i++) {
-            kr[i] = *(const uint4 *)(kb[i] + ((uint64_t)(uint32_t)max(kpg[i], 0) * page_bytes + at * hd));
-            vr[i] = *(const uint4 *)(vb[i] + vp);
-        }
+        for (int i = 0; i < NU; i++) kr[i] = *(const uint4 *)(kb[i] + ((uint64_t)(uint32_t)max(kpg[i], 0) * page_bytes + at * hd));
         if (tid < 8) scale = vpg >= 0 ? (tid < 4 ? A.C.ks : A.C.vs)[(int64_t)vpg * A.C.n_kv + h] : -1.0f;
     };
-    auto put_chunk = [&](int buf) {
+    auto load_values = [&](int u) {
+        const uint64_t at = (uint64_t)(uint32_t)max(vpg, 0) * page_bytes + (ap_chunk(S, u) * 64 & (B - 1));
+#pragma unroll
+        for (int i = 0; i < NU; i++) vr[i] = *(const uint4 *)(vb[i] + at);
+    };
+    auto put_keys = [&](int buf) {
         const uint4 zero = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NU; i++) {
-            const int key = unit(i) / NS, d16 = unit(i) % NS, dim = unit(i) >> 2;
+            const int key = unit(i) / NS, d16 = unit(i) % NS;
             // dims past hd meet zeros of q: they must be numbers
             const uint4 a = d16 * 16 < hd ? kr[i] : zero;
             const int kx = (key & 3) | ((key >> 2) & 4) | ((key << 1) & 8), x = KC % 16 ? kx >> 1 : kx;
-            const int c = 2 * (tid & 3), y = (dim >> 1) & 7;
             k_lds[buf][key][(2 * d16) ^ x] = __builtin_bit_cast(uint4, ap_cvt8(a.x, a.y));
             k_lds[buf][key][(2 * d16 + 1) ^ x] = __builtin_bit_cast(uint4, ap_cvt8(a.z, a.w));
+        }
+        if (tid < 8) s_lds[buf][tid] = scale;
+    };
+    auto put_values = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NU; i++) {
+            const int dim = unit(i) >> 2, c = 2 * (tid & 3), y = (dim >> 1) & 7;
             v_lds[buf][dim][c ^ y] = __builtin_bit_cast(uint4, ap_cvt8(vr[i].x, vr[i].y));
             v_lds[buf][dim][(c + 1) ^ y] = __builtin_bit_cast(uint4, ap_cvt8(vr[i].z, vr[i].w));
         }
-        if (tid < 8) s_lds[buf][tid] = scale;
     };
 
     float m = kApNone, l = 0.0f, ref = 0.0f, over = 0.0f;
     if (u0 < u1) {
         load_pages(u0);
-        load_chunk(u0);
+        load_keys(u0);
+        load_values(u0);
         load_pages(min(u0 + 1, u1 - 1));
     }
     // the query, while the first chunk is on its way
@@ -917,100 +933,123 @@ __global__ __launch_bounds__(64 * WAVES, NS <= 8 ? 2 : 1) void attnp_tiles_kerne
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    // nothing in a chunk for this wave's rows
+    auto blind = [&](int u) {
+        const int j0 = ap_chunk(S, u) * 64;
+        return idle || (j0 >= S.prefix && (j0 > W.p_hi || (A.window && j0 + 63 <= W.p_lo - A.window)));
+    };
+    const int key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
+    const int x = KC % 16 ? (col >> 1) & 7 : col & 15, y = (col >> 1) & 7;
+    ap_f16 sc;
+    auto scores = [&](int buf, int i) {
+        const uint4 *kl = k_lds[buf][32 * i + key];
+#pragma unroll
+        for (int e = 0; e < 16; e++) sc[e] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NS; c++) {
+            const ap_h8 a = __builtin_bit_cast(ap_h8, kl[(2 * c + half) ^ x]);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], sc, 0, 0, 0);
+        }
+    };
     if (u0 < u1) {
-        put_chunk(0);
-        load_chunk(min(u0 + 1, u1 - 1));
+        put_keys(0);
+        put_values(0);
+        load_keys(min(u0 + 1, u1 - 1));
+        load_values(min(u0 + 1, u1 - 1));
         load_pages(min(u0 + 2, u1 - 1));
+        __syncthreads();
+        if (!blind(u0)) scores(0, 0);
+        if (kTurns && wave >= 4) __syncthreads();
     }
     for (int u = u0; u < u1; u++) {
-        const int buf = (u - u0) & 1;
-        __syncthreads();
-        if (u + 1 < u1) {
-            put_chunk(buf ^ 1);
-            load_chunk(min(u + 2, u1 - 1));
-            load_pages(min(u + 3, u1 - 1));
-        }
-        const int j0 = ap_chunk(S, u) * 64;
-        // nothing here for this wave's rows
-        if (idle || (j0 >= S.prefix && (j0 > W.p_hi || (A.window && j0 + 63 <= W.p_lo - A.window)))) continue;
-
-        const bool whole = ap_whole(A, W, j0, 64);
-        const int key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
-        const int x = KC % 16 ? (col >> 1) & 7 : col & 15, y = (col >> 1) & 7;
-#pragma unroll 1
+        const int buf = (u - u0) & 1, j0 = ap_chunk(S, u) * 64;
+        const bool skip = blind(u), whole = ap_whole(A, W, j0, 64);
+#pragma unroll
         for (int i = 0; i < 2; i++) {
-            const uint4 *kl = k_lds[buf][32 * i + key];
-            ap_f16 sc;
+            // weights of the half's 32 keys, and a part of the next chunk
+            ap_h8 ph[2], pl[2];
+            if (!skip) {
+                // scores in log2 units are sc * f; the factor is kept above zero,
+                // so that it leaves -inf as it is, and is a number where no key is seen
+                const float ksc = s_lds[buf][2 * i + half];
+                float vsc = s_lds[buf][4 + 2 * i + half], f = fmaxf(f_row * ksc, 0x1p-120f);
+                if (A.cap != 0.0f) {
+                    const float fc = fc_row * ksc;
 #pragma unroll
-            for (int e = 0; e < 16; e++) sc[e] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NS; c++) {
-                const ap_h8 a = __builtin_bit_cast(ap_h8, kl[(2 * c + half) ^ x]);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], sc, 0, 0, 0);
-            }
-            // scores in log2 units are sc * f; the factor is kept above zero, so
-            // that it leaves -inf as it is, and is a number where no key is seen
-            const float ksc = s_lds[buf][2 * i + half];
-            float vsc = s_lds[buf][4 + 2 * i + half], f = fmaxf(f_row * ksc, 0x1p-120f);
-            if (A.cap != 0.0f) {
-                const float fc = fc_row * ksc;
-#pragma unroll
-                for (int e = 0; e < 16; e++) sc[e] = ap_capped(A, sc[e] * f, sc[e] * fc);
-                f = 1.0f;
-            }
-            const int j1 = j0 + 32 * i + 16 * half;
-            if (A.slopes) {
-                const float far = (float)(j1 - p), base = slope * far;
-                if (j0 + 63 <= W.p_lo) {  // no key behind a row's own
-#pragma unroll
-                    for (int e = 0; e < 16; e++) sc[e] = fmaf(sc[e], f, fmaf(slope, (float)e, base));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) sc[e] = fmaf(sc[e], f, -slope * fabsf(far + (float)e));
+                    for (int e = 0; e < 16; e++) sc[e] = ap_capped(A, sc[e] * f, sc[e] * fc);
+                    f = 1.0f;
                 }
-                f = 1.0f;
-            }
-            if (!whole || __any(vsc < 0.0f)) {
-                const uint32_t hidden = vsc < 0.0f ? 0xffffu : ap_hidden(A, S, p, j1);
+                const int j1 = j0 + 32 * i + 16 * half;
+                if (A.slopes) {
+                    const float far = (float)(j1 - p), base = slope * far;
+                    if (j0 + 63 <= W.p_lo) {  // no key behind a row's own
 #pragma unroll
-                for (int e = 0; e < 16; e++) sc[e] = ap_hide(sc[e], hidden, e);
-                vsc = hidden != 0xffffu ? vsc : 0.0f;
-            }
-            float mx = sc[0];
+                        for (int e = 0; e < 16; e++) sc[e] = fmaf(sc[e], f, fmaf(slope, (float)e, base));
+                    } else {
 #pragma unroll
-            for (int e = 1; e < 16; e++) mx = fmaxf(mx, sc[e]);
-            mx = ap_max_halves(mx * f);
-            const float top = ap_max_halves(ap_power(vsc));
-            if (__any(mx > m + kApLate || top > ref)) {
-                const float m2 = fmaxf(m, mx), r2 = fmaxf(ref, top), am = __builtin_amdgcn_exp2f(m - m2), ao = am * (ref / r2);
-                l *= am;
-#pragma unroll
-                for (int d = 0; d < ND; d++) o[d] *= ao;
-                m = m2;
-                ref = r2;
-                over = kApUnit / ref;
-            }
-            const float w = vsc * over;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                ap_h8 ph, pl;
-                float pr[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    pr[j] = __builtin_amdgcn_exp2f(fmaf(sc[8 * e + j], f, -m));
-                    l += pr[j];
+                        for (int e = 0; e < 16; e++) sc[e] = fmaf(sc[e], f, -slope * fabsf(far + (float)e));
+                    }
+                    f = 1.0f;
                 }
-                ap_split8w(pr, w, ph, pl);
+                if (!whole || __any(vsc < 0.0f)) {
+                    const uint32_t hidden = vsc < 0.0f ? 0xffffu : ap_hidden(A, S, p, j1);
 #pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const ap_h8 a = __builtin_bit_cast(ap_h8, v_lds[buf][32 * d + col][(4 * i + 2 * half + e) ^ y]);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl, o[d], 0, 0, 0);
+                    for (int e = 0; e < 16; e++) sc[e] = ap_hide(sc[e], hidden, e);
+                    vsc = hidden != 0xffffu ? vsc : 0.0f;
+                }
+                float mx = sc[0];
+#pragma unroll
+                for (int e = 1; e < 16; e++) mx = fmaxf(mx, sc[e]);
+                mx = ap_max_halves(mx * f);
+                const float top = ap_max_halves(ap_power(vsc));
+                if (__any(mx > m + kApLate || top > ref)) {
+                    const float m2 = fmaxf(m, mx), r2 = fmaxf(ref, top), am = __builtin_amdgcn_exp2f(m - m2), ao = am * (ref / r2);
+                    l *= am;
+#pragma unroll
+                    for (int d = 0; d < ND; d++) o[d] *= ao;
+                    m = m2;
+                    ref = r2;
+                    over = kApUnit / ref;
+                }
+                const float w = vsc * over;
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float pr[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        pr[j] = __builtin_amdgcn_exp2f(fmaf(sc[8 * e + j], f, -m));
+                        l += pr[j];
+                    }
+                    ap_split8w(pr, w, ph[e], pl[e]);
                 }
             }
+            if (i == 0) {
+                if (u + 1 < u1) put_keys(buf ^ 1);
+                load_keys(min(u + 2, u1 - 1));
+            } else {
+                if (u + 1 < u1) put_values(buf ^ 1);
+                load_values(min(u + 2, u1 - 1));
+                load_pages(min(u + 3, u1 - 1));
+            }
+            __syncthreads();
+            // their products with the values, and the next half's scores
+            if (!skip) {
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int d = 0; d < ND; d++) {
+                        const ap_h8 a = __builtin_bit_cast(ap_h8, v_lds[buf][32 * d + col][(4 * i + 2 * half + e) ^ y]);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[e], o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[e], o[d], 0, 0, 0);
+                    }
+                if (i == 0) scores(buf, 1);
+            }
+            if (i == 1 && u + 1 < u1 && !blind(u + 1)) scores(buf ^ 1, 0);
+            __syncthreads();
         }
     }
+    if (kTurns && u0 < u1 && wave < 4) __syncthreads();
     l += __shfl_xor(l, 32);
 
     const float back = ref * (1.0f / kApUnit);

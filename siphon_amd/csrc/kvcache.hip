@@ -174,29 +174,116 @@ namespace {
 // counters at the front of a caller's workspace, whatever the call's size
 constexpr size_t kCounterBytes = (size_t)kGemmCounters * 4;
 
-struct AttnPPlan {
+// One launch: the kernel for few rows of a request (16-row blocks) or the one
+// for many (blocks of 128 or 256).
+struct AttnPLaunch {
     AttnPArgs A;
-    int waves;  // of 32 rows in a large row block, 0: 16-row blocks
-    int row_waves;  // waves that share a 16-row block's chunks
-    int64_t blocks, items;  // row blocks, and those times the KV heads
-    int64_t gx;             // of the grid
-    int block_rows;
-    size_t part_bytes;
+    int waves = 0;      // of 32 rows in a large row block, 0: 16-row blocks
+    int row_waves = 0;  // waves that share a 16-row block's chunks
+    int64_t blocks = 0, gx = 0, pieces = 0;  // row blocks, the grid, parts of split blocks
+    size_t part_bytes = 0;
 };
 
-// Waves of 32 rows in a row block of the prompt kernel, 0: 16-row blocks.
-int attn_waves(const sihip_ctx *ctx, const AttnPArgs &A, int64_t rows) {
+struct AttnPPlan {
+    AttnPLaunch l[2];
+    int n = 0;
+    size_t part_bytes() const { return (n > 0 ? l[0].part_bytes : 0) + (n > 1 ? l[1].part_bytes : 0); }
+};
+
+// Rows of a request up to which it counts as one with few, where a batch has both.
+constexpr int kApFewRows = 64;
+
+// Waves of a large row block, 0: 16-row blocks throughout. The work is 16-row
+// blocks times 64-key chunks (as far as the host knows the lengths: bounds)
+// times the head's width. us, 16-row blocks against the large ones:
+//   32 heads of 128: 512 rows 23 / 40, 1024 50 / 63, 1500 88 / 91, 2500 190 / 143;
+//     512 behind 4000 keys 126 / 92, 128 behind 4000 37 / 37; window of 512 142 / 122
+//   14 heads of 64 on 2: 1200 28 / 34, 4096 137 / 125; 32 on 8: 4096 247 / 170
+//   wider than 128 the large blocks' sums leave one wave a SIMD: 16 heads of 256,
+//     4096 rows 478 / 627
+// Eight waves where their blocks, split by 512 keys, leave no CU idle (two groups
+// of four take turns, attnp.h: 512 rows behind 4000 keys 92 against 105, 4096
+// 278 against 304), four below that (1500 rows 91 against 97) and for heads up
+// to 64, of which three workgroups fit a CU (4096 rows: 170 against 210).
+int attn_waves(const sihip_ctx *ctx, const AttnPArgs &A, int64_t rows, int64_t all_rows) {
+    if (A.C.hd > 128) return 0;
     const int64_t o = ctx->opt.attnp_waves;
-    if (o == 0 || ((o == 2 || o == 4 || o == 8) && (A.C.hd <= 128 || o == 4))) return (int)o;
+    if (o == 0 || o == 4 || o == 8) return (int)o;
     if (rows <= 32) return 0;
-    return rows <= 1024 || A.C.hd > 128 ? 4 : 8;
+    int64_t keys = A.R.max_kv - A.R.max_q / 2;  // of a row, on average, without a window
+    if (A.window) keys = std::min<int64_t>(keys, (int64_t)A.window + 64);
+    const double work = (double)(all_rows / 16 * A.C.n_kv) * ((double)keys / 64) * A.C.hd;
+    if (work < 45e3 * 128) return 0;
+    const int64_t pieces = (all_rows / 256 + A.n_req) * A.C.n_kv * std::max<int64_t>(1, A.R.max_kv / 512);
+    return A.C.hd > 64 && pieces >= 2 * ctx->n_cu ? 8 : 4;
+}
+
+// Blocks, pieces and grid of a launch over requests of up to `rows` rows,
+// `all_rows` together.
+int plan_launch(sihip_ctx *ctx, AttnPLaunch &L, int64_t rows, int64_t all_rows) {
+    AttnPArgs &A = L.A;
+    const int block_rows = L.waves ? 32 * L.waves : kApRows;
+    A.n_tiles = (int)((rows + block_rows - 1) / block_rows);
+    // row blocks of all requests: as many as the longest has each, and, listed,
+    // no more than the step's rows fill
+    L.blocks = (int64_t)A.n_req * A.n_tiles;
+    if (A.placed) L.blocks = std::min(L.blocks, all_rows / block_rows + A.n_req);
+    const int64_t items = L.blocks * A.C.n_kv;
+    A.chunk = L.waves || A.C.hd <= 128 ? 6 : 5;
+    const int64_t chunks = std::max<int64_t>(1, ((int64_t)A.R.max_kv + (1 << A.chunk) - 1) >> A.chunk);
+    const int64_t forced = ctx->opt.attnp_splits;
+    if (L.waves || !A.placed) {
+        // splits of a row block's keys: until every CU has its workgroups, none
+        // shorter than four chunks
+        L.row_waves = 4;
+        const int64_t per_cu = L.waves ? 8 / L.waves : 4;
+        int64_t n = (per_cu * ctx->n_cu + items - 1) / std::max<int64_t>(items, 1);
+        if (forced > 0) n = forced;
+        n = std::max<int64_t>(1, std::min<int64_t>(n, 64));
+        A.per_split = (int)std::max<int64_t>((chunks + n - 1) / n, forced > 0 ? 1 : 4);
+        A.n_split = (int)((chunks + A.per_split - 1) / A.per_split);
+        A.whole = 0;
+        L.pieces = items * A.n_split;
+        L.gx = L.waves ? (A.placed ? L.blocks : A.n_tiles) * A.C.n_kv : (int64_t)A.n_tiles * A.n_split;
+    } else {
+        // Four waves share a piece, or, where there are row blocks enough, each
+        // has its own. Workgroups that the pieces are made for: one a CU for few
+        // long requests (32 heads of 128 over 131072 keys 55 us, 65 with 1.5 a
+        // CU), more where lengths differ (64 requests of up to 8192 keys 95 us with
+        // one, 90 with three; 16 of 16000 with 8 heads 71, 58 with 1.5). The row
+        // blocks of prompts fill the CUs by themselves, and are as long as each
+        // other (128 rows behind 4000 keys 37 us with one, 52 with three).
+        const int64_t w = ctx->opt.attnp_row_waves;
+        L.row_waves = w == 1 || w == 4 || w == 8 ? (int)w : items >= 4 * ctx->n_cu ? 1 : 4;
+        A.slots = (A.R.max_q > 1 ? (L.row_waves == 1 ? 8 : 2) : L.row_waves == 1 ? 16 : items < 64 ? 2 : items < 256 ? 3 : 6) *
+                  ctx->n_cu / 2;
+        A.per_split = L.row_waves == 1 ? 6 : L.row_waves;
+        A.whole = L.row_waves == 1 ? 8 : 2 * L.row_waves;
+        if (forced > 0) {
+            A.slots = (int)std::min<int64_t>(forced * std::max<int64_t>(items, 1), 1 << 20);
+            A.per_split = 1;
+            A.whole = 0;
+        }
+        A.n_split = chunks > std::max(A.whole, A.per_split) ? INT32_MAX : 1;
+        L.pieces = items + A.slots;
+        // pieces join by counters, one for each at most
+        if (L.pieces > kGemmCounters) {
+            A.n_split = 1;
+            A.per_split = INT32_MAX;
+        }
+        L.gx = A.n_split > 1 ? L.pieces : items;
+    }
+    L.part_bytes = A.n_split > 1 ? (size_t)L.pieces * block_rows * (A.C.hd / 4 + 1) * 16 : 0;
+    if (L.gx * 512 > UINT32_MAX)
+        return set_err(ctx, SIHIP_EINVAL, "attn_paged_dev: max_q %d of %d heads has no grid", A.R.max_q, A.G * A.C.n_kv);
+    return SIHIP_OK;
 }
 
 int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch *batch, const sihip_attn_paged *a,
               AttnPPlan &P) {
     const char *fn = "attn_paged_dev";
     if (!ctx || !a) return set_err(ctx, SIHIP_EINVAL, "%s: NULL argument", fn);
-    AttnPArgs &A = P.A;
+    AttnPArgs A = {};
     int rc = check_cache(ctx, fn, cache, A.C);
     if (!rc) rc = check_batch(ctx, fn, batch, cache->block, A.R);
     if (rc) return rc;
@@ -211,8 +298,13 @@ int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch 
         return set_err(ctx, SIHIP_EINVAL, "%s: kq_scale %g or softcap %g", fn, (double)a->kq_scale,
                        (double)a->softcap);
     if (a->window < 0) return set_err(ctx, SIHIP_EINVAL, "%s: window %lld", fn, (long long)a->window);
-    if (A.R.max_q > 0 && (!a->q || !a->out || !aligned(a->q, 4) || !aligned(a->out, 4)))
+    if (A.R.max_q == 0) return SIHIP_OK;
+    if (!a->q || !a->out || !aligned(a->q, 4) || !aligned(a->out, 4))
         return set_err(ctx, SIHIP_EINVAL, "%s: q and out must be f32 arrays", fn);
+    A.G = (int)(a->n_head / A.C.n_kv);
+    const int64_t rows = (int64_t)A.R.max_q * A.G, all_rows = A.R.n_tok * A.G;
+    if (rows > INT32_MAX)
+        return set_err(ctx, SIHIP_EINVAL, "%s: max_q %d times %d heads a KV head pass 2^31 rows", fn, A.R.max_q, A.G);
     A.q = a->q;
     A.out = a->out;
     A.ldq = a->ldq;
@@ -222,71 +314,62 @@ int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch 
     A.slopes = a->slopes;
     A.prefix = a->prefix;
     A.n_req = (int)batch->n_req;
-    A.G = (int)(a->n_head / A.C.n_kv);
     A.window = (int)std::min<int64_t>(a->window, INT32_MAX);
-    const double scale = std::fabs((double)a->kq_scale);
+    const double scale = std::fabs((double)a->kq_scale), log2e = 1.4426950408889634;
     A.sign = a->kq_scale < 0 ? -1.0f : 1.0f;
-    A.scale2 = (float)(scale * 1.4426950408889634);
-    A.cap = (float)((double)a->softcap * 1.4426950408889634);
-    A.cap_in = a->softcap > 0 ? (float)(2.0 * scale / a->softcap * 1.4426950408889634) : 0.0f;
-    const int64_t rows = (int64_t)A.R.max_q * A.G;
-    P.waves = attn_waves(ctx, A, rows);
-    const int block_rows = P.waves ? 32 * P.waves : kApRows;
-    A.n_tiles = (int)((rows + block_rows - 1) / block_rows);
-    // row blocks of all requests: as many as the longest has each, or, listed
-    // (ap_place), no more than the step's rows fill
-    P.blocks = (int64_t)A.n_req * A.n_tiles;
+    A.scale2 = (float)(scale * log2e);
+    A.cap = (float)((double)a->softcap * log2e);
+    A.cap_in = a->softcap > 0 ? (float)(2.0 * scale / a->softcap * log2e) : 0.0f;
     A.placed = A.n_req <= 64 * kPlaceRegs;
-    if (A.placed && P.waves) P.blocks = std::min(P.blocks, A.R.n_tok * A.G / block_rows + A.n_req);
-    P.items = P.blocks * A.C.n_kv;
-    A.chunk = P.waves || A.C.hd <= 128 ? 6 : 5;
-    const int64_t chunks = std::max<int64_t>(1, ((int64_t)A.R.max_kv + (1 << A.chunk) - 1) >> A.chunk);
-    const int64_t forced = ctx->opt.attnp_splits;
-    int64_t pieces = 0;
-    if (P.waves || !A.placed) {
-        // splits of a row block's keys: until every CU has its workgroups, none
-        // shorter than a chunk per wave
-        P.row_waves = 4;
-        const int64_t per_cu = P.waves ? std::max(1, 8 / P.waves) : 4;
-        int64_t n = (per_cu * ctx->n_cu + P.items - 1) / std::max<int64_t>(P.items, 1);
-        if (forced > 0) n = forced;
-        n = std::max<int64_t>(1, std::min<int64_t>(n, 64));
-        A.per_split = (int)std::max<int64_t>((chunks + n - 1) / n, forced > 0 ? 1 : 4);
-        A.n_split = (int)((chunks + A.per_split - 1) / A.per_split);
-        A.whole = 0;
-        pieces = P.items * A.n_split;
-    } else {
-        // Four waves share a piece, or, where there are row blocks enough, each
-        // has its own. Workgroups that the pieces are made for: one a CU for few
-        // long requests (32 heads of 128 over 131072 keys 55 us, 65 with 1.5 a
-        // CU), more where lengths differ (64 requests of up to 8192 keys 95 us with
-        // one, 90 with three; 16 of 16000 with 8 heads 71, 58 with 1.5).
-        const int64_t w = ctx->opt.attnp_row_waves;
-        P.row_waves = w == 1 || w == 4 || w == 8 ? (int)w : P.items >= 4 * ctx->n_cu ? 1 : 4;
-        A.slots = (P.row_waves == 1 ? 16 : P.items < 64 ? 2 : P.items < 256 ? 3 : 6) * ctx->n_cu / 2;
-        A.per_split = P.row_waves;
-        A.whole = 2 * P.row_waves;
-        if (forced > 0) {
-            A.slots = (int)std::min<int64_t>(forced * std::max<int64_t>(P.items, 1), 1 << 20);
-            A.per_split = 1;
-            A.whole = 0;
+    A.least = 0;
+    A.most = INT32_MAX;
+    P.l[0].A = A;
+    P.l[0].waves = attn_waves(ctx, A, rows, all_rows);
+    P.n = 1;
+    // Lengths that differ: a request of few rows would fill little of a large
+    // block, and go through all its keys in it alone
+    if (P.l[0].waves && A.placed && A.n_req > 1 && A.R.n_tok < (int64_t)A.n_req * A.R.max_q && rows > kApFewRows) {
+        P.l[0].A.least = kApFewRows + 1;
+        P.l[1].A = A;
+        P.l[1].A.most = kApFewRows;
+        P.n = 2;
+        rc = plan_launch(ctx, P.l[1], kApFewRows, std::min<int64_t>(all_rows, (int64_t)A.n_req * kApFewRows));
+        if (rc) return rc;
+    }
+    return plan_launch(ctx, P.l[0], rows, all_rows);
+}
+
+int launch_attn(sihip_ctx *ctx, const AttnPLaunch &L, hipStream_t st) {
+    const AttnPArgs &A = L.A;
+    const int hd = A.C.hd, z = A.placed ? 1 : A.n_req;
+    if (L.waves) {
+        const dim3 grid((unsigned)L.gx, (unsigned)A.n_split, (unsigned)z), t(L.waves * 64);
+#define SIHIP_APT(NS)                                                                         \
+    if (L.waves == 4) hipLaunchKernelGGL((attnp_tiles_kernel<NS, 4>), grid, t, 0, st, A);     \
+    else hipLaunchKernelGGL((attnp_tiles_kernel<NS, 8>), grid, t, 0, st, A);
+        if (hd <= 64) { SIHIP_APT(4) }
+        else if (hd <= 96) { SIHIP_APT(6) }
+        else { SIHIP_APT(8) }
+#undef SIHIP_APT
+        if (A.n_split > 1) {
+            const int per_wg = kApJoinThreads / (32 * L.waves);  // four-dim columns
+            const dim3 jg((unsigned)L.gx, (unsigned)((hd / 4 + per_wg - 1) / per_wg), (unsigned)z);
+            if (L.waves == 4) hipLaunchKernelGGL(attnp_join_kernel<128>, jg, dim3(kApJoinThreads), 0, st, A);
+            else hipLaunchKernelGGL(attnp_join_kernel<256>, jg, dim3(kApJoinThreads), 0, st, A);
         }
-        A.n_split = chunks > std::max(A.whole, A.per_split) ? INT32_MAX : 1;
-        pieces = P.items + A.slots;
+    } else {
+        const dim3 grid((unsigned)L.gx, A.placed ? 1u : (unsigned)A.C.n_kv, (unsigned)z), t(L.row_waves * 64);
+#define SIHIP_APR(NK, TT)                                                                                  \
+    if (L.row_waves == 1) hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 1>), grid, t, 0, st, A);           \
+    else if (L.row_waves == 4) hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 4>), grid, t, 0, st, A);      \
+    else hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 8>), grid, t, 0, st, A);
+        if (hd <= 64) { SIHIP_APR(1, 4) }
+        else if (hd <= 128) { SIHIP_APR(2, 4) }
+        else if (hd <= 192) { SIHIP_APR(3, 2) }
+        else { SIHIP_APR(4, 2) }
+#undef SIHIP_APR
     }
-    // 16-row blocks join by counters, one for each piece at most
-    if (!P.waves && pieces > kGemmCounters) {
-        A.n_split = 1;
-        A.per_split = INT32_MAX;
-    }
-    P.block_rows = block_rows;
-    P.part_bytes = A.n_split > 1 ? (size_t)pieces * block_rows * (A.C.hd / 4 + 1) * 16 : 0;
-    A.part = nullptr;
-    P.gx = P.waves ? (A.placed ? P.blocks : A.n_tiles) * A.C.n_kv : A.placed ? (A.n_split > 1 ? pieces : P.items) : (int64_t)A.n_tiles * A.n_split;
-    if (P.gx * 512 > UINT32_MAX)
-        return set_err(ctx, SIHIP_EINVAL, "%s: max_q %d of %lld heads has no grid", fn, A.R.max_q,
-                       (long long)a->n_head);
-    return SIHIP_OK;
+    return launched(ctx, "attn_paged");
 }
 
 }  // namespace
@@ -297,7 +380,7 @@ extern "C" int sihip_attn_paged_workspace(sihip_ctx *ctx, const sihip_kv_cache *
     AttnPPlan P;
     const int rc = plan_attn(ctx, cache, batch, args, P);
     if (rc) return rc;
-    *bytes = P.part_bytes ? kCounterBytes + P.part_bytes : 0;
+    *bytes = P.part_bytes() ? kCounterBytes + P.part_bytes() : 0;
     return SIHIP_OK;
 }
 
@@ -305,63 +388,36 @@ extern "C" int sihip_attn_paged_dev(sihip_ctx *ctx, const sihip_kv_cache *cache,
                                     const sihip_attn_paged *args, void *stream) {
     AttnPPlan P;
     int rc = plan_attn(ctx, cache, batch, args, P);
-    if (rc) return rc;
-    AttnPArgs &A = P.A;
-    if (A.R.max_q == 0) return SIHIP_OK;
+    if (rc || P.n == 0) return rc;
     const OnDevice on(ctx->device);
     const hipStream_t st = (hipStream_t)stream;
-    const bool shared = A.n_split > 1 && !args->workspace;
+    const size_t bytes = P.part_bytes();
+    const bool shared = bytes && !args->workspace;
+    uint32_t *cnt = nullptr;
+    uint8_t *part = nullptr;
     if (shared) {
         try {
-            rc = ensure(ctx, &ctx->d_attn, &ctx->d_attn_cap, P.part_bytes, st);
+            rc = ensure(ctx, &ctx->d_attn, &ctx->d_attn_cap, bytes, st);
         } catch (...) {
             rc = set_err(ctx, SIHIP_ENOMEM, "attn_paged_dev: out of host memory");
         }
         if (!rc) rc = order_before(ctx, ctx->order, st);
         if (rc) return rc;
-        A.cnt = ctx->d_gcnt;
-        A.part = (float *)ctx->d_attn;
-    } else if (A.n_split > 1) {
-        if (args->workspace_bytes < kCounterBytes + P.part_bytes || !aligned(args->workspace, 16))
+        cnt = ctx->d_gcnt;
+        part = (uint8_t *)ctx->d_attn;
+    } else if (bytes) {
+        if (args->workspace_bytes < kCounterBytes + bytes || !aligned(args->workspace, 16))
             return set_err(ctx, SIHIP_EINVAL, "attn_paged_dev: a workspace of %zu bytes, 16-byte aligned, is needed",
-                           kCounterBytes + P.part_bytes);
-        A.cnt = (uint32_t *)args->workspace;
-        A.part = (float *)((uint8_t *)args->workspace + kCounterBytes);
+                           kCounterBytes + bytes);
+        cnt = (uint32_t *)args->workspace;
+        part = (uint8_t *)args->workspace + kCounterBytes;
     }
-    const int hd = A.C.hd;
-    if (P.waves) {
-        const dim3 grid((unsigned)P.gx, (unsigned)A.n_split, A.placed ? 1u : (unsigned)A.n_req), t(P.waves * 64);
-#define SIHIP_APT(NS)                                                                         \
-    if (P.waves == 2) hipLaunchKernelGGL((attnp_tiles_kernel<NS, 2>), grid, t, 0, st, A);     \
-    else if (P.waves == 4) hipLaunchKernelGGL((attnp_tiles_kernel<NS, 4>), grid, t, 0, st, A); \
-    else hipLaunchKernelGGL((attnp_tiles_kernel<NS, 8>), grid, t, 0, st, A);
-        if (hd <= 64) { SIHIP_APT(4) }
-        else if (hd <= 96) { SIHIP_APT(6) }
-        else if (hd <= 128) { SIHIP_APT(8) }
-        else if (hd <= 192) hipLaunchKernelGGL((attnp_tiles_kernel<12, 4>), grid, t, 0, st, A);
-        else hipLaunchKernelGGL((attnp_tiles_kernel<16, 4>), grid, t, 0, st, A);
-#undef SIHIP_APT
-    } else {
-        const dim3 grid((unsigned)P.gx, A.placed ? 1u : (unsigned)A.C.n_kv, A.placed ? 1u : (unsigned)A.n_req), t(P.row_waves * 64);
-#define SIHIP_APR(NK, TT)                                                                                  \
-    if (P.row_waves == 1) hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 1>), grid, t, 0, st, A);           \
-    else if (P.row_waves == 4) hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 4>), grid, t, 0, st, A);      \
-    else hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 8>), grid, t, 0, st, A);
-        if (hd <= 64) { SIHIP_APR(1, 4) }
-        else if (hd <= 128) { SIHIP_APR(2, 4) }
-        else if (hd <= 192) { SIHIP_APR(3, 2) }
-        else { SIHIP_APR(4, 2) }
-#undef SIHIP_APR
+    for (int i = 0; i < P.n; i++) {
+        P.l[i].A.cnt = cnt;
+        P.l[i].A.part = (float *)part;
+        part += P.l[i].part_bytes;
+        rc = launch_attn(ctx, P.l[i], st);
+        if (rc) return rc;
     }
-    if (P.waves && A.n_split > 1) {
-        const int per_wg = kApJoinThreads / P.block_rows;  // four-dim columns
-        const dim3 grid((unsigned)((A.placed ? P.blocks : A.n_tiles) * A.C.n_kv), (unsigned)((hd / 4 + per_wg - 1) / per_wg),
-                        A.placed ? 1u : (unsigned)A.n_req), t(kApJoinThreads);
-        if (P.block_rows == 64) hipLaunchKernelGGL(attnp_join_kernel<64>, grid, t, 0, st, A);
-        else if (P.block_rows == 128) hipLaunchKernelGGL(attnp_join_kernel<128>, grid, t, 0, st, A);
-        else hipLaunchKernelGGL(attnp_join_kernel<256>, grid, t, 0, st, A);
-    }
-    rc = launched(ctx, "attn_paged");
-    if (rc) return rc;
     return shared ? order_after(ctx, ctx->order, st) : SIHIP_OK;
 }
