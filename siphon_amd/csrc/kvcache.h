@@ -15,7 +15,6 @@ namespace sihip {
 
 // ---- the plan of a step --------------------------------------------------------
 
-constexpr int kPlanThreads = 1024;
 constexpr int64_t kMaxRequests = 4096;  // three prefix arrays of them fit 48 KiB of LDS
 
 struct PlanArgs {
@@ -58,16 +57,21 @@ __device__ inline PlanSum plan_request(const PlanArgs &A, int r, int &bad, int &
 // spread over the grid and find their request by bisection in LDS. Nothing
 // that a workgroup reads is written in the same launch: list entries at and
 // past n_free and table entries of new blocks are only written.
-__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs A) {
+//
+// Nothing but dependent loads bounds it: 64 requests with a token each take
+// 6.0 us, 1000 with 24600 tokens 8.9 us, a launch with nothing to do 3.5 us.
+// With 1024 threads the 64 take 6.3 us.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_plan_kernel(PlanArgs A) {
     extern __shared__ int32_t plan_lds[];
-    __shared__ PlanSum wave_sum[kPlanThreads / 64];
-    __shared__ int wave_bad[kPlanThreads / 64];
+    __shared__ PlanSum wave_sum[THREADS / 64];
+    __shared__ int wave_bad[THREADS / 64];
     int32_t *tok0 = plan_lds, *need0 = tok0 + A.n_req, *back0 = need0 + A.n_req;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int n_free = *A.n_free;
 
     // exclusive prefix sums: a span of requests per thread
-    const int per = (A.n_req + kPlanThreads - 1) / kPlanThreads;
+    const int per = (A.n_req + THREADS - 1) / THREADS;
     const int r0 = min(tid * per, A.n_req), r1 = min(r0 + per, A.n_req);
     int bad = 0, unused;
     PlanSum own = {0, 0, 0};
@@ -83,7 +87,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs A) {
     __syncthreads();
     PlanSum before = {0, 0, 0}, all = {0, 0, 0};
     int status = 0;
-    for (int w = 0; w < kPlanThreads / 64; w++) {
+    for (int w = 0; w < THREADS / 64; w++) {
         if (w == wave) before = all;
         all = all + wave_sum[w];
         status |= wave_bad[w];
@@ -139,8 +143,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs A) {
         const int r = find(back0, i - n_free);
         return A.table[(int64_t)r * A.max_blocks + (i - n_free - back0[r])];
     };
-    const int64_t step = (int64_t)gridDim.x * kPlanThreads;
-    const int64_t first = (int64_t)blockIdx.x * kPlanThreads + tid;
+    const int64_t step = (int64_t)gridDim.x * THREADS;
+    const int64_t first = (int64_t)blockIdx.x * THREADS + tid;
     if (!status)
         for (int64_t i = n_free + first; i < n_out; i += step) A.free_pages[i] = list((int)i);
     const int top = (int)(n_free + all.back) - 1;
@@ -196,14 +200,12 @@ __device__ inline Span request_span(const BatchArgs &A, int r) {
 
 // ---- append ------------------------------------------------------------------------
 
-constexpr int kAppendThreads = 256;
-
 struct AppendArgs {
     CacheArgs C;
     BatchArgs R;
     const float *k, *v;
     int64_t ldk, ldv;
-    int blocks;  // most blocks of a request that get new tokens
+    bool k_wide;  // rows of k and their heads are 16-byte aligned
 };
 
 // Magnitudes below this count as zero, so that a scale's reciprocal and the
@@ -224,6 +226,34 @@ __device__ inline int quantize_exact(float x, float scale, float inv) {
     return (int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
+// 16 values to codes. The sum with 1.5 2^23 leaves the product rounded to an
+// integer, ties to even, in the low bits; what is within 10^-4 of a border (or
+// no number) is rounded exactly, all 16 of the thread.
+__device__ inline void quantize16(const float *x, float scale, float inv, uint32_t *w) {
+    constexpr float kMagic = 12582912.0f;
+    bool clear = true;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t b[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float r = fmaf(x[4 * i + e], inv, kMagic);
+            const float d = fabsf(fmaf(x[4 * i + e], inv, kMagic - r));
+            clear &= d <= 0.4999f;
+            b[e] = __builtin_bit_cast(uint32_t, r);
+        }
+        const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
+        w[i] = lo | hi << 16;
+    }
+    if (clear) return;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        w[i] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[i] |= (uint32_t)(uint8_t)quantize_exact(x[4 * i + e], scale, inv) << (8 * e);
+    }
+}
+
 // code * was / now rounded to an integer, ties to even, exactly: the product
 // of a code and an f32 has 31 bits, so f64 holds it and the remainders.
 __device__ inline int requantize_exact(int code, float was, float now, double inv) {
@@ -241,8 +271,20 @@ __device__ inline int requantize_exact(int code, float was, float now, double in
 // rows over 127, or what it was where that is more; codes of tokens that
 // were there are rounded again when it grows. A page whose first token is new
 // starts from nothing. Bytes behind the last token are left as they are.
-__global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs A) {
-    __shared__ float wave_max[kAppendThreads / 64];
+//
+// A thread has 16 bytes of the page: 16 dims of a token (keys) or 16 tokens of
+// a dim (values, so that the lanes of a wave read a row each time and write
+// whole granules of the transposed page), U times; the f32 values stay in
+// registers from the search for the largest to their rounding.
+//
+// Bound by memory: each new row is read once, each touched page written once.
+// 5 prompt chunks, 5760 rows of 8 heads of 128, pages of 64: 59 MB in 19.5 us
+// (3.0 TB/s); one 16-byte unit a thread, not 2 of half as many threads (22 us),
+// as long as 1024 threads reach. One new token for 64 requests: 7.5 us, of
+// which a launch with nothing to do takes 3.5; the rest are dependent loads.
+template <int U, int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs A) {
+    __shared__ float wave_max[THREADS / 64];
     const int h = blockIdx.x % A.C.n_kv, j = blockIdx.x / A.C.n_kv, r = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
     const int tid = threadIdx.x, B = 1 << A.C.shift, hd = A.C.hd;
@@ -260,40 +302,77 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs A)
     int8_t *codes = (is_v ? A.C.v : A.C.k) + (page * A.C.n_kv + h) * ((int64_t)hd << A.C.shift);
     const float was = lo > 0 ? *sp : 0.0f;
 
-    float top = 0.0f;
-    for (int i = tid; i < (hi - lo) * hd; i += kAppendThreads) {
-        const float a = fabsf(x[(int64_t)(lo + i / hd) * ld + i % hd]);
-        if (a < INFINITY) top = fmaxf(top, a);
+    const int units = (hd << A.C.shift) / 16, per_token = hd / 16;
+    float val[U][16], top = 0.0f;
+    union Codes {
+        uint4 w;
+        int8_t c[16];
+    } buf[U];
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+        const int u = tid + THREADS * i;
+        const int outer = is_v ? u % hd : u / per_token, inner = (is_v ? u / hd : u % per_token) * 16;
+        const int t0 = is_v ? inner : outer, t1 = is_v ? inner + 16 : outer + 1;
+        const bool has_new = u < units && t0 < hi && t1 > lo;
+        if (u < units && t0 < hi && (t0 < lo || t1 > hi)) buf[i].w = *(const uint4 *)(codes + (is_v ? (outer << A.C.shift) + inner : outer * hd + inner));
+        if (!has_new) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) val[i][e] = 0.0f;
+        } else if (is_v) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) val[i][e] = inner + e >= lo && inner + e < hi ? x[(int64_t)(inner + e) * ld + outer] : 0.0f;
+        } else if (A.k_wide) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float4 y = ((const float4 *)(x + (int64_t)outer * ld + inner))[e];
+                val[i][4 * e] = y.x, val[i][4 * e + 1] = y.y, val[i][4 * e + 2] = y.z, val[i][4 * e + 3] = y.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) val[i][e] = x[(int64_t)outer * ld + inner + e];
+        }
     }
+#pragma unroll
+    for (int i = 0; i < U; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const float a = fabsf(val[i][e]);
+            top = fmaxf(top, a < INFINITY ? a : 0.0f);
+        }
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     if ((tid & 63) == 0) wave_max[tid >> 6] = top;
     __syncthreads();
-    for (int w = 0; w < kAppendThreads / 64; w++) top = fmaxf(top, wave_max[w]);
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) top = fmaxf(top, wave_max[w]);
     const float now = fmaxf(was, top < kTinyAmax ? 0.0f : top / 127.0f);
     const bool grew = now > was;
     const float inv = now > 0.0f ? 1.0f / now : 0.0f;
-    const double inv64 = now > 0.0f ? 1.0 / (double)now : 0.0;
 
-    // 16 bytes a thread: dims of one token (keys), tokens of one dim (values)
-    for (int u = tid; u < (hd << A.C.shift) / 16; u += kAppendThreads) {
-        const int outer = is_v ? u % hd : u / (hd / 16);
-        const int inner = (is_v ? u / hd : u % (hd / 16)) * 16;
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+        const int u = tid + THREADS * i;
+        const int outer = is_v ? u % hd : u / per_token, inner = (is_v ? u / hd : u % per_token) * 16;
         const int t0 = is_v ? inner : outer, t1 = is_v ? inner + 16 : outer + 1;
         const bool has_new = t0 < hi && t1 > lo, has_old = t0 < lo;
-        if (!has_new && !(has_old && grew)) continue;
-        int8_t *at = codes + (is_v ? ((int64_t)outer << A.C.shift) + inner : (int64_t)outer * hd + inner);
-        union {
-            uint4 w;
-            int8_t c[16];
-        } buf;
-        if (t0 < lo || t1 > hi) buf.w = *(const uint4 *)at;
+        if (u >= units || !(has_new || (has_old && grew))) continue;
+        if (has_old && grew) {
+            const double inv64 = 1.0 / (double)now;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int t = is_v ? inner + e : outer, d = is_v ? outer : inner + e;
-            if (t >= lo && t < hi) buf.c[e] = (int8_t)quantize_exact(x[(int64_t)t * ld + d], now, inv);
-            else if (t < lo && grew) buf.c[e] = (int8_t)requantize_exact(buf.c[e], was, now, inv64);
+            for (int e = 0; e < 16; e++)
+                if ((is_v ? inner + e : outer) < lo) buf[i].c[e] = (int8_t)requantize_exact(buf[i].c[e], was, now, inv64);
         }
-        *(uint4 *)at = buf.w;
+        Codes q;
+        quantize16(val[i], now, inv, &q.w.x);
+        if (t0 >= lo && t1 <= hi) {
+            buf[i] = q;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int t = is_v ? inner + e : outer;
+                buf[i].c[e] = t >= lo && t < hi ? q.c[e] : buf[i].c[e];
+            }
+        }
+        *(uint4 *)(codes + (is_v ? (outer << A.C.shift) + inner : outer * hd + inner)) = buf[i].w;
     }
     if (tid == 0 && (grew || lo == 0)) *sp = now;
 }
@@ -301,29 +380,125 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs A)
 // ---- read ---------------------------------------------------------------------------
 
 constexpr int kReadThreads = 256;
-constexpr int kReadRows = 16;
 
 struct ReadArgs {
     CacheArgs C;
     const int64_t *slots;
     float *k, *v;
     int64_t n, ldk, ldv;
+    bool wide;  // rows of k and v and their heads are 16-byte aligned
 };
 
-// One workgroup: kReadRows slots of one KV head, keys and values.
+// bytes `from` .. from + 15 of 32
+__device__ inline uint4 read_window(uint4 a, uint4 b, int from) {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int s = 4; s; s >>= 1)
+        if (from & (4 * s))
+#pragma unroll
+            for (int i = 0; i + s < 8; i++) w[i] = w[i + s];
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_alignbyte(w[i + 1], w[i], from & 3);
+    return uint4{o[0], o[1], o[2], o[3]};
+}
+
+// One workgroup: ROWS slots of one KV head, keys (z = 0): four dims of a
+// slot a thread; or values: two dims of 16 slots a thread, so that the lanes of
+// a wave write rows. 16 slots that go on from one another lie in one or two
+// 16-token segments of the transposed pages: two loads a dim. Any others are
+// read byte by byte, all 32 loads of a thread before the first use.
+//
+// Bound by memory: 4 requests of 7000 tokens, 8 heads of 128: 97 MB in 22.5 us
+// (4.3 TB/s, a large copy 4.8); a byte at a time for all slots 43 us. 600
+// tokens of 8 heads of 64: 4.3 us with 16 slots a workgroup, 6.0 with 64.
+template <int ROWS>
 __global__ __launch_bounds__(kReadThreads) void kv_read_kernel(ReadArgs A) {
-    const int h = blockIdx.y, hd = A.C.hd, B = 1 << A.C.shift;
-    const int64_t i0 = (int64_t)blockIdx.x * kReadRows;
-    for (int u = threadIdx.x; u < kReadRows * hd; u += kReadThreads) {
-        const int64_t i = i0 + u / hd;
-        const int d = u % hd;
-        if (i >= A.n) break;
-        const int64_t slot = A.slots[i], page = slot >> A.C.shift;
-        if (slot < 0 || page >= A.C.n_pages) continue;
-        const int off = (int)(slot & (B - 1));
-        const int64_t ph = page * A.C.n_kv + h, at = ph * ((int64_t)hd << A.C.shift);
-        A.k[i * A.ldk + (int64_t)h * hd + d] = (float)A.C.k[at + (int64_t)off * hd + d] * A.C.ks[ph];
-        A.v[i * A.ldv + (int64_t)h * hd + d] = (float)A.C.v[at + ((int64_t)d << A.C.shift) + off] * A.C.vs[ph];
+    __shared__ int64_t at[ROWS];  // first code of the page and head, or -1
+    __shared__ int off[ROWS];     // place in the page
+    __shared__ float scale[ROWS];
+    __shared__ int run[ROWS / 16];  // whether the 16 slots go on from one another
+    const int h = blockIdx.y, hd = A.C.hd, tid = threadIdx.x;
+    const bool is_v = blockIdx.z != 0;
+    const int64_t i0 = (int64_t)blockIdx.x * ROWS;
+    if (tid < ROWS) {
+        const int64_t slot = i0 + tid < A.n ? A.slots[i0 + tid] : -1, page = slot >> A.C.shift;
+        const bool ok = slot >= 0 && page < A.C.n_pages;
+        const int64_t ph = page * A.C.n_kv + h;
+        at[tid] = ok ? ph * ((int64_t)hd << A.C.shift) : -1;
+        off[tid] = (int)(slot & ((1 << A.C.shift) - 1));
+        scale[tid] = ok ? (is_v ? A.C.vs : A.C.ks)[ph] : 0.0f;
+        const int64_t s0 = __shfl(slot, tid & 48);
+        const int left = 16 - (int)(s0 & 15), k = tid & 15;
+        const int64_t s1 = __shfl(slot, (tid & 48) + (left & 15));
+        const bool on = ok && (k < left ? slot == s0 + k : (s1 & 15) == 0 && slot == s1 + k - left);
+        const uint64_t all = __ballot(on);
+        if (k == 0) run[tid >> 4] = (all >> (tid & 48) & 0xffffu) == 0xffffu;
+    }
+    __syncthreads();
+    if (!is_v) {
+        const int per_row = hd / 4;
+#pragma unroll 4
+        for (int u = tid; u < ROWS * per_row; u += kReadThreads) {
+            const int i = u / per_row, d = u % per_row * 4;
+            if (at[i] < 0) continue;
+            const char4 c = *(const char4 *)(A.C.k + at[i] + off[i] * hd + d);
+            float *to = A.k + (i0 + i) * A.ldk + (int64_t)h * hd + d;
+            const float s = scale[i];
+            if (A.wide) {
+                *(float4 *)to = float4{c.x * s, c.y * s, c.z * s, c.w * s};
+            } else {
+                to[0] = c.x * s;
+                to[1] = c.y * s;
+                to[2] = c.z * s;
+                to[3] = c.w * s;
+            }
+        }
+        return;
+    }
+    union Codes {
+        uint4 w;
+        int8_t c[16];
+    };
+    for (int u = tid; u < ROWS / 16 * (hd / 2); u += kReadThreads) {
+        const int first = u / (hd / 2) * 16, d = u % (hd / 2) * 2;
+        float *to = A.v + (i0 + first) * A.ldv + (int64_t)h * hd + d;
+        if (run[first >> 4]) {
+            const int from = off[first] & 15, left = 16 - from, next = first + (left & 15);
+            const int8_t *a = A.C.v + at[first] + (off[first] & ~15) + (d << A.C.shift);
+            const int8_t *b = A.C.v + at[next] + (off[next] & ~15) + (d << A.C.shift);
+            const int step = 1 << A.C.shift;
+            Codes x, y;
+            x.w = read_window(*(const uint4 *)a, *(const uint4 *)b, from);
+            y.w = read_window(*(const uint4 *)(a + step), *(const uint4 *)(b + step), from);
+            const float sa = scale[first], sb = scale[next];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float s = i < left ? sa : sb;
+                if (A.wide) {
+                    *(float2 *)(to + i * A.ldv) = float2{x.c[i] * s, y.c[i] * s};
+                } else {
+                    to[i * A.ldv] = x.c[i] * s;
+                    to[i * A.ldv + 1] = y.c[i] * s;
+                }
+            }
+            continue;
+        }
+        int8_t x[16], y[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            // (a slot that is none reads the first page, and writes nothing)
+            const int64_t from = at[first + i] < 0 ? 0 : at[first + i] + off[first + i];
+            const int8_t *a = A.C.v + from + (d << A.C.shift);
+            x[i] = a[0];
+            y[i] = a[1 << A.C.shift];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            if (at[first + i] < 0) continue;
+            to[i * A.ldv] = x[i] * scale[first + i];
+            to[i * A.ldv + 1] = y[i] * scale[first + i];
+        }
     }
 }
 

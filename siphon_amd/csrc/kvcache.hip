@@ -104,9 +104,12 @@ extern "C" int sihip_kv_plan_dev(sihip_ctx *ctx, const sihip_kv_plan *p, void *s
     const PlanArgs A = {p->len, p->add, p->n_free, p->free_pages, p->table, p->q_start, p->kv_len, p->pos,
                         p->n_free_out, p->status, p->slot, p->n_tok, (int)p->n_req, (int)p->n_pages,
                         (int)p->max_blocks, shift};
-    const int64_t wgs = std::min<int64_t>(std::max<int64_t>(1, (p->n_tok + kPlanThreads - 1) / kPlanThreads), ctx->n_cu);
-    hipLaunchKernelGGL(kv_plan_kernel, dim3((unsigned)wgs), dim3(kPlanThreads), (size_t)p->n_req * 12,
-                       (hipStream_t)stream, A);
+    // few requests need few waves, which start and meet sooner
+    const bool few = p->n_req <= 256;
+    const int64_t threads = few ? 256 : 1024;
+    const int64_t wgs = std::min<int64_t>(std::max<int64_t>(1, (p->n_tok + threads - 1) / threads), ctx->n_cu);
+    hipLaunchKernelGGL(few ? kv_plan_kernel<256> : kv_plan_kernel<1024>, dim3((unsigned)wgs), dim3((unsigned)threads),
+                       (size_t)p->n_req * 12, (hipStream_t)stream, A);
     return launched(ctx, "kv_plan");
 }
 
@@ -128,14 +131,22 @@ extern "C" int sihip_kv_append_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, 
     A.v = v;
     A.ldk = ldk;
     A.ldv = ldv;
-    const int64_t blocks = ((int64_t)A.R.max_q + cache->block - 2) / cache->block + 1;
-    A.blocks = (int)std::min<int64_t>(blocks, A.R.max_blocks);
-    const int64_t gx = (int64_t)A.blocks * A.C.n_kv;
-    if (gx * kAppendThreads > UINT32_MAX)
+    A.k_wide = aligned(k, 16) && ldk % 4 == 0;
+    // blocks of a request that max_q tokens can touch
+    const int64_t blocks = std::min<int64_t>(((int64_t)A.R.max_q + cache->block - 2) / cache->block + 1, A.R.max_blocks);
+    const int64_t gx = blocks * A.C.n_kv;
+    if (gx * 1024 > UINT32_MAX)
         return set_err(ctx, SIHIP_EINVAL, "kv_append_dev: max_q %d of %d heads has no grid", A.R.max_q, A.C.n_kv);
     const OnDevice on(ctx->device);
-    hipLaunchKernelGGL(kv_append_kernel, dim3((unsigned)gx, (unsigned)batch->n_req, 2), dim3(kAppendThreads), 0,
-                       (hipStream_t)stream, A);
+    const dim3 grid((unsigned)gx, (unsigned)batch->n_req, 2);
+    const hipStream_t st = (hipStream_t)stream;
+    const int64_t units = cache->block * A.C.hd / 16;
+    if (units <= 128) hipLaunchKernelGGL((kv_append_kernel<1, 128>), grid, dim3(128), 0, st, A);
+    else if (units <= 256) hipLaunchKernelGGL((kv_append_kernel<1, 256>), grid, dim3(256), 0, st, A);
+    else if (units <= 512) hipLaunchKernelGGL((kv_append_kernel<1, 512>), grid, dim3(512), 0, st, A);
+    else if (units <= 1024) hipLaunchKernelGGL((kv_append_kernel<1, 1024>), grid, dim3(1024), 0, st, A);
+    else if (units <= 2048) hipLaunchKernelGGL((kv_append_kernel<2, 1024>), grid, dim3(1024), 0, st, A);
+    else hipLaunchKernelGGL((kv_append_kernel<4, 1024>), grid, dim3(1024), 0, st, A);
     return launched(ctx, "kv_append");
 }
 
@@ -158,12 +169,16 @@ extern "C" int sihip_kv_read_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, co
     A.n = n;
     A.ldk = ldk;
     A.ldv = ldv;
-    const int64_t gx = (n + kReadRows - 1) / kReadRows;
+    A.wide = aligned(k, 16) && ldk % 4 == 0 && aligned(v, 16) && ldv % 4 == 0;
+    // 64 slots a workgroup use the lines of a page that they load; while those
+    // are too few workgroups to fill the device, 16
+    const bool few = (n + 63) / 64 * A.C.n_kv * 2 < 4 * ctx->n_cu;
+    const int64_t rows = few ? 16 : 64, gx = (n + rows - 1) / rows;
     if (gx * kReadThreads > UINT32_MAX)
         return set_err(ctx, SIHIP_EINVAL, "kv_read_dev: %lld rows have no grid", (long long)n);
     const OnDevice on(ctx->device);
-    hipLaunchKernelGGL(kv_read_kernel, dim3((unsigned)gx, (unsigned)A.C.n_kv), dim3(kReadThreads), 0,
-                       (hipStream_t)stream, A);
+    hipLaunchKernelGGL(few ? kv_read_kernel<16> : kv_read_kernel<64>, dim3((unsigned)gx, (unsigned)A.C.n_kv, 2),
+                       dim3(kReadThreads), 0, (hipStream_t)stream, A);
     return launched(ctx, "kv_read");
 }
 
