@@ -80,9 +80,9 @@ const char *sihip_last_error(const sihip_ctx *ctx);
  * GEMMD_MIN_M (the smallest M on the prompt GEMMs of the K-quants and of the
  * other formats, 0: never), RING_MT and RING_SBK (m tiles and K-slice length of
  * these two), ATTN_FUSE (k: decode attention in one launch up to 512 k
- * positions, at most 1536, 0: never), ATTNP_WAVES (paged attention: 4 or 8
- * waves of 32 rows in a row block, 0: blocks of 16 rows), ATTNP_ROW_WAVES (1, 4
- * or 8 waves that share a 16-row block's keys), ATTNP_SPLITS (splits of a row
+ * positions, at most 1536, 0: never), ATTNP_LARGE (paged attention: 1:
+ * large row blocks, 0: blocks of 16 rows), ATTNP_ROW_WAVES (1 or
+ * 4 waves that share a 16-row block's keys), ATTNP_SPLITS (splits of a row
  * block's keys), and
  * Q80_SCALAR: 1 quantizes Q8_0-pair
  * activations with the reference's portable scalar routine (reference

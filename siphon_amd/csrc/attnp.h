@@ -457,6 +457,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
         tile = (i - before) / parts / A.C.n_kv;
         per = D.per;
         piece = i;
+        // (spans that overlap are more than the grid was made for: what a block
+        // cannot join in it, it does not begin)
+        if (i < split || i - split + parts > (int)gridDim.x) return;
     } else {
         s = request_span(A.R, r);
         // workgroups go to the eight XCDs in turn, and of a ragged batch only the
@@ -797,9 +800,15 @@ __device__ inline bool ap_place(const AttnPArgs &A, int rows, int64_t i, int &r,
     return true;
 }
 
+// Waves of a large row block, heads of up to hd dims: up to 64 three workgroups
+// of four fit a CU and fill each other's gaps (4096 rows of 32 heads: 170 us, two
+// groups that take turns 213); wider ones take turns (256 rows behind 7000 keys
+// 77 us, workgroups of four 84).
+constexpr int ap_tile_waves(int hd) { return hd <= 64 ? 4 : 8; }
+
 // hd rounded up to 16 NS dims
-template <int NS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, NS <= 4 && WAVES == 4 ? 3 : 2) void attnp_tiles_kernel(AttnPArgs A) {
+template <int NS, int WAVES = ap_tile_waves(16 * NS)>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 2) void attnp_tiles_kernel(AttnPArgs A) {
     constexpr int kApTileRows = 32 * WAVES, kApTileThreads = 64 * WAVES;
     constexpr bool kTurns = WAVES == 8;
     constexpr int ND = (NS + 1) / 2;             // 32-dim tiles of the output

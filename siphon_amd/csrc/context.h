@@ -45,8 +45,8 @@ struct Options {
     int64_t ring_mt = -1;      // m tiles of the ring-buffered GEMMs (gemmx.h, gemmd.h), where they have that instance (rule: plan_tiles)
     int64_t ring_sbk = -1;     // their K-slice length in steps, 0: none (rule: plan_tiles)
     int64_t gemm_group = -1;   // Q4_K matrices over one X in one 16x16 GEMM launch, 0: off (rule: on)
-    int64_t attnp_waves = -1;  // paged attention: waves of 32 rows in a row block (4, 8), 0: blocks of 16 rows (rule: attn_waves)
-    int64_t attnp_row_waves = -1; // paged attention: waves that share a 16-row block's keys (1, 4, 8) (rule: plan_launch)
+    int64_t attnp_large = -1;  // paged attention: large row blocks (1), blocks of 16 rows (0) (rule: attn_waves)
+    int64_t attnp_row_waves = -1; // paged attention: waves that share a 16-row block's keys (1, 4) (rule: plan_launch)
     int64_t attnp_splits = -1; // paged attention: splits of a row block's keys, 1..64 (rule: plan_launch)
     int64_t q80_scalar = -1;   // Q8_0 activations by the scalar quantizer (reference
                                // kernels.c:542-558, its SI_SCALAR mode), 1: on (rule: off)

@@ -211,26 +211,21 @@ constexpr int kApFewRows = 64;
 // Waves of a large row block, 0: 16-row blocks throughout. The work is 16-row
 // blocks times 64-key chunks (as far as the host knows the lengths: bounds)
 // times the head's width. us, 16-row blocks against the large ones:
-//   32 heads of 128: 512 rows 23 / 40, 1024 50 / 63, 1500 88 / 91, 2500 190 / 143;
-//     512 behind 4000 keys 126 / 92, 128 behind 4000 37 / 37; window of 512 142 / 122
+//   32 heads of 128: 512 rows 23 / 40, 1024 50 / 63, 1500 88 / 91, 1800 115 / 115,
+//     2048 133 / 120; 190 behind 8000 keys 98 / 105, 256 behind 8000 101 / 83, 64
+//     behind 30000 116 / 74; window of 512 142 / 122
 //   14 heads of 64 on 2: 1200 28 / 34, 4096 137 / 125; 32 on 8: 4096 247 / 170
 //   wider than 128 the large blocks' sums leave one wave a SIMD: 16 heads of 256,
 //     4096 rows 478 / 627
-// Eight waves where their blocks, split by 512 keys, leave no CU idle (two groups
-// of four take turns, attnp.h: 512 rows behind 4000 keys 92 against 105, 4096
-// 278 against 304), four below that (1500 rows 91 against 97) and for heads up
-// to 64, of which three workgroups fit a CU (4096 rows: 170 against 210).
 int attn_waves(const sihip_ctx *ctx, const AttnPArgs &A, int64_t rows, int64_t all_rows) {
     if (A.C.hd > 128) return 0;
-    const int64_t o = ctx->opt.attnp_waves;
-    if (o == 0 || o == 4 || o == 8) return (int)o;
+    const int waves = ap_tile_waves(A.C.hd);
+    if (ctx->opt.attnp_large >= 0) return ctx->opt.attnp_large ? waves : 0;
     if (rows <= 32) return 0;
     int64_t keys = A.R.max_kv - A.R.max_q / 2;  // of a row, on average, without a window
     if (A.window) keys = std::min<int64_t>(keys, (int64_t)A.window + 64);
     const double work = (double)(all_rows / 16 * A.C.n_kv) * ((double)keys / 64) * A.C.hd;
-    if (work < 45e3 * 128) return 0;
-    const int64_t pieces = (all_rows / 256 + A.n_req) * A.C.n_kv * std::max<int64_t>(1, A.R.max_kv / 512);
-    return A.C.hd > 64 && pieces >= 2 * ctx->n_cu ? 8 : 4;
+    return work < 45e3 * 128 ? 0 : waves;
 }
 
 // Blocks, pieces and grid of a launch over requests of up to `rows` rows,
@@ -269,7 +264,7 @@ int plan_launch(sihip_ctx *ctx, AttnPLaunch &L, int64_t rows, int64_t all_rows) 
         // blocks of prompts fill the CUs by themselves, and are as long as each
         // other (128 rows behind 4000 keys 37 us with one, 52 with three).
         const int64_t w = ctx->opt.attnp_row_waves;
-        L.row_waves = w == 1 || w == 4 || w == 8 ? (int)w : items >= 4 * ctx->n_cu ? 1 : 4;
+        L.row_waves = w == 1 || w == 4 ? (int)w : items >= 4 * ctx->n_cu ? 1 : 4;
         A.slots = (A.R.max_q > 1 ? (L.row_waves == 1 ? 8 : 2) : L.row_waves == 1 ? 16 : items < 64 ? 2 : items < 256 ? 3 : 6) *
                   ctx->n_cu / 2;
         A.per_split = L.row_waves == 1 ? 6 : L.row_waves;
@@ -281,12 +276,13 @@ int plan_launch(sihip_ctx *ctx, AttnPLaunch &L, int64_t rows, int64_t all_rows) 
         }
         A.n_split = chunks > std::max(A.whole, A.per_split) ? INT32_MAX : 1;
         L.pieces = items + A.slots;
-        // pieces join by counters, one for each at most
-        if (L.pieces > kGemmCounters) {
-            A.n_split = 1;
-            A.per_split = INT32_MAX;
-        }
         L.gx = A.n_split > 1 ? L.pieces : items;
+    }
+    // pieces of 16-row blocks join by counters, one for each at most
+    if (!L.waves && L.pieces > kGemmCounters) {
+        A.n_split = 1;
+        A.per_split = INT32_MAX;
+        L.gx = A.placed ? items : A.n_tiles;
     }
     L.part_bytes = A.n_split > 1 ? (size_t)L.pieces * block_rows * (A.C.hd / 4 + 1) * 16 : 0;
     if (L.gx * 512 > UINT32_MAX)
@@ -359,13 +355,9 @@ int launch_attn(sihip_ctx *ctx, const AttnPLaunch &L, hipStream_t st) {
     const int hd = A.C.hd, z = A.placed ? 1 : A.n_req;
     if (L.waves) {
         const dim3 grid((unsigned)L.gx, (unsigned)A.n_split, (unsigned)z), t(L.waves * 64);
-#define SIHIP_APT(NS)                                                                         \
-    if (L.waves == 4) hipLaunchKernelGGL((attnp_tiles_kernel<NS, 4>), grid, t, 0, st, A);     \
-    else hipLaunchKernelGGL((attnp_tiles_kernel<NS, 8>), grid, t, 0, st, A);
-        if (hd <= 64) { SIHIP_APT(4) }
-        else if (hd <= 96) { SIHIP_APT(6) }
-        else { SIHIP_APT(8) }
-#undef SIHIP_APT
+        if (hd <= 64) hipLaunchKernelGGL(attnp_tiles_kernel<4>, grid, t, 0, st, A);
+        else if (hd <= 96) hipLaunchKernelGGL(attnp_tiles_kernel<6>, grid, t, 0, st, A);
+        else hipLaunchKernelGGL(attnp_tiles_kernel<8>, grid, t, 0, st, A);
         if (A.n_split > 1) {
             const int per_wg = kApJoinThreads / (32 * L.waves);  // four-dim columns
             const dim3 jg((unsigned)L.gx, (unsigned)((hd / 4 + per_wg - 1) / per_wg), (unsigned)z);
@@ -376,8 +368,7 @@ int launch_attn(sihip_ctx *ctx, const AttnPLaunch &L, hipStream_t st) {
         const dim3 grid((unsigned)L.gx, A.placed ? 1u : (unsigned)A.C.n_kv, (unsigned)z), t(L.row_waves * 64);
 #define SIHIP_APR(NK, TT)                                                                                  \
     if (L.row_waves == 1) hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 1>), grid, t, 0, st, A);           \
-    else if (L.row_waves == 4) hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 4>), grid, t, 0, st, A);      \
-    else hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 8>), grid, t, 0, st, A);
+    else hipLaunchKernelGGL((attnp_rows_kernel<NK, TT, 4>), grid, t, 0, st, A);
         if (hd <= 64) { SIHIP_APR(1, 4) }
         else if (hd <= 128) { SIHIP_APR(2, 4) }
         else if (hd <= 192) { SIHIP_APR(3, 2) }

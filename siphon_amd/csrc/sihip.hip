@@ -59,7 +59,7 @@ static const OptionName kOptionNames[] = {
     {"GEMMKF_MAX_M", &Options::gemmkf_max_m}, {"GEMMKF_SBK", &Options::gemmkf_sbk},
     {"GEMM_GROUP", &Options::gemm_group}, {"GEMMSK_MAX_M", &Options::gemmsk_max_m},
     {"GEMMX_MIN_M", &Options::gemmx_min_m}, {"GEMMD_MIN_M", &Options::gemmd_min_m},
-    {"ATTNP_WAVES", &Options::attnp_waves}, {"ATTNP_SPLITS", &Options::attnp_splits},
+    {"ATTNP_LARGE", &Options::attnp_large}, {"ATTNP_SPLITS", &Options::attnp_splits},
     {"ATTNP_ROW_WAVES", &Options::attnp_row_waves},
     {"RING_MT", &Options::ring_mt},       {"RING_SBK", &Options::ring_sbk},
 };

@@ -65,12 +65,12 @@ def test_single_tokens(dev, heads, n_kv, hd, block):
 
 
 @pytest.mark.parametrize("heads,n_kv,hd,block", SHAPES)
-@pytest.mark.parametrize("waves", [0, 4, 8])
-def test_prompts(dev, option, heads, n_kv, hd, block, waves):
+@pytest.mark.parametrize("large", [0, 1])
+def test_prompts(dev, option, heads, n_kv, hd, block, large):
     """Requests of 0 to 300 new tokens, behind nothing or behind a context, in
     blocks of 16, 128 and 256 rows (the large ones: heads up to 128, and the
     requests of more than 64 rows)."""
-    option("ATTNP_WAVES", waves)
+    option("ATTNP_LARGE", large)
     rng = np.random.default_rng(heads + hd + block)
     lengths, adds = [0, 0, 37, 500, 64, 9, 0], [1, 300, 65, 17, 64, 0, 129]
     cache, table, q_start, kv_len = ko.requests(rng, lengths, adds, block, n_kv, hd)
@@ -87,11 +87,11 @@ CHANGES = {
 
 @pytest.mark.parametrize("change", CHANGES)
 @pytest.mark.parametrize("heads,n_kv,hd,block", [(8, 2, 128, 16), (5, 1, 64, 64), (4, 4, 80, 128), (2, 1, 256, 32)])
-@pytest.mark.parametrize("steps,waves", [("single", 0), ("prompt", 0), ("prompt", 4), ("prompt", 8)])
-def test_masks_and_scores(dev, option, change, heads, n_kv, hd, block, steps, waves):
-    if hd > 128 and waves:
+@pytest.mark.parametrize("steps,large", [("single", 0), ("prompt", 0), ("prompt", 1)])
+def test_masks_and_scores(dev, option, change, heads, n_kv, hd, block, steps, large):
+    if hd > 128 and large:
         pytest.skip("heads of more than 128 have no large row blocks")
-    option("ATTNP_WAVES", waves)
+    option("ATTNP_LARGE", large)
     rng = np.random.default_rng(len(change) * 100 + hd)
     lengths = [0, 1, 63, 64, 200, 450, 1300] if steps == "single" else [0, 40, 0, 333, 100]
     adds = [1] * 7 if steps == "single" else [70, 129, 1, 33, 200]
@@ -107,9 +107,9 @@ def test_masks_and_scores(dev, option, change, heads, n_kv, hd, block, steps, wa
 
 @pytest.mark.parametrize("kq", [-0.25, 0.0, 1e-30, 3.0])
 @pytest.mark.parametrize("cap", [0.0, 10.0])
-@pytest.mark.parametrize("waves", [0, 8])
-def test_score_factors(dev, option, kq, cap, waves):
-    option("ATTNP_WAVES", waves)
+@pytest.mark.parametrize("large", [0, 1])
+def test_score_factors(dev, option, kq, cap, large):
+    option("ATTNP_LARGE", large)
     rng = np.random.default_rng(17)
     cache, table, q_start, kv_len = ko.requests(rng, [400, 0, 90], [1, 60, 3], 32, 2, 64)
     check(dev, cache, table, q_start, kv_len, queries(rng, 64, 4, 64), kq, cap=cap)
@@ -117,7 +117,7 @@ def test_score_factors(dev, option, kq, cap, waves):
 
 
 @pytest.mark.parametrize("splits", [1, 3, 64])
-@pytest.mark.parametrize("row_waves", [1, 4, 8])
+@pytest.mark.parametrize("row_waves", [1, 4])
 @pytest.mark.parametrize("heads,n_kv,hd", [(8, 2, 128), (3, 3, 64), (6, 2, 256), (20, 1, 96)])
 def test_pieces(dev, option, heads, n_kv, hd, row_waves, splits):
     """Pieces of any number, joined by the last workgroup to arrive; lengths
@@ -130,32 +130,31 @@ def test_pieces(dev, option, heads, n_kv, hd, row_waves, splits):
 
 
 @pytest.mark.parametrize("splits", [1, 2, 5])
-@pytest.mark.parametrize("waves", [4, 8])
 @pytest.mark.parametrize("hd", [128, 64, 96])
-def test_splits_of_large_blocks(dev, option, hd, waves, splits):
-    option("ATTNP_WAVES", waves)
+def test_splits_of_large_blocks(dev, option, hd, splits):
+    option("ATTNP_LARGE", 1)
     option("ATTNP_SPLITS", splits)
-    rng = np.random.default_rng(waves * splits)
+    rng = np.random.default_rng(splits)
     cache, table, q_start, kv_len = ko.requests(rng, [900, 0, 3000, 5], [150, 100, 129, 40], 64, 2, hd)
     check(dev, cache, table, q_start, kv_len, queries(rng, 419, 4, hd, 2.0), 0.09)
 
 
-@pytest.mark.parametrize("waves", [4, 8])
-def test_prompts_beside_single_tokens(dev, option, waves):
+@pytest.mark.parametrize("hd", [128, 64])
+def test_prompts_beside_single_tokens(dev, option, hd):
     """Both row blocks in one call, in any order of the requests."""
-    option("ATTNP_WAVES", waves)
-    rng = np.random.default_rng(waves)
+    option("ATTNP_LARGE", 1)
+    rng = np.random.default_rng(hd)
     lengths, adds = [1500, 0, 333, 70, 40, 2000, 9], [1, 200, 1, 16, 17, 90, 5]
-    cache, table, q_start, kv_len = ko.requests(rng, lengths, adds, 32, 2, 128)
-    check(dev, cache, table, q_start, kv_len, queries(rng, sum(adds), 8, 128, 2.0), 0.09)
+    cache, table, q_start, kv_len = ko.requests(rng, lengths, adds, 32, 2, hd)
+    check(dev, cache, table, q_start, kv_len, queries(rng, sum(adds), 8, hd, 2.0), 0.09)
 
 
 @pytest.mark.parametrize("n_req", [63, 64, 65, 200, 256, 257, 300])
-@pytest.mark.parametrize("waves", [0, 4])
-def test_many_requests(dev, option, n_req, waves):
+@pytest.mark.parametrize("large", [0, 1])
+def test_many_requests(dev, option, n_req, large):
     """More than the 64 requests that a wave keeps in one register, and more
     than the 256 that are listed on the device."""
-    option("ATTNP_WAVES", waves)
+    option("ATTNP_LARGE", large)
     rng = np.random.default_rng(n_req)
     lengths = [int(x) for x in np.exp(rng.uniform(0, 6.5, n_req))]
     adds = [int(x) for x in rng.choice([0, 1, 1, 1, 4, 40], n_req)]
@@ -234,11 +233,11 @@ def test_rows_at_odd_addresses_with_gaps(dev):
     check(dev, cache, table, q_start, kv_len, queries(rng, 41, 6, 80, 2.0), 0.1, ldq=6 * 80 + 7, ldo=6 * 80 + 1, shift=3)
 
 
-@pytest.mark.parametrize("waves", [0, 4, 8])
-def test_rows_that_see_nothing(dev, option, waves):
+@pytest.mark.parametrize("large", [0, 1])
+def test_rows_that_see_nothing(dev, option, large):
     """Requests with impossible numbers write nothing; keys in pages outside
     the pool are not seen, and a row that sees none is zero."""
-    option("ATTNP_WAVES", waves)
+    option("ATTNP_LARGE", large)
     rng = np.random.default_rng(12)
     cache, table, q_start, kv_len = ko.requests(rng, [40, 20, 30, 9], [2, 2, 2, 2], 16, 2, 64)
     q = queries(rng, 9, 4, 64)
@@ -273,11 +272,11 @@ def test_bounds_cut(dev):
     assert (np.abs(got[1:9] - want[1:9]) <= err[1:9]).all()
 
 
-@pytest.mark.parametrize("steps,waves", [("single", 0), ("prompt", 0), ("prompt", 4), ("prompt", 8)])
-def test_garbage_that_no_row_sees(dev, option, steps, waves):
+@pytest.mark.parametrize("steps,large", [("single", 0), ("prompt", 0), ("prompt", 1)])
+def test_garbage_that_no_row_sees(dev, option, steps, large):
     """NaN scales and any codes behind the window and past the length, and
     large, tiny and zero scales of what is seen."""
-    option("ATTNP_WAVES", waves)
+    option("ATTNP_LARGE", large)
     rng = np.random.default_rng(14)
     lengths, adds = ([700, 300], [1, 1]) if steps == "single" else ([400, 0], [200, 150])
     cache, table, q_start, kv_len = ko.requests(rng, lengths, adds, 16, 2, 64)
@@ -322,3 +321,25 @@ def test_same_bits_every_time(dev, option, row_waves):
     first = run(dev, cache, table, q_start, kv_len, q, 0.09)
     for _ in range(4):
         assert np.array_equal(run(dev, cache, table, q_start, kv_len, q, 0.09).view(np.uint32), first.view(np.uint32))
+
+
+def test_overlapping_spans_leave_the_workspace_clean(dev, option):
+    """Numbers that give the same rows to several requests are more blocks than
+    the grid was made for: what it cannot join is not begun, and the next call
+    finds its counters at zero."""
+    option("ATTNP_LARGE", 0)
+    rng = np.random.default_rng(17)
+    lengths = [2000, 0] * 6
+    cache, table, q_start, kv_len = ko.requests(rng, lengths, [64, 0] * 6, 32, 2, 64)
+    q = queries(rng, 64, 2, 64)
+    with ko.OnDevice(dev, q=q, out=np.zeros_like(q)) as d:
+        c = ko.put_cache(d, cache)
+        b = ko.put_batch(d, table, [0, 64] * 6 + [0], kv_len, 64, max_q=64)
+        a = sa.AttnPaged(q=d.ptr("q"), ldq=128, out=d.ptr("out"), ldo=128, n_head=2, kq_scale=0.1)
+        n = dev.attn_paged_workspace(c, b, a)
+        assert n > 0
+        d.put("ws", np.zeros(n, np.uint8))
+        a.workspace, a.workspace_bytes = d.ptr("ws"), n
+        dev.attn_paged_dev(c, b, a)
+        dev.synchronize()
+        assert not d.get("ws")[:256 << 10].any()

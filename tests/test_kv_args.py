@@ -91,7 +91,7 @@ result = launched()
     assert got == []
     # a step in which every request ends or waits still has a plan
     got = fake_hip.run(SETUP + "dev.kv_plan_dev(plan(n_tok=0, slot=0, pos=0)); result = launched()")
-    assert [k for k, *_ in got] == ["kv_plan_kernel"]
+    assert [k for k, *_ in got] == ["kv_plan_kernel<256>"]
 
 
 @pytest.mark.parametrize("what", ["small", "exact", "aligned", "capture"])
@@ -120,6 +120,60 @@ else:
         assert "capture" in got[1] and got[2] == ""
     else:
         assert "workspace" in got[1]
+
+
+@pytest.mark.parametrize("call,want", [
+    # single tokens: blocks of 16 rows, a wave each where they fill the device
+    ("batch(), attn()", ["attnp_rows_kernel<2,4,4>"]),
+    ("batch(n_req=200, n_tok=200), attn()", ["attnp_rows_kernel<2,4,1>"]),
+    ("batch(n_req=300, n_tok=300), attn()", ["attnp_rows_kernel<2,4,4>"]),
+    # prompts: large blocks from some work on, split and joined where they are few
+    ("batch(n_req=1, n_tok=200, max_q=200), attn()", ["attnp_rows_kernel<2,4,4>"]),
+    ("batch(n_req=1, n_tok=1500, max_q=1500, max_kv=1500), attn()", ["attnp_rows_kernel<2,4,1>"]),
+    ("batch(n_req=1, n_tok=4096, max_q=4096, max_kv=4096), attn()", ["attnp_tiles_kernel<8,8>"]),
+    ("batch(n_req=1, n_tok=512, max_q=512, max_kv=4512), attn()", ["attnp_tiles_kernel<8,8>", "attnp_join_kernel<256>"]),
+    # beside single tokens, which have their own launch
+    ("batch(n_req=9, n_tok=4104, max_q=4096, max_kv=4096), attn()", ["attnp_rows_kernel<2,4,4>", "attnp_tiles_kernel<8,8>"]),
+    # other heads
+    ("batch(n_req=1, n_tok=4096, max_q=4096, max_kv=4096), attn()|head_dim=64", ["attnp_tiles_kernel<4,4>"]),
+    ("batch(n_req=1, n_tok=4096, max_q=4096, max_kv=4096), attn()|head_dim=96", ["attnp_tiles_kernel<6,8>"]),
+    ("batch(n_req=1, n_tok=4096, max_q=4096, max_kv=4096), attn(ldq=8192, ldo=8192)|head_dim=256", ["attnp_rows_kernel<4,2,1>"]),
+    ("batch(), attn(ldq=8192, ldo=8192)|head_dim=144", ["attnp_rows_kernel<3,2,4>"]),
+    ("batch(), attn()|head_dim=16", ["attnp_rows_kernel<1,4,4>"])])
+def test_the_kernels_of_a_shape(call, want):
+    args, _, heads = call.partition("|")
+    got = fake_hip.run(SETUP + f"batch_ = batch\ndef batch(**o): return batch_(max_blocks=200, **o)\ndev.attn_paged_dev(cache({heads}), {args}); result = launched()")
+    assert sorted(k for k, *_ in got) == sorted(want)
+
+
+@pytest.mark.parametrize("block,hd,want", [(16, 64, "1,128"), (16, 128, "1,128"), (32, 128, "1,256"), (64, 128, "1,512"),
+                                           (128, 128, "1,1024"), (256, 128, "2,1024"), (256, 256, "4,1024")])
+def test_the_kernels_of_a_page(block, hd, want):
+    got = fake_hip.run(SETUP + f"""
+c = cache(block={block}, head_dim={hd})
+dev.kv_append_dev(c, batch(), X, 4096, X, 4096)
+for n in 600, 5000:
+    dev.kv_read_dev(c, X, n, X, 4096, X, 4096)
+dev.kv_plan_dev(plan(n_req=256))
+dev.kv_plan_dev(plan(n_req=257))
+result = launched()
+""")
+    assert [k for k, *_ in got] == [f"kv_append_kernel<{want}>", "kv_read_kernel<16>", "kv_read_kernel<64>", "kv_plan_kernel<256>",
+                                    "kv_plan_kernel<1024>"]
+
+
+def test_as_many_pieces_as_counters():
+    """Many requests over splits that an option asks for: more pieces than
+    the workspace has counters are not made."""
+    got = fake_hip.run(SETUP + """
+dev.set_option("ATTNP_SPLITS", 64)
+c, a = cache(n_pages=1 << 20), attn()
+big, few = (batch(n_req=n, n_tok=n, max_blocks=200, max_kv=6400) for n in (4096, 100))
+result = [dev.attn_paged_workspace(c, b, a) for b in (big, few)]
+dev.attn_paged_dev(c, big, a)
+result.append(launched())
+""")
+    assert got[0] == 0 and got[1] > 0 and got[2] == [["attnp_rows_kernel<2,4,4>", 1, 8]]
 
 
 def test_a_failed_launch_is_reported():
