@@ -54,6 +54,7 @@ struct AttnPArgs {
     float scale2;    // |kq_scale| * log2 e, so that factors of scores are not negative
     float cap, cap_in;  // softcap * log2 e (0: none), 2 |kq_scale| / softcap * log2 e
     int n_tiles;     // most row blocks of a request
+    int ranks;       // most row blocks' worth of keys before a request's new ones
     int n_split, per_split;  // most splits of a row block's keys, least chunks of one
     int whole;       // chunks that are not split
     int slots;       // placed 16-row blocks: workgroups that share the chunks of all
@@ -760,12 +761,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
 // (row c, half e) the scores of keys 32 u + 16 e + i in register i: row m of
 // the operand is key 16 (m / 4 % 2) + 4 (m / 8) + m % 4.
 
-// Large row blocks lie in the grid by their number in their request, high
-// ones first, whatever the request: those see the most keys, and a launch that
-// starts them last would end with them alone. Block i of that order: with F(t)
-// = sum over requests of max(0, blocks - t), its number t has F(t + 1) <= i <
-// F(t), and it is the i - F(t + 1)th of the requests with more than t blocks.
-// The lanes try 64 numbers at once; up to 64 kPlaceRegs requests.
+// Large row blocks lie in the grid by their rank, the position of their first
+// row in blocks, high ones first, whatever the request: those see the most keys,
+// and a launch that starts them last would end with them alone (3 prompts of up
+// to 4096 tokens behind up to 1000 keys, 40 heads: by rank 701 us, by their number
+// in their request 770; 8 of 2048 behind up to 8000, 32 heads: 1210, 1409). Block
+// i of that order: with F(t) = the blocks of rank t and above, its rank t has
+// F(t + 1) <= i < F(t), and it is the i - F(t + 1)th of the requests that have
+// one of that rank. Up to 64 kPlaceRegs requests.
 __device__ inline bool ap_place(const AttnPArgs &A, int rows, int64_t i, int &r, int &tile) {
     const int lane = threadIdx.x & 63;
     if (A.n_req == 1) {
@@ -774,44 +777,75 @@ __device__ inline bool ap_place(const AttnPArgs &A, int rows, int64_t i, int &r,
         tile = (n + rows - 1) / rows - 1 - (int)i;
         return n >= A.least && tile >= 0;
     }
-    int blocks[kPlaceRegs];
+    int blocks[kPlaceRegs], first[kPlaceRegs];
 #pragma unroll
     for (int k = 0; k < kPlaceRegs; k++) {
         const int q = lane + 64 * k;
-        const int n = q < A.n_req ? min(request_span(A.R, q).n, A.R.max_q) * A.G : 0;
+        const Span s = q < A.n_req ? request_span(A.R, q) : Span{0, 0, 0, 0};
+        const int n = min(s.n, A.R.max_q) * A.G;
         blocks[k] = n < A.least ? 0 : (n + rows - 1) / rows;
+        first[k] = (int)min((int64_t)min(s.p0, A.R.max_kv) * A.G / rows, (int64_t)A.ranks);
     }
-    int lo = 0, span = A.n_tiles;
-    int64_t f = 0;
-    for (;;) {
-        const int step = (span + 63) / 64, t = lo + lane * step;
-        f = 0;
+    int lo = 0, span = A.ranks + A.n_tiles;  // past the highest rank
+    uint32_t f = 0;  // F(lo): at most 2^31, as the grid bounds the blocks of a request
+    const uint32_t n = (uint32_t)i;
+    if (A.n_req <= 32) {
+        // the lanes try 64 ranks at once
+        for (;;) {
+            const int step = (span + 63) / 64, t = lo + lane * step;
+            f = 0;
+            for (int q = 0; q < A.n_req; q++) {
+                const int b = __builtin_amdgcn_readlane(blocks[0], q);
+                f += min(b, max(0, __builtin_amdgcn_readlane(first[0], q) + b - t));
+            }
+            const int c = __popcll(__ballot(f > n));
+            if (c == 0) return false;  // (of the first round only: past the last block)
+            lo += (c - 1) * step;
+            f = (uint32_t)__builtin_amdgcn_readlane((int)f, c - 1);
+            if (step == 1) break;
+            span = step;
+        }
+    } else {
+        // each lane has its requests, and the ranks are bisected (200 prompts of
+        // up to 512: 697 us, 888 with the loop above; 64 of up to 1024: 2200, 2245)
+        auto from = [&](int t) {
+            uint32_t x = 0;
 #pragma unroll
-        for (int k = 0; k < kPlaceRegs; k++)
-            for (int q = 0; q < min(64, A.n_req - 64 * k); q++) f += max(0, __builtin_amdgcn_readlane(blocks[k], q) - t);
-        const int c = __popcll(__ballot(f > i));
-        if (c == 0) return false;  // (of the first round only: past the last block)
-        lo += (c - 1) * step;
-        f = __shfl(f, c - 1);
-        if (step == 1) break;
-        span = step;
+            for (int k = 0; k < kPlaceRegs; k++) x += min(blocks[k], max(0, first[k] + blocks[k] - t));
+            return (uint32_t)__builtin_amdgcn_readlane((int)ap_scan(x), 63);
+        };
+        f = from(0);
+        if (f <= n) return false;
+        while (span > 1) {
+            const int half = span / 2;
+            const uint32_t g = from(lo + half);
+            if (g > n) {
+                lo += half;
+                f = g;
+                span -= half;
+            } else {
+                span = half;
+            }
+        }
     }
     int more = 0;
 #pragma unroll
-    for (int k = 0; k < kPlaceRegs; k++) more += __popcll(__ballot(blocks[k] > lo));
-    int rank = (int)(i - (f - more));
+    for (int k = 0; k < kPlaceRegs; k++) more += __popcll(__ballot(first[k] <= lo && lo - first[k] < blocks[k]));
+    int rank = (int)(n - (f - more));
 #pragma unroll
     for (int k = 0; k < kPlaceRegs; k++) {
-        uint64_t has = __ballot(blocks[k] > lo);
-        const int n = __popcll(has);
-        if (rank >= 0 && rank < n) {
+        uint64_t has = __ballot(first[k] <= lo && lo - first[k] < blocks[k]);
+        const int m = __popcll(has);
+        if (rank >= 0 && rank < m) {
             for (; rank; rank--) has &= has - 1;
-            r = 64 * k + __ffsll((unsigned long long)has) - 1;
+            const int l = __ffsll((unsigned long long)has) - 1;
+            r = 64 * k + l;
+            tile = lo - __builtin_amdgcn_readlane(first[k], l);
         }
-        rank -= n;
+        rank -= m;
     }
     r = __builtin_amdgcn_readfirstlane(r);
-    tile = lo;
+    tile = __builtin_amdgcn_readfirstlane(tile);
     return true;
 }
 

@@ -234,6 +234,7 @@ int plan_launch(sihip_ctx *ctx, AttnPLaunch &L, int64_t rows, int64_t all_rows) 
     AttnPArgs &A = L.A;
     const int block_rows = L.waves ? 32 * L.waves : kApRows;
     A.n_tiles = (int)((rows + block_rows - 1) / block_rows);
+    A.ranks = (int)std::min<int64_t>((int64_t)A.R.max_kv * A.G / block_rows, 1 << 30);
     // row blocks of all requests: as many as the longest has each, and, listed,
     // no more than the step's rows fill
     L.blocks = (int64_t)A.n_req * A.n_tiles;
