@@ -214,6 +214,8 @@ constexpr int kApFewRows = 64;
 //   32 heads of 128: 512 rows 23 / 40, 1024 50 / 63, 1500 88 / 91, 1800 115 / 115,
 //     2048 133 / 120; 190 behind 8000 keys 98 / 105, 256 behind 8000 101 / 83, 64
 //     behind 30000 116 / 74; window of 512 142 / 122
+//     rows of few keys, however many: 200 prompts of up to 256 311 / 362, 50 of up
+//     to 512 183 / 204, 8 of up to 1024 129 / 124
 //   14 heads of 64 on 2: 1200 28 / 34, 4096 137 / 125; 32 on 8: 4096 247 / 170
 //   wider than 128 the large blocks' sums leave one wave a SIMD: 16 heads of 256,
 //     4096 rows 478 / 627
@@ -224,6 +226,7 @@ int attn_waves(const sihip_ctx *ctx, const AttnPArgs &A, int64_t rows, int64_t a
     if (rows <= 32) return 0;
     int64_t keys = A.R.max_kv - A.R.max_q / 2;  // of a row, on average, without a window
     if (A.window) keys = std::min<int64_t>(keys, (int64_t)A.window + 64);
+    if (keys < 384) return 0;
     const double work = (double)(all_rows / 16 * A.C.n_kv) * ((double)keys / 64) * A.C.hd;
     return work < 45e3 * 128 ? 0 : waves;
 }
