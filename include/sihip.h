@@ -327,9 +327,12 @@ int sihip_kv_read_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const int64_t
  *         window > 0, p - j < window; prefix: or j < prefix[r], later ones
  *         included. No such key: zeros.
  * q and out: f32 rows [n_head * head_dim] at token * ldq and token * ldo; rows
- * behind the last token are left as they were. Products are of f32 accuracy
- * (22 bits of q and of the probabilities), sums are f32; results do not
- * depend on the order in which workgroups run.
+ * behind the last token are left as they were. Products are of f32 accuracy:
+ * a value of q counts to 2^-22 of itself (2^-38 of its row's largest where that
+ * is more), a key's probability times its value scale to 2^-22 of that (2^-34
+ * of the row's largest such product), and probabilities below 2^-126 of the
+ * row's largest are zero. Sums are f32; results do not depend on the order in
+ * which workgroups run.
  * workspace: NULL, or device memory of sihip_attn_paged_workspace bytes
  * (16-byte aligned) of its own for calls that may overlap other work of the
  * context, on other streams or in graphs: zeroed once, before its first use,

@@ -14,10 +14,12 @@
 // f16 numbers, x = hi + lo with 22 bits: each product runs twice, and the
 // results keep f32's accuracy (a single f16 would leave 2^-11, 70 times the
 // f32 rounding of the sums). Query rows are scaled by a power of two to
-// [2^13, 2^14) first; weights, times their value scale over the power of two
-// below the largest scale so far, by 2^9, and reach 2^14 (kApLate): the lower
-// halves stay clear of the subnormal numbers but for weights too small to
-// count. Results differ from 64 bits by 2 to 7 10^-7 of their norm.
+// [2^13, 2^14) first; weights times their value scale by one that puts the
+// largest such product of the row so far into [2^9, 2^13) (Running): a page of
+// large values that the row hardly looks at takes no bits from the others. What
+// the lower halves lose as subnormal numbers is below 2^-34 of that product a
+// key, and 2^-38 of a query row's largest value. Results differ from 64 bits
+// by 2 to 7 10^-7 of their norm.
 //
 // Scores are computed transposed, S^T = K Q^T: a lane then holds the scores
 // of one row against 16 consecutive tokens, which all lie in one page (pages
@@ -265,9 +267,41 @@ __device__ inline float ap_max_quarters(float x) {
     return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 
-// A row's maximum follows the scores when they pass it by 2^4, so that most
-// chunks leave the sums alone: weights reach 2^4 and are held times 2^9.
-constexpr float kApLate = 4.0f, kApUnit = 0x1p9f;
+// The state of a row's softmax in a wave, in log2 units: weights are 2^(s - m),
+// l is their sum, and the sums of weights times values are held in units of
+// ref / 2^9. m follows the scores when they pass it by 4, and ref the products of
+// weight and value scale when they pass it 16 times, so that most chunks leave
+// the sums alone; what is multiplied stays below 2^14. m is a whole number and
+// ref a power of two: both move without a rounding. ref goes down with m, so
+// that it never is above the largest product of the row's keys so far, but
+// for two floors: 2^-100, and 2^-104 of the value scales (the quotient of a
+// scale and ref is to be a number; weights below 2^-126 are zero anyway).
+constexpr float kApLate = 4.0f, kApUnit = 0x1p9f, kApLeast = 0x1p-100f;
+
+struct Running {
+    float m = kApNone, l = 0.0f, ref = 0.0f, over = 0.0f;  // over = kApUnit / ref
+
+    // largest weight of a lane's keys (raw: their largest score is raw * f) times their value scale
+    __device__ float most(float raw, float f, float vs) const {
+        return vs * fmaxf(__builtin_amdgcn_exp2f(fmaf(raw, f, -m)), kApLeast);
+    }
+    // whether a lane's largest score, or that product, asks for a move of the row's
+    __device__ bool late(float mx, float most) const { return mx > m + kApLate || most > 16.0f * ref; }
+    // to a new maximum; returns the power of two that it takes from the weights so far
+    __device__ float raise(float mx) {
+        const float m2 = fmaxf(m, ceilf(mx)), am = ldexpf(1.0f, (int)fmaxf(m - m2, -256.0f));
+        m = m2;
+        l *= am;
+        return am;
+    }
+    // the reference, for `most` under the new maximum; returns the factor of the sums so far
+    __device__ float refer(float am, float most) {
+        const float kept = ref * am;
+        ref = fmaxf(kept, ap_power(most));
+        over = kApUnit / ref;
+        return kept / ref;
+    }
+};
 
 // ---- few rows ----------------------------------------------------------------------
 //
@@ -581,7 +615,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
         fc_row = f_row * A.cap_in;
         f_row *= A.scale2;
     }
-    float m = kApNone, l = 0.0f, ref = 0.0f, over = 0.0f;
+    Running R;
     ap_f4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = ap_f4{0, 0, 0, 0};
@@ -636,26 +670,20 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
         float mx = sc[0][0];
 #pragma unroll
         for (int i = 1; i < SEG; i++) mx = fmaxf(mx, sc[i >> 2][i & 3]);
-        mx = ap_max_quarters(mx * f);
-        const float top = ap_max_quarters(ap_power(vs));
-        if (__any(mx > m + kApLate || top > ref)) {
-            const float m2 = fmaxf(m, mx), r2 = fmaxf(ref, top), am = __builtin_amdgcn_exp2f(m - m2), ao = am * (ref / r2);
-            l *= am;
+        if (__any(R.late(mx * f, R.most(mx, f, vs)))) {
+            const float am = R.raise(ap_max_quarters(mx * f)), ao = R.refer(am, ap_max_quarters(R.most(mx, f, vs)));
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= ao;
-            m = m2;
-            ref = r2;
-            over = kApUnit / ref;
         }
-        const float w = vs * over;
+        const float w = vs * R.over;
         ap_h8 ph[TT / 2], pl[TT / 2];
 #pragma unroll
         for (int e = 0; e < TT / 2; e++) {
             float pr[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                pr[j] = __builtin_amdgcn_exp2f(fmaf(sc[2 * e + (j >> 2)][j & 3], f, -m));
-                l += pr[j];
+                pr[j] = __builtin_amdgcn_exp2f(fmaf(sc[2 * e + (j >> 2)][j & 3], f, -R.m));
+                R.l += pr[j];
             }
             ap_split8w(pr, w, ph[e], pl[e]);
         }
@@ -675,9 +703,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
     }
 
     // all lanes of a column hold the same m and parts of l
+    float m = R.m, l = R.l;
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    const float back = ref * (1.0f / kApUnit);
+    const float back = R.ref * (1.0f / kApUnit);
     const int rows = min(16, n_rows - tile * 16);
     const __amdgpu_buffer_rsrc_t part = ap_pieces(A, piece, 1);
     if constexpr (WAVES == 1) {
@@ -954,7 +983,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 2) void attnp_tiles_ke
         }
     };
 
-    float m = kApNone, l = 0.0f, ref = 0.0f, over = 0.0f;
+    Running R;
     if (u0 < u1) {
         load_pages(u0);
         load_keys(u0);
@@ -1059,25 +1088,19 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 2) void attnp_tiles_ke
                 float mx = sc[0];
 #pragma unroll
                 for (int e = 1; e < 16; e++) mx = fmaxf(mx, sc[e]);
-                mx = ap_max_halves(mx * f);
-                const float top = ap_max_halves(ap_power(vsc));
-                if (__any(mx > m + kApLate || top > ref)) {
-                    const float m2 = fmaxf(m, mx), r2 = fmaxf(ref, top), am = __builtin_amdgcn_exp2f(m - m2), ao = am * (ref / r2);
-                    l *= am;
+                if (__any(R.late(mx * f, R.most(mx, f, vsc)))) {
+                    const float am = R.raise(ap_max_halves(mx * f)), ao = R.refer(am, ap_max_halves(R.most(mx, f, vsc)));
 #pragma unroll
                     for (int d = 0; d < ND; d++) o[d] *= ao;
-                    m = m2;
-                    ref = r2;
-                    over = kApUnit / ref;
                 }
-                const float w = vsc * over;
+                const float w = vsc * R.over;
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     float pr[8];
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        pr[j] = __builtin_amdgcn_exp2f(fmaf(sc[8 * e + j], f, -m));
-                        l += pr[j];
+                        pr[j] = __builtin_amdgcn_exp2f(fmaf(sc[8 * e + j], f, -R.m));
+                        R.l += pr[j];
                     }
                     ap_split8w(pr, w, ph[e], pl[e]);
                 }
@@ -1108,9 +1131,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 2) void attnp_tiles_ke
         }
     }
     if (kTurns && u0 < u1 && wave < 4) __syncthreads();
+    float m = R.m, l = R.l;
     l += __shfl_xor(l, 32);
 
-    const float back = ref * (1.0f / kApUnit);
+    const float back = R.ref * (1.0f / kApUnit);
     if (row0 + col < n_rows) {
         // four dims in a row a register group: 32 d + 8 a + 4 half ..
         if (n_split == 1) {
