@@ -259,8 +259,10 @@ typedef struct sihip_kv_batch {
     int64_t n_req, max_blocks;
     int64_t n_tok;          /* rows of the step's arrays */
     int64_t max_q, max_kv;  /* bounds on a request's new tokens and length, which
-                             * size the launches; what lies past them is not
-                             * written, or not seen */
+                             * size the launches: of its new tokens those past
+                             * the first max_q have no keys, values or results
+                             * written, and positions from max_kv on are neither
+                             * written nor seen */
 } sihip_kv_batch;
 
 /* Bookkeeping of a step. Request r has len[r] cached tokens and gets add[r]

@@ -288,10 +288,13 @@ __global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs A) {
     const int h = blockIdx.x % A.C.n_kv, j = blockIdx.x / A.C.n_kv, r = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
     const int tid = threadIdx.x, B = 1 << A.C.shift, hd = A.C.hd;
-    const Span s = request_span(A.R, r);
+    // tokens past the host's bounds are not written (max_kv is at most what
+    // the table's rows hold)
+    Span s = request_span(A.R, r);
+    s.end = min(s.p0 + min(s.n, A.R.max_q), A.R.max_kv);
     const int b = (s.p0 >> A.C.shift) + j;
     const int64_t base = (int64_t)b << A.C.shift;
-    if (s.n == 0 || base >= s.end || b >= A.R.max_blocks) return;
+    if (s.end <= s.p0 || base >= s.end) return;
     const int64_t page = A.R.table[(int64_t)r * A.R.max_blocks + b];
     if (page < 0 || page >= A.C.n_pages) return;
     const int lo = (int)max((int64_t)s.p0 - base, (int64_t)0), hi = (int)min((int64_t)s.end - base, (int64_t)B);
