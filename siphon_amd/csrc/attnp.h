@@ -156,10 +156,6 @@ __device__ inline bool ap_whole(const AttnPArgs &A, const Sight &g, int j0, int 
     return j1 < g.prefix || (j1 <= g.p_lo && (!A.window || j0 > g.p_hi - A.window));
 }
 
-__device__ inline bool ap_visible(const AttnPArgs &A, const Sight &g, int p, int j) {
-    return j < g.keys && (j < g.prefix || (j <= p && (!A.window || j > p - A.window)));
-}
-
 // bits 0 .. n - 1 of 16
 __device__ inline uint32_t ap_below(int n) { return (1u << max(0, min(n, 16))) - 1u; }
 
@@ -189,14 +185,6 @@ __device__ inline float ap_capped(const AttnPArgs &A, float s, float x2) {
     y = fmaf(z, y, -1.0f / 3.0f);
     const float near = fmaf(s * z, y, s);
     return z < 0.1f ? near : far;
-}
-
-// The score of a raw product: `f` is the factor to log2 units, fc the one of
-// the tanh's argument where scores are capped.
-__device__ inline float ap_score(const AttnPArgs &A, float raw, float f, float fc, float slope, int p, int j) {
-    float s = raw * f;
-    if (A.cap != 0.0f) s = ap_capped(A, s, raw * fc);
-    return fmaf(-slope, fabsf((float)(p - j)), s);
 }
 
 // Power of two (as an exponent) by which a query row is multiplied.
