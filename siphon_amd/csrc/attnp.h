@@ -140,10 +140,11 @@ __device__ inline Sight ap_sight(const AttnPArgs &A, int r, const Span &s, int t
     g.prefix = A.prefix ? max(0, min(A.prefix[r], g.keys)) : 0;
     const int end = min(max(g.p_hi + 1, g.prefix), g.keys);
     const int start = A.window ? max(0, g.p_lo - A.window + 1) : 0;
-    const int up = (1 << A.chunk) - 1;
-    g.np = A.window ? (g.prefix + up) >> A.chunk : 0;
+    // (keys come up to 2^31 - 16: rounded up to whole chunks without a sign)
+    auto chunks = [&](int keys) { return (int)(((uint32_t)keys + (1u << A.chunk) - 1) >> A.chunk); };
+    g.np = A.window ? chunks(g.prefix) : 0;
     g.c0 = max(start >> A.chunk, g.np);
-    g.n = g.np + max(0, ((end + up) >> A.chunk) - g.c0);
+    g.n = g.np + max(0, chunks(end) - g.c0);
     return g;
 }
 
@@ -151,7 +152,7 @@ __device__ inline int ap_chunk(const Sight &g, int u) { return u < g.np ? u : u 
 
 // whether every row of the block sees the n keys from j0 on
 __device__ inline bool ap_whole(const AttnPArgs &A, const Sight &g, int j0, int n) {
-    const int j1 = j0 + n - 1;
+    const int j1 = j0 + (n - 1);  // (j0 + n can be 2^31)
     if (j1 >= g.keys) return false;
     return j1 < g.prefix || (j1 <= g.p_lo && (!A.window || j0 > g.p_hi - A.window));
 }
