@@ -366,7 +366,7 @@ __device__ inline Deal ap_deal(const AttnPArgs &A) {
                 D.n[k] = ap_sight(A, r, D.s[k], 0, n - 1).n;
             }
         }
-        all += (float)tiles[k] * (float)(A.C.n_kv * D.n[k]);
+        all += (float)tiles[k] * (float)A.C.n_kv * (float)D.n[k];
     }
     // rounded up by more than the sum can be off: a piece too long by that is
     // harmless, one too short would make more pieces than the grid has
