@@ -27,6 +27,7 @@
 // operand of out^T = V^T P^T as they lie: no transposition, no exchange.
 #pragma once
 
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -601,7 +602,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
                 ap_split8(x[c][e], qh[c][e], ql[c][e]);
             }
         f_row = ldexpf(1.0f, -e2);
-        fc_row = f_row * A.cap_in;
+        fc_row = fminf(f_row * A.cap_in, FLT_MAX);
         f_row *= A.scale2;
     }
     Running R;
@@ -636,7 +637,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
         // that it leaves -inf as it is, and is a number where no key is seen
         const int j0 = c * CH + g * SEG;  // key of register (t, i): j0 + 4 t + i
         float f = fmaxf(f_row * ksc, 0x1p-120f), vs = vsc;
-        const float fc = fc_row * ksc;
+        const float fc = fminf(fc_row * ksc, FLT_MAX);  // a number: zero times it is zero
         const int pv_next = pv;
         load_keys(next);
         if (A.cap != 0.0f) {
@@ -1001,7 +1002,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 2) void attnp_tiles_ke
             ap_split8(x[c], qh[c], ql[c]);
         }
         f_row = ldexpf(1.0f, -e2);
-        fc_row = f_row * A.cap_in;
+        fc_row = fminf(f_row * A.cap_in, FLT_MAX);
         f_row *= A.scale2;
     }
     ap_f16 o[ND];
@@ -1051,7 +1052,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 2) void attnp_tiles_ke
                 const float ksc = s_lds[buf][2 * i + half];
                 float vsc = s_lds[buf][4 + 2 * i + half], f = fmaxf(f_row * ksc, 0x1p-120f);
                 if (A.cap != 0.0f) {
-                    const float fc = fc_row * ksc;
+                    const float fc = fminf(fc_row * ksc, FLT_MAX);
 #pragma unroll
                     for (int e = 0; e < 16; e++) sc[e] = ap_capped(A, sc[e] * f, sc[e] * fc);
                     f = 1.0f;

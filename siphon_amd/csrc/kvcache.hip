@@ -333,8 +333,8 @@ int plan_attn(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch 
     const double scale = std::fabs((double)a->kq_scale), log2e = 1.4426950408889634;
     A.sign = a->kq_scale < 0 ? -1.0f : 1.0f;
     A.scale2 = (float)(scale * log2e);
-    A.cap = (float)((double)a->softcap * log2e);
-    A.cap_in = a->softcap > 0 ? (float)(2.0 * scale / a->softcap * log2e) : 0.0f;
+    A.cap = (float)std::min((double)a->softcap * log2e, (double)FLT_MAX);
+    A.cap_in = a->softcap > 0 ? (float)std::min(2.0 * scale / a->softcap * log2e, (double)FLT_MAX) : 0.0f;
     A.placed = A.n_req <= 64 * kPlaceRegs;
     A.least = 0;
     A.most = INT32_MAX;

@@ -9,7 +9,9 @@ d_j, what its exponent may be off by (absolute, natural units):
   split of q into two f16 halves) and 2^-38 max|q| sum |k_j| (a half that is
   subnormal: rows are scaled to [2^13, 2^14), half a step there is 2^-25), all
   times kq_scale; 2^-21 |s_j| for a handful of f32 roundings of the factors;
-  2^-21 of the cap; 2^-23 of the bias; and 2^-24 (|s_j - s_max| + 8) for the
+  where scores are capped no more than twice the cap of that (tanh is not
+  steeper than 1 and within 1), and 2^-21 of the cap for the tanh, or of 4
+  |s_j| if that is less (below 0.32 of the cap it is a series); 2^-23 of the bias; and 2^-24 (|s_j - s_max| + 8) for the
   rounding of the exponent that is taken (the running maximum is at most 4
   late and rounded up to the next integer, in log2 units).
 r, what its weight may be off by besides, relative: 2^-20 for the exponential,
@@ -62,8 +64,8 @@ def attention(cache, table, q_start, kv_len, q, kq_scale, cap=0.0, slopes=None, 
             d = ((2 * hd * 2.0 ** -24 + 2.0 ** -22) * (np.abs(x) @ np.abs(kh).T)
                  + 2.0 ** -38 * np.abs(x).max(1, keepdims=True) * np.abs(kh).sum(1)) * abs(kq_scale) + 2.0 ** -21 * np.abs(s)
             if cap:
-                s = cap * np.tanh(s / cap)
-                d += 2.0 ** -21 * cap
+                with np.errstate(over="ignore"):
+                    d, s = np.minimum(d, 2 * cap) + 2.0 ** -21 * np.minimum(cap, 4 * np.abs(s)), cap * np.tanh(s / cap)
             if slopes is not None:
                 bias = float(slopes[h]) * np.abs(p - at)
                 s = s - bias
