@@ -310,7 +310,7 @@ struct Running {
 // to do takes 3.5; 131072 keys 55 us, 268 MB at 4.9 TB/s; 64 requests of up to
 // 8192 keys, 408 MB, 91 us, 4.5 TB/s (a read of as much that does nothing else
 // 5.4 to 5.9, a copy 4.8). Prompts of up to 1500 rows by the vector
-// instructions between the products: 512 rows 23 us.
+// instructions between the products: 512 rows 24 us.
 
 constexpr int kApRows = 16;
 constexpr int kPlaceRegs = 4;  // requests a lane keeps in ap_deal and ap_place
@@ -770,11 +770,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
 // scores). Of eight waves four are a step behind the others, which leaves each
 // SIMD one wave of either kind at any time: kTurns.
 //
-// Bound by the vector step: a wave that is alone in it on its SIMD issues an
-// instruction every 6 to 7 cycles, about 1850 a half, where the matrix step
-// takes 1024. 32 heads of 128 on 8: 4096 rows 280 us, 16384 rows 3.8 ms, at
-// 580 TFLOP/s of f16 products (290 of the formula's: each runs twice); capped
-// 420 us, with slopes 333. Heads of 64: 170 us.
+// Bound by the latency of the vector step: a wave that is alone in it on its
+// SIMD issues an instruction every 6 to 7 cycles, about 1850 a half, where the
+// matrix step takes 1024. Neither pipe is full: of 3 prompts of up to 4096 vector
+// instructions take half of the launch's cycles, products 0.37. 32 heads of 128
+// on 8: 4096 rows 290 us, 16384 rows 3.8 ms, at 1150 TFLOP/s of f16 products (575
+// of the formula's: each runs twice); 4096 capped 420 us, with slopes 332. Heads
+// of 64: 4096 rows 180 us.
 //
 // A wave's 32x32 tile of S^T has its key rows in the order that gives lane
 // (row c, half e) the scores of keys 32 u + 16 e + i in register i: row m of
@@ -826,7 +828,8 @@ __device__ inline bool ap_place(const AttnPArgs &A, int rows, int64_t i, int &r,
         }
     } else {
         // each lane has its requests, and the ranks are bisected (200 prompts of
-        // up to 512: 697 us, 888 with the loop above; 64 of up to 1024: 2200, 2245)
+        // up to 512: 697 us, 888 with the loop above; 64 of up to 1024 behind up to
+        // 8000: 2185, 2230)
         auto from = [&](int t) {
             uint32_t x = 0;
 #pragma unroll

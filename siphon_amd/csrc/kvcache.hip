@@ -211,14 +211,14 @@ constexpr int kApFewRows = 64;
 // Waves of a large row block, 0: 16-row blocks throughout. The work is 16-row
 // blocks times 64-key chunks (as far as the host knows the lengths: bounds)
 // times the head's width. us, 16-row blocks against the large ones:
-//   32 heads of 128: 512 rows 23 / 40, 1024 50 / 63, 1500 88 / 91, 1800 115 / 115,
-//     2048 133 / 120; 190 behind 8000 keys 98 / 105, 256 behind 8000 101 / 83, 64
-//     behind 30000 116 / 74; window of 512 142 / 122
+//   32 heads of 128: 512 rows 24 / 50, 1024 51 / 72, 1500 86 / 99, 1800 114 / 116,
+//     2048 132 / 120; 190 behind 8000 keys 96 / 107, 256 behind 8000 105 / 85, 64
+//     behind 30000 118 / 77; window of 512 140 / 119
 //     rows of few keys, however many: 200 prompts of up to 256 311 / 362, 50 of up
-//     to 512 183 / 204, 8 of up to 1024 129 / 124
-//   14 heads of 64 on 2: 1200 28 / 34, 4096 137 / 125; 32 on 8: 4096 247 / 170
-//   wider than 128 the large blocks' sums leave one wave a SIMD: 16 heads of 256,
-//     4096 rows 478 / 627
+//     to 512 184 / 205, 8 of up to 1024 128 / 125
+//   14 heads of 64 on 2: 1200 27 / 33, 4096 133 / 124; 32 on 8: 4096 239 / 171
+//   wider than 128 the large blocks' sums would leave one wave a SIMD: 16 heads of
+//     256, 4096 rows 467, 627 in a build that had them
 int attn_waves(const sihip_ctx *ctx, const AttnPArgs &A, int64_t rows, int64_t all_rows) {
     if (A.C.hd > 128) return 0;
     const int waves = ap_tile_waves(A.C.hd);
@@ -261,12 +261,17 @@ int plan_launch(sihip_ctx *ctx, AttnPLaunch &L, int64_t rows, int64_t all_rows) 
         L.gx = L.waves ? (A.placed ? L.blocks : A.n_tiles) * A.C.n_kv : (int64_t)A.n_tiles * A.n_split;
     } else {
         // Four waves share a piece, or, where there are row blocks enough, each
-        // has its own. Workgroups that the pieces are made for: one a CU for few
-        // long requests (32 heads of 128 over 131072 keys 55 us, 65 with 1.5 a
-        // CU), more where lengths differ (64 requests of up to 8192 keys 95 us with
-        // one, 90 with three; 16 of 16000 with 8 heads 71, 58 with 1.5). The row
-        // blocks of prompts fill the CUs by themselves, and are as long as each
-        // other (128 rows behind 4000 keys 37 us with one, 52 with three).
+        // has its own. Workgroups that the pieces are made for, of single tokens
+        // by the number of row blocks: the host knows no more. Few blocks: one a
+        // CU; more: more, as the pieces of blocks of different lengths end at
+        // different times. us with 1 / 1.5 / 3 a CU, heads of 128, blocks of up to
+        // so many keys: 8 of 131072 46 / 56 / 65; 32 of 30000 41 / 35 / 40; 64 of
+        // 16000 36 / 31 / 36; 128 of 16000 64 / 51 / 59; 248 of 8191 45 / 49 / 44;
+        // 256 of 8191 49 / 41 / 45; 400 of 8191 67 / 73 / 63; 512 of 8191 89 / 88 /
+        // 81. Blocks that are all of one length would do better with one: 128 of
+        // 8000 46 / 54 / 58, 256 of 4095 43 / 48 / 58, 512 of 4095 100 / 100 / 110.
+        // The row blocks of prompts fill the CUs by themselves, and are as long as
+        // each other (128 rows behind 4000 keys 37 us with one, 52 with three).
         const int64_t w = ctx->opt.attnp_row_waves;
         L.row_waves = w == 1 || w == 4 ? (int)w : items >= 4 * ctx->n_cu ? 1 : 4;
         A.slots = (A.R.max_q > 1 ? (L.row_waves == 1 ? 8 : 2) : L.row_waves == 1 ? 16 : items < 64 ? 2 : items < 256 ? 3 : 6) *

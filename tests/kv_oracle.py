@@ -122,11 +122,10 @@ def attention(cache, table, q_start, kv_len, q, kq_scale, cap=0.0, slopes=None, 
     twice the largest of them for a quotient of sums of exponentials, plus
     2^-20 for the exponentials and their split, and 2^-24 for each of the
     2 n + 64 additions of an output's chain: relative to sum p |v|. A key's
-    weight times its value scale is held in f16 halves in units of 2^-9 of the
-    power of two below the largest scale (2^-13 where the maximum is never
-    late), so its last half is a multiple of 2^-24 there: half of that, 2^-34
-    of the largest scale, times codes up to 128, for each key (the weight of
-    a row's largest score is at least 1)."""
+    weight times its value scale is held in f16 halves whose last one is off by
+    at most 2^-34 of the row's largest such product. The bound has 2^-34 of the
+    largest scale of all the request's pages and heads, times codes up to 128,
+    for each key, which is more: kv_scores has a bound for each row and head."""
     T, H, hd = q.shape
     G = H // cache.n_kv
     out, err = np.zeros((T, H, hd)), np.zeros((T, H, hd))
