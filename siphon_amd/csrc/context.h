@@ -106,6 +106,10 @@ struct sihip_ctx {
 // sihip_init; launches with more tiles than this are not sliced.
 constexpr int64_t kGemmCounters = 65536;
 
+// What follows is one copy for the library's translation units and not exported
+// from it: the host's process may hold the same names.
+#pragma GCC visibility push(hidden)
+
 // the last failure of sihip_init, and of calls without a context
 inline char g_init_err[512];
 
@@ -179,3 +183,5 @@ inline int ensure(sihip_ctx *ctx, void **buf, size_t *cap, size_t bytes, hipStre
     *cap = bytes;
     return SIHIP_OK;
 }
+
+#pragma GCC visibility pop
