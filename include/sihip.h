@@ -363,6 +363,105 @@ int sihip_attn_paged_workspace(sihip_ctx *ctx, const sihip_kv_cache *cache,
                                const sihip_kv_batch *batch, const sihip_attn_paged *args,
                                uint64_t *bytes);
 
+/* ---- rotation on the way into a paged cache ------------------------------
+ * A step's new rows, for one layer. q rows are [n_head * head_dim] f32, k and v rows
+ * [n_head_kv * head_dim], row t at t * ld of each.
+ * rope: f32 [rope_len][rope_dim / 2][2], cosine and sine of each position and pair; of a
+ * head of q and k the pair i, (a, b), becomes (a cos - b sin, a sin + b cos), computed in
+ * 64 bits and rounded once. Pair i is dims i and i + rope_dim / 2 or, rope_neighbours
+ * not 0, dims 2 i and 2 i + 1; dims from rope_dim on stay as they are. rope_dim is even and at most
+ * head_dim; positions go up to the batch's max_kv (or what max_blocks hold, where that
+ * is less), which rope_len must not be below.
+ * q NULL: keys alone are rotated. Else the rotated queries go to q_out, whose
+ * rows may be those of q themselves (with ldq_out = ldq) but not overlap them otherwise.
+ * Rows of tokens that are not written (past max_q, from max_kv on, or behind the last) are left
+ * as they were; a page outside the cache drops its keys and values, not its queries. */
+typedef struct sihip_kv_rows {
+    const float *k, *v;
+    int64_t ldk, ldv;
+    const float *q;
+    float *q_out;
+    int64_t ldq, ldq_out, n_head;
+    const float *rope;
+    int64_t rope_len, rope_dim, rope_neighbours;
+} sihip_kv_rows;
+
+/* sihip_kv_append_dev of the rotated keys and of the values, and the rotation of the step's
+ * queries, in one launch. */
+int sihip_kv_append_rope_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch *batch,
+                             const sihip_kv_rows *rows, void *stream);
+
+/* ---- paged 4-bit KV cache ------------------------------------------------
+ * A cache of about half the bytes: pages, requests, plans (sihip_kv_plan_dev) and batches as
+ * for the 8-bit one. A value is code * sub * scale:
+ *   k        codes [n_pages][n_head_kv][block][head_dim]
+ *   v        codes [n_pages][n_head_kv][head_dim][block]  (transposed)
+ *   k_sub, v_sub      int8 [n_pages][n_head_kv][head_dim / 32][block]
+ *   k_scale, v_scale  bfloat16 [n_pages][n_head_kv][block]
+ * Codes are -8 .. 7, eight to a 32-bit word of the last dimension: elements 0, 2, 4,
+ * 6, 1, 3, 5, 7 from the lowest nibble up, each plus 8. For the 32 dims of a sub the
+ * step is -1/8 of their value of largest magnitude (of two, the negative); the scale is the token's
+ * largest step / 127 rounded up to bfloat16; a sub is its step / scale rounded away
+ * from zero, 1 to 127 in magnitude; a code is value / (sub * scale) rounded to the nearest, ties
+ * to even, exactly, at most 7. Rows of magnitudes below 2^-100 become zeros; those above 2^126
+ * saturate; infinities do not count for steps and saturate, NaN becomes 0.
+ * All arrays are 16-byte aligned. block: 16, 32, 64, 128 or 256; head_dim: a multiple of
+ * 32, at most 256. Memory that no token was written to may hold anything. */
+typedef struct sihip_kv4_cache {
+    uint8_t *k, *v;
+    int8_t *k_sub, *v_sub;
+    uint16_t *k_scale, *v_scale;
+    int64_t n_pages, n_head_kv, head_dim, block;
+} sihip_kv4_cache;
+
+/* Write the step's keys and values, each row quantized by itself, with the rotation of
+ * sihip_kv_append_rope_dev, or as they are (rows->rope NULL, then q must be too).
+ * Requests must not share a page that gets new tokens. */
+int sihip_kv4_append_dev(sihip_ctx *ctx, const sihip_kv4_cache *cache, const sihip_kv_batch *batch,
+                         const sihip_kv_rows *rows, void *stream);
+
+/* Rows back as f32, as sihip_kv_read_dev. */
+int sihip_kv4_read_dev(sihip_ctx *ctx, const sihip_kv4_cache *cache, const int64_t *slots, int64_t n,
+                       float *k, int64_t ldk, float *v, int64_t ldv, void *stream);
+
+/* Attention over it: sihip_attn_paged_dev in every respect, of the same accuracy (a
+ * key's probability times its value scale counts to 2^-22 of that, 2^-34 of the row's
+ * largest such product), and with the same workspace rules. */
+int sihip_attn_paged4_dev(sihip_ctx *ctx, const sihip_kv4_cache *cache, const sihip_kv_batch *batch,
+                          const sihip_attn_paged *args, void *stream);
+int sihip_attn_paged4_workspace(sihip_ctx *ctx, const sihip_kv4_cache *cache,
+                                const sihip_kv_batch *batch, const sihip_attn_paged *args,
+                                uint64_t *bytes);
+
+/* ---- log probabilities -----------------------------------------------------
+ * Of n_rows rows of n_vocab logits (f32, row i at i * ld), as sihip_gemm_dev of the head
+ * leaves them, with log p_j = x_j - log sum e^x:
+ *   logprob   f32 [n_rows][n_token], of the tokens token[n_rows][n_token]; an entry whose
+ *             token is outside 0 .. n_vocab - 1 is left as it was
+ *   entropy   f32 [n_rows], - sum p log p
+ *   top_id, top_logprob  [n_rows][n_top], the most likely tokens and theirs, in order; of
+ *             equal logits the lowest token first. n_top <= 64 and <= n_vocab
+ * Each may be NULL (token with logprob, top_id with top_logprob; n_token or n_top 0). A
+ * logit of -inf is a token that is not allowed: its log probability is -inf, and it adds nothing
+ * to the entropy. A row of -inf alone has entropy 0. A row with a NaN or +inf has NaN in
+ * all but top_id, where NaN counts as -inf. Sums are f64 of f32 exponentials.
+ * workspace: as for sihip_attn_paged_dev (sihip_logprobs_workspace bytes). */
+typedef struct sihip_logprobs {
+    const float *logits;
+    int64_t ld, n_rows, n_vocab;
+    const int32_t *token;
+    int64_t n_token;
+    float *logprob, *entropy;
+    int64_t n_top;
+    int32_t *top_id;
+    float *top_logprob;
+    void *workspace;
+    uint64_t workspace_bytes;
+} sihip_logprobs;
+
+int sihip_logprobs_dev(sihip_ctx *ctx, const sihip_logprobs *args, void *stream);
+int sihip_logprobs_workspace(sihip_ctx *ctx, const sihip_logprobs *args, uint64_t *bytes);
+
 /* ---- device memory for hosts without a HIP runtime of their own -------
  * The reference host is plain C17 and never links HIP; these let it (and
  * tests) hold activations and outputs on the device for the *_dev entry

@@ -84,6 +84,26 @@ class AttnPaged(_Args):
                 ("prefix", _vp), ("window", _i64), ("workspace", _vp), ("workspace_bytes", _u64)]
 
 
+class KvRows(_Args):
+    """sihip_kv_rows: a step's new rows, and their rotation."""
+    _fields_ = [("k", _vp), ("v", _vp), ("ldk", _i64), ("ldv", _i64), ("q", _vp), ("q_out", _vp),
+                ("ldq", _i64), ("ldq_out", _i64), ("n_head", _i64), ("rope", _vp), ("rope_len", _i64),
+                ("rope_dim", _i64), ("rope_neighbours", _i64)]
+
+
+class Kv4Cache(_Args):
+    """sihip_kv4_cache: one layer's paged 4-bit cache."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_sub", _vp), ("v_sub", _vp), ("k_scale", _vp), ("v_scale", _vp),
+                ("n_pages", _i64), ("n_head_kv", _i64), ("head_dim", _i64), ("block", _i64)]
+
+
+class Logprobs(_Args):
+    """sihip_logprobs: log probabilities of rows of logits."""
+    _fields_ = [("logits", _vp), ("ld", _i64), ("n_rows", _i64), ("n_vocab", _i64), ("token", _vp),
+                ("n_token", _i64), ("logprob", _vp), ("entropy", _vp), ("n_top", _i64), ("top_id", _vp),
+                ("top_logprob", _vp), ("workspace", _vp), ("workspace_bytes", _u64)]
+
+
 def load_library(path: str = HIP_SO) -> ctypes.CDLL:
     """Load libsiphon_hip.so; raises if it has not been built."""
     global _lib
@@ -121,6 +141,13 @@ def load_library(path: str = HIP_SO) -> ctypes.CDLL:
     L.sihip_kv_read_dev.argtypes = [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]
     L.sihip_attn_paged_dev.argtypes = [_vp, _vp, _vp, _vp, _vp]
     L.sihip_attn_paged_workspace.argtypes = [_vp, _vp, _vp, _vp, ctypes.POINTER(_u64)]
+    L.sihip_kv_append_rope_dev.argtypes = [_vp, _vp, _vp, _vp, _vp]
+    L.sihip_kv4_append_dev.argtypes = [_vp, _vp, _vp, _vp, _vp]
+    L.sihip_kv4_read_dev.argtypes = [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]
+    L.sihip_attn_paged4_dev.argtypes = [_vp, _vp, _vp, _vp, _vp]
+    L.sihip_attn_paged4_workspace.argtypes = [_vp, _vp, _vp, _vp, ctypes.POINTER(_u64)]
+    L.sihip_logprobs_dev.argtypes = [_vp, _vp, _vp]
+    L.sihip_logprobs_workspace.argtypes = [_vp, _vp, ctypes.POINTER(_u64)]
     L.sihip_gemm_dev.argtypes = [_vp, _vp, _vp, _i64, _vp, _vp]
     L.sihip_gemm_dev_noalloc.argtypes = [_vp, _vp, _vp, _i64, _vp, _vp]
     L.sihip_gemv_multi_dev.argtypes = [_vp, ctypes.c_int, ctypes.POINTER(_vp), _vp,
@@ -280,6 +307,37 @@ class Device:
         n = _u64()
         self._check(self.L.sihip_attn_paged_workspace(self.ctx, cache.ref, batch.ref, args.ref,
                                                       ctypes.byref(n)))
+        return n.value
+
+    def kv_append_rope_dev(self, cache: KvCache, batch: KvBatch, rows: KvRows,
+                           stream: int | None = None):
+        self._check(self.L.sihip_kv_append_rope_dev(self.ctx, cache.ref, batch.ref, rows.ref, stream))
+
+    # the paged 4-bit KV cache
+    def kv4_append_dev(self, cache: Kv4Cache, batch: KvBatch, rows: KvRows, stream: int | None = None):
+        self._check(self.L.sihip_kv4_append_dev(self.ctx, cache.ref, batch.ref, rows.ref, stream))
+
+    def kv4_read_dev(self, cache: Kv4Cache, slots_ptr: int, n: int, k_ptr: int, ldk: int, v_ptr: int,
+                     ldv: int, stream: int | None = None):
+        self._check(self.L.sihip_kv4_read_dev(self.ctx, cache.ref, slots_ptr, n, k_ptr, ldk, v_ptr,
+                                              ldv, stream))
+
+    def attn_paged4_dev(self, cache: Kv4Cache, batch: KvBatch, args: AttnPaged,
+                        stream: int | None = None):
+        self._check(self.L.sihip_attn_paged4_dev(self.ctx, cache.ref, batch.ref, args.ref, stream))
+
+    def attn_paged4_workspace(self, cache: Kv4Cache, batch: KvBatch, args: AttnPaged) -> int:
+        n = _u64()
+        self._check(self.L.sihip_attn_paged4_workspace(self.ctx, cache.ref, batch.ref, args.ref,
+                                                       ctypes.byref(n)))
+        return n.value
+
+    def logprobs_dev(self, args: Logprobs, stream: int | None = None):
+        self._check(self.L.sihip_logprobs_dev(self.ctx, args.ref, stream))
+
+    def logprobs_workspace(self, args: Logprobs) -> int:
+        n = _u64()
+        self._check(self.L.sihip_logprobs_workspace(self.ctx, args.ref, ctypes.byref(n)))
         return n.value
 
     def gemm_dev(self, w: Weight, X_ptr: int, M: int, Y_ptr: int, stream: int | None = None):

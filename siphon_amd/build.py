@@ -22,7 +22,7 @@ ROOT = os.path.dirname(PKG)
 LIB_DIR = os.path.join(PKG, "lib")
 HIP_SO = os.path.join(LIB_DIR, "libsiphon_hip.so")
 # translation units of the library: csrc/<unit>.hip
-HIP_UNITS = ["sihip", "kvcache"]
+HIP_UNITS = ["sihip", "kvcache", "kvcache4", "logprobs"]
 
 ARCH = "gfx950"
 HIPCC_FLAGS = [

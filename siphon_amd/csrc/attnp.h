@@ -468,22 +468,17 @@ __device__ inline void ap_join_rows(const AttnPArgs &A, const Span &s, int h, in
     if (tid == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// hd rounded up to 64 NK dims
-template <int NK, int TT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) {
-    constexpr int ND = NK * 4;  // 16-dim tiles
-    constexpr int CH = 16 * TT, SEG = 4 * TT;
-    constexpr uint32_t kAll = (1u << SEG) - 1;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
-    const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
-    int r = blockIdx.z, h = blockIdx.y, tile, split, per = A.per_split;
-    int64_t piece;
-    Span s;
+// The row block and the split of a workgroup of the kernels for few rows; false: it has none.
+__device__ __forceinline__ bool ap_rows_place(const AttnPArgs &A, int &r, int &h, int &tile, int &split, int &per, int64_t &piece,
+                                              Span &s) {
+    r = blockIdx.z;
+    h = blockIdx.y;
+    per = A.per_split;
     if (A.placed) {
         const Deal D = ap_deal(A);
         const int i = blockIdx.x;
         r = ap_dealt_to(D, i);
-        if (r < 0) return;
+        if (r < 0) return false;
         int n;
         const int before = ap_dealt(D, r, n, s), parts = D.splits(A, n);
         split = (i - before) % parts;
@@ -493,7 +488,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
         piece = i;
         // (spans that overlap are more than the grid was made for: what a block
         // cannot join in it, it does not begin)
-        if (i < split || i - split + parts > (int)gridDim.x) return;
+        if (i < split || i - split + parts > (int)gridDim.x) return false;
     } else {
         s = request_span(A.R, r);
         // workgroups go to the eight XCDs in turn, and of a ragged batch only the
@@ -502,6 +497,89 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
         split = (blockIdx.x % A.n_split + h + r) % A.n_split;
         piece = (((int64_t)r * A.n_tiles + tile) * A.C.n_kv + h) * A.n_split + split;
     }
+    return true;
+}
+
+// The end of a 16-row block's piece: its waves' sums joined through LDS, then whole
+// rows to out, or a part for ap_join_rows. o: sums of 16-dim tiles, dims 16 d + 4 (lane / 16) ..
+// of the row lane % 16.
+template <int ND, int WAVES>
+__device__ __forceinline__ void ap_rows_end(const AttnPArgs &A, const Span &s, const Running &R, const ap_f4 (&o)[ND], int h, int tile,
+                                            int n_rows, int64_t piece, int split, int n_split, int tok, int head) {
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4, hd = A.C.hd;
+    // all lanes of a column hold the same m and parts of l
+    float m = R.m, l = R.l;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const float back = R.ref * (1.0f / kApUnit);
+    const int rows = min(16, n_rows - tile * 16);
+    const __amdgpu_buffer_rsrc_t part = ap_pieces(A, piece, 1);
+    if constexpr (WAVES == 1) {
+        if (n_split == 1) {
+            if (col >= rows) return;
+            const float z = l > 0.0f || l != l ? back / l : 0.0f;
+            float *to = A.out + (s.q0 + tok) * A.ldo + (int64_t)head * hd + 4 * g;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+                if (16 * d < hd) ap_put4(to + 16 * d, o[d][0] * z, o[d][1] * z, o[d][2] * z, o[d][3] * z, A.out_vec);
+        } else if (col < rows) {
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+                if (16 * d < hd)
+                    ap_store4(part, (4 * d + g) * 16 + col, float4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back});
+            if (g == 0) ap_store4(part, 4 * hd + col, float4{m, l, 0, 0});
+        }
+    } else {
+        __shared__ float4 o_lds[WAVES][ND * 4][17];
+        __shared__ float m_lds[WAVES][16], l_lds[WAVES][16];
+        if (g == 0) {
+            m_lds[wave][col] = m;
+            l_lds[wave][col] = l;
+        }
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+            o_lds[wave][4 * d + g][col] = float4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back};
+        __syncthreads();
+        for (int i = tid; i < 4 * hd; i += WAVES * 64) {
+            // whole rows to out, the sums of a dim for all rows to the splits
+            const int c = n_split == 1 ? i / (hd / 4) : i % 16, d4 = n_split == 1 ? i % (hd / 4) : i / 16;
+            if (c >= rows) continue;
+            float mm = kApNone, ll = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) mm = fmaxf(mm, m_lds[w][c]);
+            float4 oo = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float e = __builtin_amdgcn_exp2f(m_lds[w][c] - mm);
+                const float4 v = o_lds[w][d4][c];
+                ll = fmaf(l_lds[w][c], e, ll);
+                oo = float4{fmaf(v.x, e, oo.x), fmaf(v.y, e, oo.y), fmaf(v.z, e, oo.z), fmaf(v.w, e, oo.w)};
+            }
+            if (n_split == 1) {
+                const int rw = tile * 16 + c;
+                ap_put4(A.out + (s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + 4 * d4,
+                        ap_quotient(oo.x, ll), ap_quotient(oo.y, ll), ap_quotient(oo.z, ll), ap_quotient(oo.w, ll), A.out_vec);
+            } else {
+                ap_store4(part, i, oo);
+                if (d4 == 0) ap_store4(part, 4 * hd + c, float4{mm, ll, 0, 0});
+            }
+        }
+    }
+    if (n_split > 1) ap_join_rows<WAVES * 64>(A, s, h, tile, rows, piece - split, n_split);
+}
+
+// hd rounded up to 64 NK dims
+template <int NK, int TT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) {
+    constexpr int ND = NK * 4;  // 16-dim tiles
+    constexpr int CH = 16 * TT, SEG = 4 * TT;
+    constexpr uint32_t kAll = (1u << SEG) - 1;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
+    int r, h, tile, split, per;
+    int64_t piece;
+    Span s;
+    if (!ap_rows_place(A, r, h, tile, split, per, piece, s)) return;
     const int32_t *table = A.R.table + (int64_t)r * A.R.max_blocks;
     const int n_tok = min(s.n, A.R.max_q), n_rows = n_tok * A.G;
     if (tile * 16 >= n_rows) return;
@@ -692,65 +770,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
         pv = page_of(min(next + WAVES, u1 - 1), g);
     }
 
-    // all lanes of a column hold the same m and parts of l
-    float m = R.m, l = R.l;
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    const float back = R.ref * (1.0f / kApUnit);
-    const int rows = min(16, n_rows - tile * 16);
-    const __amdgpu_buffer_rsrc_t part = ap_pieces(A, piece, 1);
-    if constexpr (WAVES == 1) {
-        if (n_split == 1) {
-            if (col >= rows) return;
-            const float z = l > 0.0f || l != l ? back / l : 0.0f;
-            float *to = A.out + (s.q0 + tok) * A.ldo + (int64_t)head * hd + 4 * g;
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-                if (16 * d < hd) ap_put4(to + 16 * d, o[d][0] * z, o[d][1] * z, o[d][2] * z, o[d][3] * z, A.out_vec);
-        } else if (col < rows) {
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-                if (16 * d < hd)
-                    ap_store4(part, (4 * d + g) * 16 + col, float4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back});
-            if (g == 0) ap_store4(part, 4 * hd + col, float4{m, l, 0, 0});
-        }
-    } else {
-        __shared__ float4 o_lds[WAVES][ND * 4][17];
-        __shared__ float m_lds[WAVES][16], l_lds[WAVES][16];
-        if (g == 0) {
-            m_lds[wave][col] = m;
-            l_lds[wave][col] = l;
-        }
-#pragma unroll
-        for (int d = 0; d < ND; d++)
-            o_lds[wave][4 * d + g][col] = float4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back};
-        __syncthreads();
-        for (int i = tid; i < 4 * hd; i += WAVES * 64) {
-            // whole rows to out, the sums of a dim for all rows to the splits
-            const int c = n_split == 1 ? i / (hd / 4) : i % 16, d4 = n_split == 1 ? i % (hd / 4) : i / 16;
-            if (c >= rows) continue;
-            float mm = kApNone, ll = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WAVES; w++) mm = fmaxf(mm, m_lds[w][c]);
-            float4 oo = {0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < WAVES; w++) {
-                const float e = __builtin_amdgcn_exp2f(m_lds[w][c] - mm);
-                const float4 v = o_lds[w][d4][c];
-                ll = fmaf(l_lds[w][c], e, ll);
-                oo = float4{fmaf(v.x, e, oo.x), fmaf(v.y, e, oo.y), fmaf(v.z, e, oo.z), fmaf(v.w, e, oo.w)};
-            }
-            if (n_split == 1) {
-                const int rw = tile * 16 + c;
-                ap_put4(A.out + (s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + 4 * d4,
-                        ap_quotient(oo.x, ll), ap_quotient(oo.y, ll), ap_quotient(oo.z, ll), ap_quotient(oo.w, ll), A.out_vec);
-            } else {
-                ap_store4(part, i, oo);
-                if (d4 == 0) ap_store4(part, 4 * hd + c, float4{mm, ll, 0, 0});
-            }
-        }
-    }
-    if (n_split > 1) ap_join_rows<WAVES * 64>(A, s, h, tile, rows, piece - split, n_split);
+    ap_rows_end<ND, WAVES>(A, s, R, o, h, tile, n_rows, piece, split, n_split, tok, head);
 }
 
 // ---- many rows ---------------------------------------------------------------------

@@ -198,6 +198,26 @@ __device__ inline Span request_span(const BatchArgs &A, int r) {
     return s;
 }
 
+// The tokens lo .. hi - 1 of the jth page that gets new tokens of request r, which
+// begins at position base; row q0 is position p0. None (lo = hi): the request has no
+// such page, or only tokens past the host's bounds, which are not written (max_kv is at
+// most what the table's rows hold).
+struct PageSpan {
+    int64_t q0, base;
+    int p0, lo, hi, block;  // block: of the request's table row
+};
+
+__device__ inline PageSpan page_span(const BatchArgs &A, int r, int j, int shift) {
+    const Span s = request_span(A, r);
+    const int end = min(s.p0 + min(s.n, A.max_q), A.max_kv), b = (s.p0 >> shift) + j;
+    const int64_t base = (int64_t)b << shift;
+    PageSpan g = {s.q0, base, s.p0, 0, 0, b};
+    if (end <= s.p0 || base >= end) return g;
+    g.lo = (int)max((int64_t)s.p0 - base, (int64_t)0);
+    g.hi = (int)min((int64_t)end - base, (int64_t)1 << shift);
+    return g;
+}
+
 // ---- append ------------------------------------------------------------------------
 
 struct AppendArgs {
@@ -284,25 +304,28 @@ __device__ inline int requantize_exact(int code, float was, float now, double in
 // which a launch with nothing to do takes 3.5; the rest are dependent loads.
 // Where every page's scale grows, and its old codes are rounded again in f64,
 // 10.3 us, and 21.3 for the chunks.
-template <int U, int THREADS>
-__global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs A) {
+//
+// Key: the 16 values of a key's dims, where they are not those of its row (the
+// rotated keys of kvrope.h).
+struct RowKeys {
+    static constexpr bool kAsTheyAre = true;
+};
+
+template <int U, int THREADS, class Key>
+__device__ __forceinline__ void kv_append_page(const AppendArgs &A, const Key &key) {
     __shared__ float wave_max[THREADS / 64];
     const int h = blockIdx.x % A.C.n_kv, j = blockIdx.x / A.C.n_kv, r = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
-    const int tid = threadIdx.x, B = 1 << A.C.shift, hd = A.C.hd;
-    // tokens past the host's bounds are not written (max_kv is at most what
-    // the table's rows hold)
-    Span s = request_span(A.R, r);
-    s.end = min(s.p0 + min(s.n, A.R.max_q), A.R.max_kv);
-    const int b = (s.p0 >> A.C.shift) + j;
-    const int64_t base = (int64_t)b << A.C.shift;
-    if (s.end <= s.p0 || base >= s.end) return;
-    const int64_t page = A.R.table[(int64_t)r * A.R.max_blocks + b];
+    const int tid = threadIdx.x, hd = A.C.hd;
+    const PageSpan g = page_span(A.R, r, j, A.C.shift);
+    const int64_t base = g.base;
+    const int lo = g.lo, hi = g.hi;
+    if (lo >= hi) return;
+    const int64_t page = A.R.table[(int64_t)r * A.R.max_blocks + g.block];
     if (page < 0 || page >= A.C.n_pages) return;
-    const int lo = (int)max((int64_t)s.p0 - base, (int64_t)0), hi = (int)min((int64_t)s.end - base, (int64_t)B);
     const int64_t ld = is_v ? A.ldv : A.ldk;
     // row of the page's token 0 (may lie before the first row)
-    const float *x = (is_v ? A.v : A.k) + (s.q0 + base - s.p0) * ld + (int64_t)h * hd;
+    const float *x = (is_v ? A.v : A.k) + (g.q0 + base - g.p0) * ld + (int64_t)h * hd;
     float *sp = (is_v ? A.C.vs : A.C.ks) + page * A.C.n_kv + h;
     int8_t *codes = (is_v ? A.C.v : A.C.k) + (page * A.C.n_kv + h) * ((int64_t)hd << A.C.shift);
     const float was = lo > 0 ? *sp : 0.0f;
@@ -326,6 +349,8 @@ __global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs A) {
         } else if (is_v) {
 #pragma unroll
             for (int e = 0; e < 16; e++) val[i][e] = inner + e >= lo && inner + e < hi ? x[(int64_t)(inner + e) * ld + outer] : 0.0f;
+        } else if constexpr (!Key::kAsTheyAre) {
+            key.load(x + (int64_t)outer * ld, (int)base + outer, inner, val[i]);
         } else if (A.k_wide) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -380,6 +405,11 @@ __global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs A) {
         *(uint4 *)(codes + (is_v ? (outer << A.C.shift) + inner : outer * hd + inner)) = buf[i].w;
     }
     if (tid == 0 && (grew || lo == 0)) *sp = now;
+}
+
+template <int U, int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs A) {
+    kv_append_page<U, THREADS>(A, RowKeys());
 }
 
 // ---- read ---------------------------------------------------------------------------
