@@ -433,7 +433,15 @@ __device__ inline __amdgpu_buffer_rsrc_t ap_pieces(const AttnPArgs &A, int64_t p
 // that the result does not depend on the order of arrival, and leaves the counter
 // zero. (A second launch took 10 to 20 us: most of its workgroups had nothing to
 // join, and each had to find that out.)
-template <int THREADS>
+//
+// RB: rows of a block. 16 lanes in a row (columns) have a row each, or, RB less than 16, one
+// group of 32 dims of one of RB rows: column group * RB + row.
+template <int RB>
+__device__ __forceinline__ int ap_column(int row, int d4) {
+    return RB == 16 ? row : (d4 >> 3) * RB + row;
+}
+
+template <int THREADS, int RB = 16>
 __device__ inline void ap_join_rows(const AttnPArgs &A, const Span &s, int h, int tile, int rows, int64_t first, int n) {
     __shared__ uint32_t last;
     const int tid = threadIdx.x, hd = A.C.hd;
@@ -455,7 +463,7 @@ __device__ inline void ap_join_rows(const AttnPArgs &A, const Span &s, int h, in
             float4 ml[16], v[16];
 #pragma unroll
             for (int k = 0; k < 16; k++) {
-                const uint32_t at = min(k0 + k, n - 1) * step + c;
+                const uint32_t at = min(k0 + k, n - 1) * step + ap_column<RB>(c, d4);
                 ml[k] = ap_fetch4(part, at + hd / 4 * kApRows);
                 v[k] = ap_fetch4(part, at + d4 * kApRows);
             }
@@ -502,8 +510,8 @@ __device__ __forceinline__ bool ap_rows_place(const AttnPArgs &A, int &r, int &h
 
 // The end of a 16-row block's piece: its waves' sums joined through LDS, then whole
 // rows to out, or a part for ap_join_rows. o: sums of 16-dim tiles, dims 16 d + 4 (lane / 16) ..
-// of the row lane % 16.
-template <int ND, int WAVES>
+// of the column lane % 16.
+template <int ND, int WAVES, int RB = 16>
 __device__ __forceinline__ void ap_rows_end(const AttnPArgs &A, const Span &s, const Running &R, const ap_f4 (&o)[ND], int h, int tile,
                                             int n_rows, int64_t piece, int split, int n_split, int tok, int head) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4, hd = A.C.hd;
@@ -516,16 +524,16 @@ __device__ __forceinline__ void ap_rows_end(const AttnPArgs &A, const Span &s, c
     const __amdgpu_buffer_rsrc_t part = ap_pieces(A, piece, 1);
     if constexpr (WAVES == 1) {
         if (n_split == 1) {
-            if (col >= rows) return;
+            if (col % RB >= rows) return;
             const float z = l > 0.0f || l != l ? back / l : 0.0f;
             float *to = A.out + (s.q0 + tok) * A.ldo + (int64_t)head * hd + 4 * g;
 #pragma unroll
             for (int d = 0; d < ND; d++)
-                if (16 * d < hd) ap_put4(to + 16 * d, o[d][0] * z, o[d][1] * z, o[d][2] * z, o[d][3] * z, A.out_vec);
-        } else if (col < rows) {
+                if (16 * d < hd && (RB == 16 || d / 2 == col / RB)) ap_put4(to + 16 * d, o[d][0] * z, o[d][1] * z, o[d][2] * z, o[d][3] * z, A.out_vec);
+        } else if (col % RB < rows) {
 #pragma unroll
             for (int d = 0; d < ND; d++)
-                if (16 * d < hd)
+                if (16 * d < hd && (RB == 16 || d / 2 == col / RB))
                     ap_store4(part, (4 * d + g) * 16 + col, float4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back});
             if (g == 0) ap_store4(part, 4 * hd + col, float4{m, l, 0, 0});
         }
@@ -544,15 +552,16 @@ __device__ __forceinline__ void ap_rows_end(const AttnPArgs &A, const Span &s, c
             // whole rows to out, the sums of a dim for all rows to the splits
             const int c = n_split == 1 ? i / (hd / 4) : i % 16, d4 = n_split == 1 ? i % (hd / 4) : i / 16;
             if (c >= rows) continue;
+            const int at = ap_column<RB>(c, d4);
             float mm = kApNone, ll = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WAVES; w++) mm = fmaxf(mm, m_lds[w][c]);
+            for (int w = 0; w < WAVES; w++) mm = fmaxf(mm, m_lds[w][at]);
             float4 oo = {0, 0, 0, 0};
 #pragma unroll
             for (int w = 0; w < WAVES; w++) {
-                const float e = __builtin_amdgcn_exp2f(m_lds[w][c] - mm);
-                const float4 v = o_lds[w][d4][c];
-                ll = fmaf(l_lds[w][c], e, ll);
+                const float e = __builtin_amdgcn_exp2f(m_lds[w][at] - mm);
+                const float4 v = o_lds[w][d4][at];
+                ll = fmaf(l_lds[w][at], e, ll);
                 oo = float4{fmaf(v.x, e, oo.x), fmaf(v.y, e, oo.y), fmaf(v.z, e, oo.z), fmaf(v.w, e, oo.w)};
             }
             if (n_split == 1) {
@@ -560,12 +569,12 @@ __device__ __forceinline__ void ap_rows_end(const AttnPArgs &A, const Span &s, c
                 ap_put4(A.out + (s.q0 + rw / A.G) * A.ldo + (int64_t)(h * A.G + rw % A.G) * hd + 4 * d4,
                         ap_quotient(oo.x, ll), ap_quotient(oo.y, ll), ap_quotient(oo.z, ll), ap_quotient(oo.w, ll), A.out_vec);
             } else {
-                ap_store4(part, i, oo);
-                if (d4 == 0) ap_store4(part, 4 * hd + c, float4{mm, ll, 0, 0});
+                ap_store4(part, d4 * 16 + at, oo);
+                if (RB == 16 ? d4 == 0 : d4 % 8 == 0) ap_store4(part, 4 * hd + at, float4{mm, ll, 0, 0});
             }
         }
     }
-    if (n_split > 1) ap_join_rows<WAVES * 64>(A, s, h, tile, rows, piece - split, n_split);
+    if (n_split > 1) ap_join_rows<WAVES * 64, RB>(A, s, h, tile, rows, piece - split, n_split);
 }
 
 // hd rounded up to 64 NK dims

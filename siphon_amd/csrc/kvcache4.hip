@@ -84,8 +84,7 @@ int plan_attn4(sihip_ctx *ctx, const sihip_kv4_cache *cache, const sihip_kv_batc
     const char *fn = "attn_paged4_dev";
     const int rc = check_cache4(ctx, fn, cache, C);
     if (rc) return rc;
-    return plan_attn(ctx, fn, {(int8_t *)C.k, (int8_t *)C.v, nullptr, nullptr, C.n_pages, C.n_kv, C.hd, C.shift}, false, batch, a,
-                     P);
+    return plan_attn(ctx, fn, {(int8_t *)C.k, (int8_t *)C.v, nullptr, nullptr, C.n_pages, C.n_kv, C.hd, C.shift}, batch, a, P);
 }
 
 int launch_attn4(sihip_ctx *ctx, const Cache4Args &C, const AttnPLaunch &L, hipStream_t st) {
@@ -96,7 +95,29 @@ int launch_attn4(sihip_ctx *ctx, const Cache4Args &C, const AttnPLaunch &L, hipS
     A.kd = C.ks;
     A.vd = C.vs;
     const int hd = C.hd, z = A.placed ? 1 : A.n_req;
+    if (L.waves) {
+        const dim3 grid((unsigned)L.gx, (unsigned)A.n_split, (unsigned)z), t(L.waves * 64);
+        if (hd <= 64) hipLaunchKernelGGL(attnp4_tiles_kernel<4>, grid, t, 0, st, A);
+        else if (hd <= 96) hipLaunchKernelGGL(attnp4_tiles_kernel<6>, grid, t, 0, st, A);
+        else hipLaunchKernelGGL(attnp4_tiles_kernel<8>, grid, t, 0, st, A);
+        if (A.n_split > 1) launch_join(L, st);
+        return launched(ctx, "attn_paged4");
+    }
     const dim3 grid((unsigned)L.gx, A.placed ? 1u : (unsigned)C.n_kv, (unsigned)z), t(L.row_waves * 64);
+    // Up to 8 rows of heads up to 64, 4 of heads up to 128, 2 of wider ones: a column for each of
+    // their groups of dims
+    const int64_t rows = (int64_t)A.R.max_q * A.G;
+#define SIHIP_AP4G(KD, NK, ND, TT, NG)                                                                                 \
+    if (rows <= 16 / NG) {                                                                                             \
+        if (L.row_waves == 1) hipLaunchKernelGGL((attnp4_groups_kernel<KD, NK, ND, TT, 1, NG>), grid, t, 0, st, A);    \
+        else hipLaunchKernelGGL((attnp4_groups_kernel<KD, NK, ND, TT, 4, NG>), grid, t, 0, st, A);                     \
+        return launched(ctx, "attn_paged4");                                                                           \
+    }
+    if (hd <= 64) { SIHIP_AP4G(16, 1, 4, 4, 2) }
+    else if (hd <= 128) { SIHIP_AP4G(32, 1, 8, 4, 4) }
+    else if (hd <= 192) { SIHIP_AP4G(32, 2, 12, 2, 8) }
+    else { SIHIP_AP4G(32, 2, 16, 2, 8) }
+#undef SIHIP_AP4G
 #define SIHIP_AP4R(KD, NK, ND, TT)                                                                                     \
     if (L.row_waves == 1) hipLaunchKernelGGL((attnp4_rows_kernel<KD, NK, ND, TT, 1>), grid, t, 0, st, A);              \
     else hipLaunchKernelGGL((attnp4_rows_kernel<KD, NK, ND, TT, 4>), grid, t, 0, st, A);

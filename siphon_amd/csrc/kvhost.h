@@ -225,9 +225,9 @@ int plan_launch(sihip_ctx *ctx, const char *fn, AttnPLaunch &L, int64_t rows, in
     return SIHIP_OK;
 }
 
-// C: the cache, which the caller has checked; large: it has large row blocks.
-int plan_attn(sihip_ctx *ctx, const char *fn, const CacheArgs &C, bool large, const sihip_kv_batch *batch,
-              const sihip_attn_paged *a, AttnPPlan &P) {
+// C: the cache, which the caller has checked.
+int plan_attn(sihip_ctx *ctx, const char *fn, const CacheArgs &C, const sihip_kv_batch *batch, const sihip_attn_paged *a,
+              AttnPPlan &P) {
     if (!a) return set_err(ctx, SIHIP_EINVAL, "%s: NULL argument", fn);
     AttnPArgs A = {};
     A.C = C;
@@ -270,7 +270,7 @@ int plan_attn(sihip_ctx *ctx, const char *fn, const CacheArgs &C, bool large, co
     A.least = 0;
     A.most = INT32_MAX;
     P.l[0].A = A;
-    P.l[0].waves = large ? attn_waves(ctx, A, rows, all_rows) : 0;
+    P.l[0].waves = attn_waves(ctx, A, rows, all_rows);
     P.n = 1;
     // Lengths that differ: a request of few rows would fill little of a large
     // block, and go through all its keys in it alone
