@@ -361,16 +361,18 @@ __device__ inline ap_h8 ap4_codes(uint32_t w) {
 // signed byte t of x
 __device__ inline float ap4_byte(uint32_t x, int t) { return (float)(int8_t)(x >> (8 * t)); }
 
-// the sum of a row over its NG columns, the same bits in each
-template <int NG>
-__device__ inline float ap4_over_groups(float x) {
-    auto from = [&](auto ctrl) {
-        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+// the sums of N numbers of a row over its NG columns, the same bits in each (one step for all
+// numbers before the next: a result is not ready for another lane at once)
+template <int NG, int N>
+__device__ inline void ap4_over_groups(float (&x)[N]) {
+    auto add = [&](auto ctrl) {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            x[i] += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x[i]), decltype(ctrl)::value, 0xf, 0xf, true));
     };
-    if constexpr (NG >= 2) x += from(std::integral_constant<int, 0x128>());  // 8 columns on
-    if constexpr (NG >= 4) x += from(std::integral_constant<int, 0x124>());  // 4
-    if constexpr (NG >= 8) x += from(std::integral_constant<int, 0x122>());  // 2
-    return x;
+    if constexpr (NG >= 2) add(std::integral_constant<int, 0x128>());  // 8 columns on
+    if constexpr (NG >= 4) add(std::integral_constant<int, 0x124>());  // 4
+    if constexpr (NG >= 8) add(std::integral_constant<int, 0x122>());  // 2
 }
 
 template <int KD, int NK, int ND, int TT, int WAVES, int NG>
@@ -548,9 +550,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
         float w[SEG], vs[SEG], f = f_row;
 #pragma unroll
         for (int i = 0; i < SEG; i++) {
-            w[i] = ap4_over_groups<NG>(sc[i % TT][i / TT] * (ap4_bf16(kd[i / 2], i & 1) * ap4_byte(ksub[i / 4], i & 3)));
+            w[i] = sc[i % TT][i / TT] * (ap4_bf16(kd[i / 2], i & 1) * ap4_byte(ksub[i / 4], i & 3));
             vs[i] = ap4_bf16(vd[i / 2], i & 1) * ap4_byte(vsub[i / 4], i & 3);
         }
+        ap4_over_groups<NG>(w);
         const bool here = pv >= 0;
         load_keys(next);
         load_entries(min(next + WAVES, u1 - 1));
@@ -621,8 +624,24 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
 // attnp_tiles_kernel (attnp.h) over 4-bit values: the codes of a 64-key chunk become f16 numbers
 // once, code * sub, on their way into LDS; the scales of its keys and values lie there beside
 // them, as f32. A unit of 16 values is 8 bytes here.
-template <int NS, int WAVES = ap_tile_waves(16 * NS)>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 2) void attnp4_tiles_kernel(Attn4Args A) {
+// Order of N operands from LDS, two products each: the reads are kAhead operands before their use.
+// (Left to itself the compiler reads each where it is used, and the products wait 16 times a half.)
+template <int N>
+__device__ __forceinline__ void ap4_reads_ahead() {
+    constexpr int kAhead = N < 3 ? N : 3, kRead = 0x100, kProduct = 0x8;
+    __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < N - kAhead; i++) {
+        __builtin_amdgcn_sched_group_barrier(kProduct, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kProduct, 2 * kAhead, 0);
+}
+
+constexpr int ap4_tile_waves(int hd) { return 4; }
+
+template <int NS, int WAVES = ap4_tile_waves(16 * NS)>
+__global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kernel(Attn4Args A) {
     constexpr int kApTileRows = 32 * WAVES, kApTileThreads = 64 * WAVES;
     constexpr bool kTurns = WAVES == 8;
     constexpr int ND = (NS + 1) / 2;             // 32-dim tiles of the output
@@ -782,19 +801,25 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 2) void attnp4_tiles_k
         const int j0 = ap_chunk(S, u) * 64;
         return idle || (j0 >= S.prefix && (j0 > W.p_hi || (A.window && j0 + 63 <= W.p_lo - A.window)));
     };
+    // where this lane's operands lie in LDS: the granules of a row are permuted by an exclusive or, so
+    // that another granule is another exclusive or of the address. The empty statements keep
+    // the compiler from holding all of these in registers, which the operands need.
     const int key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
-    const int x = KC % 16 ? (col >> 1) & 7 : col & 15, y = (col >> 1) & 7;
+    const uint32_t k_at = key * KC * 16 + ((half ^ (KC % 16 ? (col >> 1) & 7 : col & 15)) << 4);
+    const uint32_t v_at = col * 128 + ((2 * half ^ ((col >> 1) & 7)) << 4);
     ap_f16 sc;
     auto scores = [&](int buf, int i) {
-        const uint4 *kl = k_lds[buf][32 * i + key];
+        uint32_t at = k_at + (64 * buf + 32 * i) * KC * 16;
+        asm("" : "+v"(at));
 #pragma unroll
         for (int e = 0; e < 16; e++) sc[e] = 0.0f;
 #pragma unroll
         for (int c = 0; c < NS; c++) {
-            const ap_h8 a = __builtin_bit_cast(ap_h8, kl[(2 * c + half) ^ x]);
+            const ap_h8 a = *(const ap_h8 *)((const char *)k_lds + (at ^ c << 5));
             sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], sc, 0, 0, 0);
             sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], sc, 0, 0, 0);
         }
+        ap4_reads_ahead<NS>();
     };
     if (u0 < u1) {
         put_keys(0);
@@ -892,14 +917,17 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 2) void attnp4_tiles_k
             __syncthreads();
             // their products with the values, and the next half's scores
             if (!skip) {
+                uint32_t at = v_at + buf * ND * 32 * 128;
+                asm("" : "+v"(at));
 #pragma unroll
                 for (int e = 0; e < 2; e++)
 #pragma unroll
                     for (int d = 0; d < ND; d++) {
-                        const ap_h8 a = __builtin_bit_cast(ap_h8, v_lds[buf][32 * d + col][(4 * i + 2 * half + e) ^ y]);
+                        const ap_h8 a = *(const ap_h8 *)((const char *)v_lds + ((at ^ (4 * i + e) << 4) + d * 4096));
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[e], o[d], 0, 0, 0);
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[e], o[d], 0, 0, 0);
                     }
+                ap4_reads_ahead<2 * ND>();
                 if (i == 0) scores(buf, 1);
             }
             if (i == 1 && u + 1 < u1 && !blind(u + 1)) scores(buf ^ 1, 0);

@@ -191,7 +191,7 @@ int plan_attn8(sihip_ctx *ctx, const sihip_kv_cache *cache, const sihip_kv_batch
     if (!ctx) return set_err(ctx, SIHIP_EINVAL, "%s: NULL argument", fn);
     CacheArgs C;
     const int rc = check_cache(ctx, fn, cache, C);
-    return rc ? rc : plan_attn(ctx, fn, C, batch, a, P);
+    return rc ? rc : plan_attn(ctx, fn, C, ap_tile_waves(C.hd), batch, a, P);
 }
 
 }  // namespace

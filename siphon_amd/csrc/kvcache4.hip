@@ -84,7 +84,8 @@ int plan_attn4(sihip_ctx *ctx, const sihip_kv4_cache *cache, const sihip_kv_batc
     const char *fn = "attn_paged4_dev";
     const int rc = check_cache4(ctx, fn, cache, C);
     if (rc) return rc;
-    return plan_attn(ctx, fn, {(int8_t *)C.k, (int8_t *)C.v, nullptr, nullptr, C.n_pages, C.n_kv, C.hd, C.shift}, batch, a, P);
+    return plan_attn(ctx, fn, {(int8_t *)C.k, (int8_t *)C.v, nullptr, nullptr, C.n_pages, C.n_kv, C.hd, C.shift}, ap4_tile_waves(C.hd), batch, a,
+                     P);
 }
 
 int launch_attn4(sihip_ctx *ctx, const Cache4Args &C, const AttnPLaunch &L, hipStream_t st) {

@@ -145,9 +145,8 @@ constexpr int kApFewRows = 64;
 //   14 heads of 64 on 2: 1200 27 / 33, 4096 133 / 124; 32 on 8: 4096 239 / 171
 //   wider than 128 the large blocks' sums would leave one wave a SIMD: 16 heads of
 //     256, 4096 rows 467, 627 in a build that had them
-int attn_waves(const sihip_ctx *ctx, const AttnPArgs &A, int64_t rows, int64_t all_rows) {
+int attn_waves(const sihip_ctx *ctx, const AttnPArgs &A, int waves, int64_t rows, int64_t all_rows) {
     if (A.C.hd > 128) return 0;
-    const int waves = ap_tile_waves(A.C.hd);
     if (ctx->opt.attnp_large >= 0) return ctx->opt.attnp_large ? waves : 0;
     if (rows <= 32) return 0;
     int64_t keys = A.R.max_kv - A.R.max_q / 2;  // of a row, on average, without a window
@@ -225,8 +224,8 @@ int plan_launch(sihip_ctx *ctx, const char *fn, AttnPLaunch &L, int64_t rows, in
     return SIHIP_OK;
 }
 
-// C: the cache, which the caller has checked.
-int plan_attn(sihip_ctx *ctx, const char *fn, const CacheArgs &C, const sihip_kv_batch *batch, const sihip_attn_paged *a,
+// C: the cache, which the caller has checked; waves: of a large row block.
+int plan_attn(sihip_ctx *ctx, const char *fn, const CacheArgs &C, int waves, const sihip_kv_batch *batch, const sihip_attn_paged *a,
               AttnPPlan &P) {
     if (!a) return set_err(ctx, SIHIP_EINVAL, "%s: NULL argument", fn);
     AttnPArgs A = {};
@@ -270,7 +269,7 @@ int plan_attn(sihip_ctx *ctx, const char *fn, const CacheArgs &C, const sihip_kv
     A.least = 0;
     A.most = INT32_MAX;
     P.l[0].A = A;
-    P.l[0].waves = attn_waves(ctx, A, rows, all_rows);
+    P.l[0].waves = attn_waves(ctx, A, waves, rows, all_rows);
     P.n = 1;
     // Lengths that differ: a request of few rows would fill little of a large
     // block, and go through all its keys in it alone
