@@ -9,13 +9,12 @@
 // probability, log l is what the others add to 1.
 //
 // The most likely: of a logit and its index a key is made, a 64-bit number that grows with the
-// logit and, of equal ones, falls with the index, so that no two are equal. A wave keeps a
-// threshold that n_top of the keys it has seen reach, and puts the keys that reach it
-// into a list in LDS. The first threshold is the n_topth largest of the lanes' largest keys
-// (each lane has one that reaches it, so n_top keys do); a list that is full is cut to its n_top
-// largest, found by counting for each key how many are larger, and the threshold goes up to
-// the last of them. Most of the time no logit of a wave reaches the threshold, which costs a
-// comparison a lane.
+// logit and, of equal ones, falls with the index, so that no two are equal. The pass itself keeps the
+// largest of each thread's 16 logits at a time, no more. Every kLpRounds of them a wave finds the n_topth largest of
+// its lanes' largest (each lane has one that reaches it, so n_top keys do): what is below is not among the most
+// likely. The few runs of 16 that reach it are read again, four lanes a run, and the keys that reach it
+// go to a list in LDS. A list that is full is cut to its n_top largest, found by counting for each key how
+// many are larger, and the threshold goes up to the last of them.
 #pragma once
 
 #include <float.h>
@@ -44,6 +43,7 @@ constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
 constexpr int kLpMostTop = 64;  // keys that a wave can choose with a lane each
 constexpr int kLpList = 192;
 constexpr int kLpGroup = 4;     // 16-byte loads of a thread at a time
+constexpr int kLpRounds = 8;    // of them between choices
 
 // bytes of a split's part
 __host__ __device__ inline int64_t lp_part_bytes(int n_top) { return 32 + (int64_t)(n_top + 1) / 2 * 16; }
@@ -85,7 +85,7 @@ __device__ inline int32_t lp_index(uint64_t key) { return (int32_t)(0xffffffffu 
 // how many of n keys in LDS are larger (n is padded to even with zeros)
 __device__ inline int lp_larger(const uint64_t *keys, int n, uint64_t key) {
     int k = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < n; i += 2) {
         const ulonglong2 o = *(const ulonglong2 *)(keys + i);
         k += (o.x > key) + (o.y > key);
@@ -126,38 +126,33 @@ struct LpChoice {
             least = last > least ? last : least;
         }
     }
-    // E keys a lane, 0 for none
-    template <int E>
-    __device__ void show(const uint64_t (&key)[E]) {
+    // raises the threshold to the n_topth largest of a key of each lane, that is reached by one of its keys
+    __device__ void limit(uint64_t key) {
         const int lane = threadIdx.x & 63;
-        uint64_t best = key[0];
-#pragma unroll
-        for (int e = 1; e < E; e++) best = key[e] > best ? key[e] : best;
-        if (__popcll(__ballot(best >= least)) >= n_top) {
-            uint64_t *all = list + kLpList;
-            all[lane] = best;
-            fence();
-            const int rank = lp_larger(all, 64, best);
-            const uint64_t last = __ballot(best && rank == n_top - 1);
-            if (last) {
-                const int from = __ffsll((unsigned long long)last) - 1;
-                const uint64_t k = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(best >> 32), from) << 32 |
-                                   (uint32_t)__builtin_amdgcn_readlane((int)best, from);
-                least = k > least ? k : least;
-            }
-            fence();
+        if (__popcll(__ballot(key >= least)) < n_top) return;
+        uint64_t *all = list + kLpList;
+        all[lane] = key;
+        fence();
+        const int rank = lp_larger(all, 64, key);
+        const uint64_t last = __ballot(key && rank == n_top - 1);
+        if (last) {
+            const int from = __ffsll((unsigned long long)last) - 1;
+            const uint64_t k = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), from) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane((int)key, from);
+            least = k > least ? k : least;
         }
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            uint64_t takes = __ballot(key[e] >= least);
-            if (!takes) continue;
-            if (count + __popcll(takes) > kLpList - 1) {
-                cut();
-                takes = __ballot(key[e] >= least);
-            }
-            if (key[e] >= least) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(takes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)takes, 0))] = key[e];
-            count += __popcll(takes);
+        fence();
+    }
+    // a key a lane, 0 for none
+    __device__ void take(uint64_t key) {
+        uint64_t takes = __ballot(key >= least);
+        if (!takes) return;
+        if (count + __popcll(takes) > kLpList - 1) {
+            cut();
+            takes = __ballot(key >= least);
         }
+        if (key >= least) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(takes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)takes, 0))] = key;
+        count += __popcll(takes);
         fence();
     }
 };
@@ -171,57 +166,100 @@ typedef uint32_t lp_u2 __attribute__((ext_vector_type(2)));
 template <bool TOP>
 __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs A) {
     __shared__ __attribute__((aligned(16))) uint64_t lists[TOP ? kLpWaves : 1][TOP ? kLpList + 64 : 1];
-    __shared__ __attribute__((aligned(16))) uint64_t chosen[TOP ? kLpWaves * kLpMostTop + 2 : 2];
+    __shared__ float largest[TOP ? kLpWaves : 1][TOP ? kLpRounds : 1][64];  // of a thread's 16 logits; then runs to read again
+    __shared__ uint64_t chosen[kLpMostTop];
+    __shared__ int counts[kLpWaves];
     __shared__ LpSums sums[kLpWaves];
     __shared__ uint32_t last;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t row = blockIdx.x / A.n_split;
     const int split = blockIdx.x % A.n_split;
     const float *x = A.x + row * A.ld;
-    const int skew = (int)((uintptr_t)x >> 2 & 3);  // elements of the first granule before the row
-    const int64_t granules = (A.n + skew + 3) / 4;
-    const int64_t g0 = split * A.per_split, g1 = min(g0 + A.per_split, granules);
+    // places of logits: from the start of the row's first granule, of which `skew` elements lie before the row
+    const uint32_t skew = (uint32_t)((uintptr_t)x >> 2 & 3), end = (uint32_t)A.n + skew;
+    const uint32_t p0 = (uint32_t)min((int64_t)split * A.per_split * 4, (int64_t)end), p1 = (uint32_t)min((int64_t)(split + 1) * A.per_split * 4, (int64_t)end);
 
     LpSums S = LpSums::none();
     LpChoice C;
     C.list = lists[TOP ? wave : 0];
     C.n_top = A.n_top;
-    for (int64_t g = g0; g < g1; g += kLpThreads * kLpGroup) {
+    constexpr uint32_t kRound = kLpThreads * kLpGroup * 4, kStep = kLpThreads * 4;
+    auto load4 = [&](uint32_t p, float *v) {
+        if (p >= skew && p + 4 <= p1) {
+            const float4 f = *(const float4 *)(x + (p - skew));
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = p + e >= skew && p + e < p1 ? x[p + e - skew] : -INFINITY;
+        }
+    };
+    auto key_at = [&](float v, uint32_t p) { return p >= skew && p < p1 ? lp_key(v, p - skew) : 0; };
+    for (uint32_t first = p0; first < p1; first += kLpRounds * kRound) {
+        const int rounds = (int)min((p1 - first + kRound - 1) / kRound, (uint32_t)kLpRounds);
         float v[4 * kLpGroup];
+        for (int r = 0; r < rounds; r++) {
 #pragma unroll
-        for (int k = 0; k < kLpGroup; k++) {
-            const int64_t at = g + k * kLpThreads + tid, i = 4 * at - skew;
-            if (at < g1 && i >= 0 && i + 4 <= A.n) {
-                const float4 f = *(const float4 *)(x + i);
-                v[4 * k] = f.x, v[4 * k + 1] = f.y, v[4 * k + 2] = f.z, v[4 * k + 3] = f.w;
-            } else {
+            for (int k = 0; k < kLpGroup; k++) load4(first + r * kRound + k * kStep + 4 * tid, v + 4 * k);
+            float most = v[0];
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[4 * k + e] = at < g1 && i + e >= 0 && i + e < A.n ? x[i + e] : -INFINITY;
+            for (int e = 1; e < 4 * kLpGroup; e++) most = fmaxf(most, v[e]);
+            if (most > S.m) S.raise(most);
+            float t = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4 * kLpGroup; e++) {
+                const float d = v[e] - S.m, p = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+                S.l += (double)p;
+                t = fmaf(p, fmaxf(d, -1e4f), t);  // (where p is zero d may be infinite)
             }
+            S.t += (double)t;
+            if constexpr (TOP) largest[wave][r][lane] = most;
         }
-        float most = v[0];
+        if constexpr (!TOP) continue;
+        if (rounds == 1) {  // they are still here
+            uint64_t key[4 * kLpGroup], low = 0;
 #pragma unroll
-        for (int e = 1; e < 4 * kLpGroup; e++) most = fmaxf(most, v[e]);
-        if (most > S.m) S.raise(most);
-        float t = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4 * kLpGroup; e++) {
-            const float d = v[e] - S.m, p = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
-            S.l += (double)p;
-            t = fmaf(p, fmaxf(d, -1e4f), t);  // (where p is zero d may be infinite)
-        }
-        S.t += (double)t;
-        if constexpr (TOP) {
-            if (__any(lp_key(most, 0) >= C.least)) {
-                uint64_t key[4 * kLpGroup];
-#pragma unroll
-                for (int e = 0; e < 4 * kLpGroup; e++) {
-                    const int64_t at = g + e / 4 * kLpThreads + tid, i = 4 * at - skew + e % 4;
-                    key[e] = at < g1 && i >= 0 && i < A.n ? lp_key(v[e], (uint32_t)i) : 0;
-                }
-                C.show(key);
+            for (int e = 0; e < 4 * kLpGroup; e++) {
+                key[e] = key_at(v[e], first + e / 4 * kStep + 4 * tid + e % 4);
+                low = key[e] > low ? key[e] : low;
             }
+            C.limit(low);
+#pragma unroll
+            for (int e = 0; e < 4 * kLpGroup; e++) C.take(key[e]);
+            continue;
         }
+        // runs of 16, by the bounds of their largest key: its place is between the run's first and last
+        LpChoice::fence();
+        const uint32_t mine = first + 4 * tid;
+        uint64_t low = 0;
+        for (int r = 0; r < rounds; r++) {
+            const uint32_t p = mine + r * kRound;
+            const uint64_t k = p < p1 ? lp_key(largest[wave][r][lane], p + 3 * kStep + 3) : 0;
+            low = k > low ? k : low;
+        }
+        C.limit(low);
+        uint32_t reach = 0;
+        for (int r = 0; r < rounds; r++) {
+            const uint32_t p = mine + r * kRound;
+            if (p < p1 && lp_key(largest[wave][r][lane], p > skew ? p - skew : 0) >= C.least) reach |= 1u << r;
+        }
+        LpChoice::fence();
+        uint16_t *runs = (uint16_t *)largest[wave];
+        int n = 0;
+        for (int r = 0; r < rounds; r++) {
+            const uint64_t all = __ballot(reach >> r & 1);
+            if (reach >> r & 1) runs[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0))] = r << 6 | lane;
+            n += __popcll(all);
+        }
+        LpChoice::fence();
+        for (int j = lane >> 2; __any(j < n); j += 16) {
+            const int run = j < n ? runs[j] : 0;
+            const uint32_t p = j < n ? first + (run >> 6) * kRound + (lane & 3) * kStep + 4 * (wave * 64 + (run & 63)) : p1;
+            float v[4];
+            load4(p, v);
+#pragma unroll
+            for (int e = 0; e < 4; e++) C.take(key_at(v[e], p + e));
+        }
+        LpChoice::fence();
     }
     // the workgroup's sums and choice
     auto join = [&]() {
@@ -234,27 +272,25 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs A) {
         }
         if (lane == 0) sums[wave] = S;
         if constexpr (TOP) {
-            C.cut();
-            chosen[wave * A.n_top + min(lane, A.n_top - 1)] = 0;
-            LpChoice::fence();
-            if (lane < min(C.count, A.n_top)) chosen[wave * A.n_top + lane] = C.list[lane];
-            if (tid < 2) chosen[kLpWaves * A.n_top + tid] = 0;
+            if (C.count > 64) C.cut();
+            if (lane == 0) {
+                counts[wave] = C.count;
+                C.list[C.count] = 0;
+            }
+            if (tid < A.n_top) chosen[tid] = 0;
         }
         __syncthreads();
         S = sums[0];
 #pragma unroll
         for (int w = 1; w < kLpWaves; w++) S.add(sums[w]);
-        uint64_t key = 0;
-        int rank = kLpMostTop;
         if constexpr (TOP) {
-            if (tid < kLpWaves * A.n_top) {
-                key = chosen[tid];
-                if (key) rank = lp_larger(chosen, kLpWaves * A.n_top, key);
+            if (lane < C.count) {
+                const uint64_t key = C.list[lane];
+                int rank = 0;
+#pragma unroll
+                for (int w = 0; w < kLpWaves; w++) rank += lp_larger(lists[w], counts[w], key);
+                if (rank < A.n_top) chosen[rank] = key;
             }
-            __syncthreads();
-            if (tid < A.n_top) chosen[tid] = 0;
-            __syncthreads();
-            if (rank < A.n_top) chosen[rank] = key;
         }
         __syncthreads();
     };
@@ -304,7 +340,12 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs A) {
                         key[e] = (uint64_t)w.y << 32 | w.x;
                     }
                 }
-                C.show(key);
+                uint64_t low = key[0];
+#pragma unroll
+                for (int e = 1; e < 4; e++) low = key[e] > low ? key[e] : low;
+                C.limit(low);
+#pragma unroll
+                for (int e = 0; e < 4; e++) C.take(key[e]);
             }
         }
         __syncthreads();
