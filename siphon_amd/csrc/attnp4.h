@@ -624,33 +624,25 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
 // attnp_tiles_kernel (attnp.h) over 4-bit values: the codes of a 64-key chunk become f16 numbers
 // once, code * sub, on their way into LDS; the scales of its keys and values lie there beside
 // them, as f32. A unit of 16 values is 8 bytes here.
-// Order of N operands from LDS, two products each: the reads are kAhead operands before their use.
-// (Left to itself the compiler reads each where it is used, and the products wait 16 times a half.)
-template <int N>
-__device__ __forceinline__ void ap4_reads_ahead() {
-    constexpr int kAhead = N < 3 ? N : 3, kRead = 0x100, kProduct = 0x8;
-    __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
-#pragma unroll
-    for (int i = 0; i < N - kAhead; i++) {
-        __builtin_amdgcn_sched_group_barrier(kProduct, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(kProduct, 2 * kAhead, 0);
+// x of another lane of the row of 16
+template <int CTRL>
+__device__ inline float ap4_from(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
 
-constexpr int ap4_tile_waves(int hd) { return 4; }
+constexpr int ap4_tile_waves(int hd) { return hd <= 64 ? 4 : 8; }
 
 template <int NS, int WAVES = ap4_tile_waves(16 * NS)>
 __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kernel(Attn4Args A) {
     constexpr int kApTileRows = 32 * WAVES, kApTileThreads = 64 * WAVES;
-    constexpr bool kTurns = WAVES == 8;
     constexpr int ND = (NS + 1) / 2;             // 32-dim tiles of the output
     constexpr int KC = (2 * NS + 7) / 8 * 8;     // granules of a key row in LDS
     constexpr int NU = (64 * NS + kApTileThreads - 1) / kApTileThreads;  // 8-byte loads of a chunk, each
     __shared__ uint4 k_lds[2][64][KC];
     __shared__ uint4 v_lds[2][ND * 32][8];
+    __shared__ uint4 q_lds[WAVES][NS][64];  // the lower halves of each wave's queries
     __shared__ __attribute__((aligned(16))) float s_lds[2][2][64];  // scales of keys and values
-    __shared__ int p_lds[2][4];  // whether a segment of 16 has a page
+    __shared__ __attribute__((aligned(16))) float m_lds[2][4];  // the largest scale of a segment of 16 values, -1 without a page
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
     const int h = blockIdx.x % A.C.n_kv, split = blockIdx.y;
@@ -668,7 +660,6 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
 
     // the wave's rows and this lane's
     const int row0 = tile * kApTileRows + wave * 32;
-    const bool idle = row0 >= n_rows;
     const int row = min(row0 + col, n_rows - 1), tok = row / A.G, head = h * A.G + row % A.G, p = s.p0 + tok;
     Sight W = S;
     W.p_lo = s.p0 + min(row0, n_rows - 1) / A.G;
@@ -693,6 +684,7 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
     uint32_t koff[NU], ksoff[NU], voff[NU], vsoff[NU];  // in a page, without the chunk's place
     uint32_t kr[NU][2], ksub[NU], vr[NU][2], vsub[NU][2], scale;
     int ek[NU], ev, vpg = -1;  // entries; the page of this thread's values and scale
+    bool seen = false;         // some row may see the key of `scale`
 #pragma unroll
     for (int i = 0; i < NU; i++) {
         const int key = unit(i) / NS, d = unit(i) % NS * 16 < hd ? unit(i) % NS * 16 : 0;
@@ -719,6 +711,9 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
             ksub[i] = *(const uint8_t *)(A.ksub + (pg * page_subs + at + ksoff[i]));
         }
         vpg = page_of(j0 + seg, ev);
+        // (what no row sees may have any scale, and counts as zero)
+        const int j = j0 + scaled;
+        seen = vpg >= 0 && j < S.keys && (!A.window || j > S.p_lo - A.window || j < S.prefix);
         if (tid < 128) scale = (tid < 64 ? A.kd : A.vd)[(uint64_t)(uint32_t)max(vpg, 0) * page_scales + at + soff];
     };
     auto load_values = [&](int u) {
@@ -744,8 +739,15 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
             k_lds[buf][key][(2 * d16) ^ x] = __builtin_bit_cast(uint4, ap4_cvt(kr[i][0], s));
             k_lds[buf][key][(2 * d16 + 1) ^ x] = __builtin_bit_cast(uint4, ap4_cvt(kr[i][1], s));
         }
-        if (tid < 128) s_lds[buf][tid >> 6][scaled] = ap4_bf16(scale, 0);
-        if (tid < 8) p_lds[buf][tid >> 1] = vpg >= 0;
+        if (tid < 128) {
+            const float x = seen ? ap4_bf16(scale, 0) : 0.0f;
+            s_lds[buf][tid >> 6][scaled] = x;
+            // the segment's 16 values are those of the lanes that differ in bits 0, 3, 4 and 5
+            float most = fmaxf(x, ap4_from<0xb1>(x));
+            most = fmaxf(most, ap4_from<0x128>(most));
+            most = ap_max_quarters(most);
+            if (tid >= 64 && tid < 72) m_lds[buf][tid >> 1 & 3] = vpg >= 0 ? most : -1.0f;
+        }
     };
     auto put_values = [&](int buf) {
 #pragma unroll
@@ -766,7 +768,7 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
         load_values(u0);
     }
     // the query, while the first chunk is on its way
-    ap_h8 qh[NS], ql[NS];
+    ap_h8 qh[NS];
     float f_row, fc_row;
     {
         const float sign = A.scale2 > 0.0f ? A.sign : 0.0f;  // (no scale: a score is zero whatever the key)
@@ -785,7 +787,9 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
         for (int c = 0; c < NS; c++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) x[c][j] = ldexpf(x[c][j], e2);
-            ap_split8(x[c], qh[c], ql[c]);
+            ap_h8 lo;
+            ap_split8(x[c], qh[c], lo);
+            q_lds[wave][c][lane] = __builtin_bit_cast(uint4, lo);
         }
         f_row = ldexpf(kAp4Unit, -e2);
         fc_row = fminf(f_row * A.cap_in, FLT_MAX);
@@ -796,19 +800,13 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    // nothing in a chunk for this wave's rows
-    auto blind = [&](int u) {
-        const int j0 = ap_chunk(S, u) * 64;
-        return idle || (j0 >= S.prefix && (j0 > W.p_hi || (A.window && j0 + 63 <= W.p_lo - A.window)));
-    };
     // where this lane's operands lie in LDS: the granules of a row are permuted by an exclusive or, so
     // that another granule is another exclusive or of the address. The empty statements keep
     // the compiler from holding all of these in registers, which the operands need.
     const int key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
     const uint32_t k_at = key * KC * 16 + ((half ^ (KC % 16 ? (col >> 1) & 7 : col & 15)) << 4);
     const uint32_t v_at = col * 128 + ((2 * half ^ ((col >> 1) & 7)) << 4);
-    ap_f16 sc;
-    auto scores = [&](int buf, int i) {
+    auto scores = [&](ap_f16 &sc, int buf, int i) {
         uint32_t at = k_at + (64 * buf + 32 * i) * KC * 16;
         asm("" : "+v"(at));
 #pragma unroll
@@ -817,10 +815,10 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
         for (int c = 0; c < NS; c++) {
             const ap_h8 a = *(const ap_h8 *)((const char *)k_lds + (at ^ c << 5));
             sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], sc, 0, 0, 0);
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, __builtin_bit_cast(ap_h8, q_lds[wave][c][lane]), sc, 0, 0, 0);
         }
-        ap4_reads_ahead<NS>();
     };
+    ap_f16 sc;
     if (u0 < u1) {
         put_keys(0);
         put_values(0);
@@ -828,22 +826,22 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
         load_entries(min(u0 + 2, u1 - 1));
         load_values(min(u0 + 1, u1 - 1));
         __syncthreads();
-        if (!blind(u0)) scores(0, 0);
-        if (kTurns && wave >= 4) __syncthreads();
+        scores(sc, 0, 0);
     }
     for (int u = u0; u < u1; u++) {
         const int buf = (u - u0) & 1, j0 = ap_chunk(S, u) * 64;
-        const bool skip = blind(u), whole = ap_whole(A, W, j0, 64);
+        const bool whole = ap_whole(A, W, j0, 64);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            // weights of the half's 32 keys, and a part of the next chunk
-            ap_h8 ph[2], pl[2];
-            if (!skip) {
+            {
                 // scores in log2 units are sc * f
+                const float4 vm = *(const float4 *)m_lds[buf];
+                const float vmax = i == 0 ? (half ? vm.y : vm.x) : (half ? vm.w : vm.z);
+                const float *kd = &s_lds[buf][0][32 * i + 16 * half], *vd = &s_lds[buf][1][32 * i + 16 * half];
                 float f = f_row;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float4 d = *(const float4 *)&s_lds[buf][0][32 * i + 16 * half + 4 * e];
+                    const float4 d = ((const float4 *)kd)[e];
                     sc[4 * e] *= d.x, sc[4 * e + 1] *= d.y, sc[4 * e + 2] *= d.z, sc[4 * e + 3] *= d.w;
                 }
                 if (A.cap != 0.0f) {
@@ -863,10 +861,8 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
                     }
                     f = 1.0f;
                 }
-                const bool here = p_lds[buf][2 * i + half], cut = !whole || __any(!here);
-                uint32_t hidden = 0;
-                if (cut) {
-                    hidden = here ? ap_hidden(A, S, p, j1) : 0xffffu;
+                if (!whole || __any(vmax < 0.0f)) {
+                    const uint32_t hidden = vmax < 0.0f ? 0xffffu : ap_hidden(A, S, p, j1);
 #pragma unroll
                     for (int e = 0; e < 16; e++) sc[e] = ap_hide(sc[e], hidden, e);
                 }
@@ -874,49 +870,35 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
 #pragma unroll
                 for (int e = 1; e < 16; e++) mx = fmaxf(mx, sc[e]);
                 mx *= f;
-                if (__any(mx > R.m + kApLate)) {
-                    const float ao = R.refer(R.raise(ap_max_halves(mx)), 0.0f);
+                // no product of a weight and its scale is more than the largest weight times the
+                // largest scale: only where that passes the reference the products are looked at
+                int late = __any(R.late(mx, __builtin_amdgcn_exp2f(fminf(mx - R.m, kApLate)) * vmax));
+                while (late) {
+                    const float am = R.raise(ap_max_halves(mx));
+                    float most = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) most = fmaxf(most, __builtin_amdgcn_exp2f(fmaf(sc[e], f, -R.m)) * vd[e]);
+                    const float ao = R.refer(am, ap_max_halves(most));
 #pragma unroll
                     for (int d = 0; d < ND; d++) o[d] *= ao;
+                    late = 0;
+                    asm("" : "+s"(late));
                 }
-                // weights, and their products with the values' scales
-                float z[16], most = 0.0f;
+                asm("" : "+v"(R.m));
+                // the next half's scores (behind the last chunk: of what is there, for nobody) beside the weights
+                ap_f16 next;
+                scores(next, i == 0 ? buf : buf ^ 1, i ^ 1);
+                float z[16];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float4 d = *(const float4 *)&s_lds[buf][1][32 * i + 16 * half + 4 * e];
-                    const float v[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float w = __builtin_amdgcn_exp2f(fmaf(sc[4 * e + k], f, -R.m));
-                        R.l += w;
-                        z[4 * e + k] = w * v[k];
-                    }
+                for (int e = 0; e < 16; e++) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[e], f, -R.m));
+                    R.l += w;
+                    z[e] = w * vd[e];
                 }
-                if (cut) {  // (what was never written may have any scale)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) z[e] = hidden >> e & 1 ? 0.0f : z[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 16; e++) most = fmaxf(most, z[e]);
-                if (__any(most > 16.0f * R.ref)) {
-                    const float ao = R.refer(1.0f, ap_max_halves(most));
-#pragma unroll
-                    for (int d = 0; d < ND; d++) o[d] *= ao;
-                }
+                ap_h8 ph[2], pl[2];
 #pragma unroll
                 for (int e = 0; e < 2; e++) ap_split8w(z + 8 * e, R.over, ph[e], pl[e]);
-            }
-            if (i == 0) {
-                if (u + 1 < u1) put_keys(buf ^ 1);
-                load_keys(min(u + 2, u1 - 1));
-                load_entries(min(u + 3, u1 - 1));
-            } else {
-                if (u + 1 < u1) put_values(buf ^ 1);
-                load_values(min(u + 2, u1 - 1));
-            }
-            __syncthreads();
-            // their products with the values, and the next half's scores
-            if (!skip) {
+                // and their products with the values
                 uint32_t at = v_at + buf * ND * 32 * 128;
                 asm("" : "+v"(at));
 #pragma unroll
@@ -927,14 +909,19 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[e], o[d], 0, 0, 0);
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[e], o[d], 0, 0, 0);
                     }
-                ap4_reads_ahead<2 * ND>();
-                if (i == 0) scores(buf, 1);
+                sc = next;
             }
-            if (i == 1 && u + 1 < u1 && !blind(u + 1)) scores(buf ^ 1, 0);
+            if (i == 0) {
+                put_keys(buf ^ 1);
+                load_keys(min(u + 2, u1 - 1));
+                load_entries(min(u + 3, u1 - 1));
+            } else {
+                put_values(buf ^ 1);
+                load_values(min(u + 2, u1 - 1));
+            }
             __syncthreads();
         }
     }
-    if (kTurns && u0 < u1 && wave < 4) __syncthreads();
     float m = R.m, l = R.l;
     l += __shfl_xor(l, 32);
 
