@@ -78,7 +78,7 @@ constexpr int k4Chunk = 64;  // tokens of a page at a time
 constexpr float k4Most = 0x1p126f;  // larger magnitudes count as this one for the steps
 
 // x / step rounded to an integer, ties to even, exactly (quantize_exact says
-// how; step = sub * scale has 15 bits), at most 7 and at least -8. NaN and a step of zero: 0.
+// how; step = |sub| * scale has 15 bits), at most 7 and at least -8. NaN and a step of zero: 0.
 __device__ inline int kv4_code(float x, float step, float inv) {
     if (x != x || step == 0.0f) return 0;
     float q = rintf(x * inv);
@@ -89,14 +89,96 @@ __device__ inline int kv4_code(float x, float step, float inv) {
     return (int)fminf(fmaxf(q, -8.0f), 7.0f);
 }
 
+// x of another lane of the row of 16
+template <int CTRL>
+__device__ inline float kv4_from(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+
 // the largest of eight lanes in a row (lanes 8 i .. 8 i + 7)
 __device__ inline float kv4_max8(float x) {
-    auto from = [&](auto ctrl) {
-        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
-    };
-    x = fmaxf(x, from(std::integral_constant<int, 0xb1>()));   // lane ^ 1
-    x = fmaxf(x, from(std::integral_constant<int, 0x4e>()));   // lane ^ 2
-    return fmaxf(x, from(std::integral_constant<int, 0x141>()));  // 7 - lane of eight
+    x = fmaxf(x, kv4_from<0xb1>(x));      // lane ^ 1
+    x = fmaxf(x, kv4_from<0x4e>(x));      // lane ^ 2
+    return fmaxf(x, kv4_from<0x141>(x));  // 7 - lane of eight
+}
+
+struct Kv4Step {
+    float sub, scale;  // sub is a whole number
+};
+
+// The sub and the scale of this lane's group of 32: eight lanes have it, four values each, and hd / 4
+// lanes from `row0` on have the row.
+__device__ inline Kv4Step kv4_step(const float *v, int hd, int row0) {
+    float most = kv4_max8(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+    float low = fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
+    if (__any(!(most < INFINITY) || !(low > -INFINITY))) {  // (numbers alone count)
+        float a = 0.0f;
+        low = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float f = fabsf(v[e]) < INFINITY ? v[e] : 0.0f;
+            a = fmaxf(a, fabsf(f));
+            low = fminf(low, f);
+        }
+        most = kv4_max8(a);
+    }
+    most = fminf(most, k4Most);
+    // the largest is negative in one of the eight lanes: code -8 is on that side
+    const bool plus = (__ballot(low <= -most) >> (threadIdx.x & 56) & 255) != 0;
+    const float size = 0.125f * most;  // |step|
+    float row = size;
+    if (hd == 128 || hd == 256 || hd == 64) {
+        row = fmaxf(row, kv4_from<0x128>(row));  // lane ^ 8
+        const uint32_t b = __builtin_bit_cast(uint32_t, row);
+        if (hd >= 128) {
+            const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+            row = fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+        }
+        if (hd == 256) {
+            const uint32_t w = __builtin_bit_cast(uint32_t, row);
+            const auto r = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+            row = fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+        }
+    } else {
+        for (int i = 0; i < hd / 32; i++) row = fmaxf(row, __shfl(size, row0 + 8 * i));
+    }
+    // row / 127, rounded to the nearest (the remainder of the product with the rounded reciprocal is
+    // exact, and corrects it), then up to bfloat16
+    const float rough = row * (1.0f / 127.0f), exact = fmaf(fmaf(-127.0f, rough, row), 1.0f / 127.0f, rough);
+    const uint32_t up = (__builtin_bit_cast(uint32_t, exact) + 0xffffu) & 0xffff0000u;
+    const float scale = row < 0.125f * kTinyAmax ? 0.0f : __builtin_bit_cast(float, up);
+    // |sub|: size / scale up to a whole number; the rough quotient is off by less than one, the
+    // products that show it are exact
+    float n = 1.0f;
+    if (scale > 0.0f) {
+        n = ceilf(size * __builtin_amdgcn_rcpf(scale));
+        if ((n - 1.0f) * scale >= size) n -= 1.0f;
+        else if (n * scale < size) n += 1.0f;
+        n = fminf(fmaxf(n, 1.0f), 127.0f);
+    }
+    return {plus ? n : -n, scale};
+}
+
+// The codes, plus 8, of four values, a byte each. The sum with 1.5 2^23 + 8 leaves the rounded quotient in the
+// low bits; what is within 10^-4 of a border between two codes (or no number) is rounded exactly.
+__device__ inline uint32_t kv4_codes(const float *v, const Kv4Step &q) {
+    constexpr float kMagic = 12582920.0f;
+    const float step = fabsf(q.sub) * q.scale, side = q.sub < 0.0f ? -1.0f : 1.0f;
+    const float inv = step > 0.0f ? side * __builtin_amdgcn_rcpf(step) : 0.0f;
+    bool clear = true;
+    uint32_t c = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float r = fmaf(v[e], inv, kMagic);
+        clear &= fabsf(fmaf(v[e], inv, kMagic - r)) <= 0.4999f;
+        c |= (__builtin_bit_cast(uint32_t, fminf(fmaxf(r, kMagic - 8.0f), kMagic + 7.0f)) & 15u) << (8 * e);
+    }
+    if (clear) return c;
+    const float near = step > 0.0f ? 1.0f / step : 0.0f;
+    c = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) c |= (uint32_t)(kv4_code(side * v[e], step, near) + 8) << (8 * e);
+    return c;
 }
 
 // A workgroup: one page of new tokens and one KV head, keys (z = 0), values (1) or, rotated,
@@ -150,34 +232,8 @@ __global__ __launch_bounds__(k4Threads) void kv4_append_kernel(Append4Args A) {
                 if (p0 + a * per_pass >= t_hi) break;
                 const int t = p0 + a * per_pass + wave * per_wave + of;
                 const float v[4] = {val[a].x, val[a].y, val[a].z, val[a].w};
-                float top = 0.0f, low = 0.0f;  // of the finite values, low: of their negatives
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float f = fabsf(v[e]) < INFINITY ? v[e] : 0.0f;
-                    top = fmaxf(top, f);
-                    low = fmaxf(low, -f);
-                }
-                top = fminf(kv4_max8(top), k4Most);
-                low = fminf(kv4_max8(low), k4Most);
-                const float size = 0.125f * fmaxf(top, low);  // |step|
-                float most = 0.0f;
-                for (int i = 0; i < hd / 32; i++) most = fmaxf(most, __shfl(size, row0 + 8 * i));
-                // up to bfloat16
-                const uint32_t up = (__builtin_bit_cast(uint32_t, most / 127.0f) + 0xffffu) & 0xffff0000u;
-                const float scale = most < 0.125f * kTinyAmax ? 0.0f : __builtin_bit_cast(float, up);
-                // |sub|: size / scale up to a whole number; the products are exact
-                float n = 1.0f;
-                if (scale > 0.0f) {
-                    n = ceilf(size / scale);
-                    if ((n - 1.0f) * scale >= size) n -= 1.0f;
-                    else if (n * scale < size) n += 1.0f;
-                    n = fminf(fmaxf(n, 1.0f), 127.0f);
-                }
-                const bool minus = !(low >= top);  // the largest is positive: its code is -8
-                const float step = n * scale, inv = step > 0.0f ? 1.0f / step : 0.0f;
-                uint32_t c = 0;
-#pragma unroll
-                for (int e = 0; e < 4; e++) c |= (uint32_t)(kv4_code(minus ? -v[e] : v[e], step, inv) + 8) << (8 * e);
+                const Kv4Step q = kv4_step(v, hd, row0);
+                const uint32_t c = kv4_codes(v, q);
                 const bool here = of < per_wave && t < t_hi;
                 if (is_v) {
                     if (here) turn[(t - c0) * pitch + li] = c;
@@ -186,8 +242,8 @@ __global__ __launch_bounds__(k4Threads) void kv4_append_kernel(Append4Args A) {
                     w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xb1, 0xf, 0xf, true);
                     if (here && !(li & 1)) codes[t * (hd / 8) + li / 2] = w;
                 }
-                if (here && li % 8 == 0) subs[((li / 8) << shift) + t] = (int8_t)(minus ? -n : n);
-                if (here && li == 0) scales[t] = (uint16_t)(__builtin_bit_cast(uint32_t, scale) >> 16);
+                if (here && li % 8 == 0) subs[((li / 8) << shift) + t] = (int8_t)q.sub;
+                if (here && li == 0) scales[t] = (uint16_t)(__builtin_bit_cast(uint32_t, q.scale) >> 16);
             }
         }
         if (!is_v) continue;
