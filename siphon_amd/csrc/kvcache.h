@@ -221,7 +221,6 @@ __device__ inline PageSpan page_span(const BatchArgs &A, int r, int j, int shift
 // ---- append ------------------------------------------------------------------------
 
 struct AppendArgs {
-    static constexpr bool kRotates = false;
     CacheArgs C;
     BatchArgs R;
     const float *k, *v;
@@ -306,11 +305,12 @@ __device__ inline int requantize_exact(int code, float was, float now, double in
 // Where every page's scale grows, and its old codes are rounded again in f64,
 // 10.3 us, and 21.3 for the chunks.
 //
-// Args: AppendArgs, or AppendRopeArgs (kvrope.h), whose keys are rotated on the way and whose third
-// layer of workgroups rotates the queries. (The body as a function that two kernels call took 82
+// Rope: none, or KeyRope (kvrope.h), by which keys are rotated on the way and a third layer of
+// workgroups rotates the queries. (The body as a function that two kernels call took 82
 // registers in place of 52, and prompts of 1000 tokens 37 us in place of 35.)
-template <int U, int THREADS, class Args = AppendArgs>
-__global__ __launch_bounds__(THREADS) void kv_append_kernel(Args A) {
+template <int U, int THREADS, class... Rope>
+__global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs A, Rope... rope) {
+    constexpr bool kRotates = sizeof...(Rope) > 0;
     __shared__ float wave_max[THREADS / 64];
     const int h = blockIdx.x % A.C.n_kv, j = blockIdx.x / A.C.n_kv, r = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
@@ -319,9 +319,9 @@ __global__ __launch_bounds__(THREADS) void kv_append_kernel(Args A) {
     const int64_t base = g.base;
     const int lo = g.lo, hi = g.hi;
     if (lo >= hi) return;
-    if constexpr (Args::kRotates) {
+    if constexpr (kRotates) {
         if (blockIdx.z == 2) {
-            A.template queries<THREADS>(g, h);
+            (rope.template queries<THREADS>(g, hd, h), ...);
             return;
         }
     }
@@ -353,8 +353,8 @@ __global__ __launch_bounds__(THREADS) void kv_append_kernel(Args A) {
         } else if (is_v) {
 #pragma unroll
             for (int e = 0; e < 16; e++) val[i][e] = inner + e >= lo && inner + e < hi ? x[(int64_t)(inner + e) * ld + outer] : 0.0f;
-        } else if constexpr (Args::kRotates) {
-            A.key(x + (int64_t)outer * ld, (int)base + outer, inner, val[i]);
+        } else if constexpr (kRotates) {
+            (rope.key(x + (int64_t)outer * ld, (int)base + outer, inner, A.k_wide, val[i]), ...);
         } else if (A.k_wide) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {

@@ -91,11 +91,12 @@ extern "C" int sihip_kv_append_rope_dev(sihip_ctx *ctx, const sihip_kv_cache *ca
                                         const sihip_kv_rows *rows, void *stream) {
     const char *fn = "kv_append_rope_dev";
     if (!ctx) return set_err(ctx, SIHIP_EINVAL, "%s: NULL argument", fn);
-    AppendRopeArgs A;
+    AppendArgs A;
+    KeyRope X;
     int64_t gx = 0;
     int rc = check_cache(ctx, fn, cache, A.C);
     if (!rc) rc = check_batch(ctx, fn, batch, cache->block, A.R);
-    if (!rc) rc = check_rows(ctx, fn, rows, A.R, A.C.n_kv, A.C.hd, A.P, A.Q);
+    if (!rc) rc = check_rows(ctx, fn, rows, A.R, A.C.n_kv, A.C.hd, X.P, X.Q);
     if (!rc && !rows->rope) rc = set_err(ctx, SIHIP_EINVAL, "%s: NULL rope", fn);
     if (!rc) rc = append_grid(ctx, fn, A.R, A.C.n_kv, cache->block, gx);
     if (rc || !gx) return rc;
@@ -105,15 +106,15 @@ extern "C" int sihip_kv_append_rope_dev(sihip_ctx *ctx, const sihip_kv_cache *ca
     A.ldv = rows->ldv;
     A.k_wide = aligned(A.k, 16) && A.ldk % 4 == 0;
     const OnDevice on(ctx->device);
-    const dim3 grid((unsigned)gx, (unsigned)batch->n_req, A.Q.q ? 3 : 2);
+    const dim3 grid((unsigned)gx, (unsigned)batch->n_req, X.Q.q ? 3 : 2);
     const hipStream_t st = (hipStream_t)stream;
     const int64_t units = cache->block * A.C.hd / 16;
-    if (units <= 128) hipLaunchKernelGGL((kv_append_kernel<1, 128, AppendRopeArgs>), grid, dim3(128), 0, st, A);
-    else if (units <= 256) hipLaunchKernelGGL((kv_append_kernel<1, 256, AppendRopeArgs>), grid, dim3(256), 0, st, A);
-    else if (units <= 512) hipLaunchKernelGGL((kv_append_kernel<1, 512, AppendRopeArgs>), grid, dim3(512), 0, st, A);
-    else if (units <= 1024) hipLaunchKernelGGL((kv_append_kernel<1, 1024, AppendRopeArgs>), grid, dim3(1024), 0, st, A);
-    else if (units <= 2048) hipLaunchKernelGGL((kv_append_kernel<2, 1024, AppendRopeArgs>), grid, dim3(1024), 0, st, A);
-    else hipLaunchKernelGGL((kv_append_kernel<4, 1024, AppendRopeArgs>), grid, dim3(1024), 0, st, A);
+    if (units <= 128) hipLaunchKernelGGL((kv_append_kernel<1, 128, KeyRope>), grid, dim3(128), 0, st, A, X);
+    else if (units <= 256) hipLaunchKernelGGL((kv_append_kernel<1, 256, KeyRope>), grid, dim3(256), 0, st, A, X);
+    else if (units <= 512) hipLaunchKernelGGL((kv_append_kernel<1, 512, KeyRope>), grid, dim3(512), 0, st, A, X);
+    else if (units <= 1024) hipLaunchKernelGGL((kv_append_kernel<1, 1024, KeyRope>), grid, dim3(1024), 0, st, A, X);
+    else if (units <= 2048) hipLaunchKernelGGL((kv_append_kernel<2, 1024, KeyRope>), grid, dim3(1024), 0, st, A, X);
+    else hipLaunchKernelGGL((kv_append_kernel<4, 1024, KeyRope>), grid, dim3(1024), 0, st, A, X);
     return launched(ctx, "kv_append_rope");
 }
 

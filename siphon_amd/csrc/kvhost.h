@@ -99,11 +99,11 @@ int check_rows(sihip_ctx *ctx, const char *fn, const sihip_kv_rows *a, const Bat
         P = {a->rope, (int)a->rope_dim / 2, a->rope_neighbours != 0, aligned(a->rope, 16) && a->rope_dim % 8 == 0};
     }
     if (a->q) {
-        const int64_t wide = a->n_head * hd;
         if (!a->rope) return set_err(ctx, SIHIP_EINVAL, "%s: queries without a rotation", fn);
         if (a->n_head < 1 || a->n_head > 4096 || a->n_head % n_kv)
             return set_err(ctx, SIHIP_EINVAL, "%s: n_head %lld must be a multiple of n_head_kv %d (<= 4096)", fn,
                            (long long)a->n_head, n_kv);
+        const int64_t wide = a->n_head * hd;
         if (a->ldq < wide || a->ldq_out < wide)
             return set_err(ctx, SIHIP_EINVAL, "%s: rows of %lld values at ldq %lld, ldq_out %lld", fn, (long long)wide,
                            (long long)a->ldq, (long long)a->ldq_out);

@@ -8,26 +8,25 @@
 
 namespace sihip {
 
-struct AppendRopeArgs : AppendArgs {
-    static constexpr bool kRotates = true;
+struct KeyRope {
     RopeArgs P;
     RopeQueries Q;  // Q.q NULL: none
 
-    // 16 dims, from `inner` on, of the key row x at position p
-    __device__ void key(const float *x, int p, int inner, float *val) const {
+    // 16 dims, from `inner` on, of the key row x at position p; wide: rows and heads are 16-byte aligned
+    __device__ void key(const float *x, int p, int inner, bool wide, float *val) const {
         const float *cs = P.table + (int64_t)p * (2 * P.pairs);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float4 y = rope_load4(P, x, cs, inner + 4 * e, k_wide);
+            const float4 y = rope_load4(P, x, cs, inner + 4 * e, wide);
             val[4 * e] = y.x, val[4 * e + 1] = y.y, val[4 * e + 2] = y.z, val[4 * e + 3] = y.w;
         }
     }
 
     // the queries of KV head h at a page's new tokens
     template <int THREADS>
-    __device__ void queries(const PageSpan &g, int h) const {
+    __device__ void queries(const PageSpan &g, int hd, int h) const {
         const int first = (int)(g.base - g.p0);
-        rope_queries<THREADS>(P, Q, C.hd, h, g.q0, g.p0, first + g.lo, first + g.hi);
+        rope_queries<THREADS>(P, Q, hd, h, g.q0, g.p0, first + g.lo, first + g.hi);
     }
 };
 

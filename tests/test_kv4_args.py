@@ -78,7 +78,7 @@ dev.kv4_append_dev(cache4(), batch(), rows(rope=0, rope_len=0, rope_dim=0, q=0))
 dev.kv_append_rope_dev(cache(), batch(), rows(q=0, q_out=0))
 result = launched()
 """)
-    assert [k for k, *_ in got] == ["kv4_append_kernel"] * 3 + ["kv_append_kernel<1,256>"]
+    assert [k for k, *_ in got] == ["kv4_append_kernel"] * 3 + ["kv_append_kernel<1,256,sihip::KeyRope>"]
 
 
 def test_bad_logprobs_are_refused():
