@@ -56,7 +56,7 @@ def test_bad_rows_are_refused():
     bad = {"k=0": "f32", "v=X + 2": "f32", "ldk=1023": "ldk", "ldv=0": "ldv", "rope_dim=0": "rope_dim", "rope_dim=-2": "rope_dim",
            "rope_dim=127": "rope_dim", "rope_dim=130": "rope_dim", "rope_len=639": "rope_len", "rope_len=0": "rope_len",
            "rope=X + 2": "f32", "q_out=0": "f32", "q_out=X + 2": "f32", "q=X + 1": "f32", "n_head=0": "n_head", "n_head=20": "n_head",
-           "n_head=4104": "n_head", "ldq=4095": "ldq", "ldq_out=100": "ldq", "ldq_out=8192": "in place"}
+           "n_head=4104": "n_head", "n_head=1 << 62": "n_head", "ldq=4095": "ldq", "ldq_out=100": "ldq", "ldq_out=8192": "in place"}
     calls = ["dev.kv4_append_dev, cache4(), batch(), rows({})", "dev.kv_append_rope_dev, cache(), batch(), rows({})"]
     refused({**{c.format(b): w for b, w in bad.items() for c in calls},
              "dev.kv_append_rope_dev, cache(), batch(), rows(rope=0, q=0)": "rope",
@@ -159,3 +159,49 @@ except sa.SihipError as e:
     result = str(e)
 """)
         assert "error -8" in got, call
+
+
+@pytest.mark.parametrize("step,want", [
+    # (tokens, requests, longest, heads, KV heads, head_dim, most tokens of a request)
+    ((1, 1, 600, 32, 8, 128, 1), [["attnp4_groups_kernel<32,1,8,4,4,4>", 264, 1]]),
+    ((64, 64, 8192, 32, 8, 128, 1), [["attnp4_groups_kernel<32,1,8,4,4,4>", 1280, 1]]),
+    ((256, 256, 8192, 32, 8, 128, 1), [["attnp4_groups_kernel<32,1,8,4,1,4>", 4096, 1]]),
+    ((2, 1, 600, 8, 8, 128, 2), [["attnp4_groups_kernel<32,1,8,4,4,4>", 264, 1]]),
+    ((1, 1, 600, 14, 2, 64, 1), [["attnp4_groups_kernel<16,1,4,4,4,2>", 258, 1]]),
+    ((1, 1, 600, 2, 1, 192, 1), [["attnp4_groups_kernel<32,2,12,2,4,8>", 257, 1]]),
+    ((1, 1, 600, 2, 1, 256, 1), [["attnp4_groups_kernel<32,2,16,2,4,8>", 257, 1]]),
+    # more rows than columns for their groups
+    ((1, 1, 600, 16, 1, 64, 1), [["attnp4_rows_kernel<16,1,4,4,4>", 257, 1]]),
+    ((1, 1, 600, 5, 1, 128, 1), [["attnp4_rows_kernel<32,1,8,4,4>", 257, 1]]),
+    ((1, 1, 600, 3, 1, 256, 1), [["attnp4_rows_kernel<32,2,16,2,4>", 257, 1]]),
+    ((509, 1, 509, 14, 2, 64, 509), [["attnp4_rows_kernel<16,1,4,4,4>", 446, 1]]),
+    ((4096, 1, 4096, 32, 8, 256, 4096), [["attnp4_rows_kernel<32,2,16,2,1>", 9216, 1]]),
+    # large row blocks, the shorter requests beside them, splits of their keys
+    ((4096, 1, 4096, 32, 8, 128, 4096), [["attnp4_tiles_kernel<8,8>", 512, 1]]),
+    ((4096, 1, 4096, 32, 8, 96, 4096), [["attnp4_tiles_kernel<6,8>", 512, 1]]),
+    ((4096, 1, 4096, 32, 8, 64, 4096), [["attnp4_tiles_kernel<4,4>", 1024, 1]]),
+    ((1100, 65, 16000, 32, 8, 128, 1024), [["attnp4_tiles_kernel<8,8>", 656, 1], ["attnp4_rows_kernel<32,1,8,4,1>", 3104, 1]]),
+    ((256, 1, 64000, 32, 8, 128, 256), [["attnp4_tiles_kernel<8,8>", 32, 8], ["attnp_join_kernel<256>", 32, 32]]),
+])
+def test_kernels_of_attention(step, want):
+    n_tok, n_req, longest, heads, n_kv, hd, max_q = step
+    assert fake_hip.run(SETUP + f"""
+dev.attn_paged4_dev(cache4(n_head_kv={n_kv}, head_dim={hd}, block=64, n_pages=10000),
+                    batch(n_tok={n_tok}, n_req={n_req}, max_q={max_q}, max_kv={longest}, max_blocks=4096),
+                    attn(n_head={heads}, ldq={heads * hd}, ldo={heads * hd}))
+result = launched()
+""") == want
+
+
+@pytest.mark.parametrize("block,hd,want", [(16, 64, "1,128"), (16, 256, "1,256"), (64, 128, "1,512"), (64, 256, "1,1024"),
+                                           (256, 128, "2,1024"), (256, 256, "4,1024")])
+def test_kernels_of_rotated_appends(block, hd, want):
+    """Of the 8-bit cache by the page's units of 16 codes, a third layer of workgroups for queries."""
+    got = fake_hip.run(SETUP + f"""
+c = dict(n_head_kv=2, head_dim={hd}, block={block})
+r = dict(ldk={2 * hd}, ldv={2 * hd}, n_head=4, ldq={4 * hd}, ldq_out={4 * hd}, rope_dim={hd}, rope_len=20 * {block})
+dev.kv_append_rope_dev(cache(**c), batch(max_kv=20 * {block}), rows(**r))
+dev.kv4_append_dev(cache4(**c), batch(max_kv=20 * {block}), rows(**r))
+result = launched()
+""")
+    assert got == [[f"kv_append_kernel<{want},sihip::KeyRope>", 2, 4], ["kv4_append_kernel", 2, 4]]
