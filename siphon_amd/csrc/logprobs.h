@@ -8,13 +8,22 @@
 // its own; exponentials are f32 and added in f64: where one token has nearly all of the
 // probability, log l is what the others add to 1.
 //
-// The most likely: of a logit and its index a key is made, a 64-bit number that grows with the
+// The most likely: of a logit and its index a key is made, a 63-bit number that grows with the
 // logit and, of equal ones, falls with the index, so that no two are equal. The pass itself keeps the
-// largest of each thread's 16 logits at a time, no more. Every kLpRounds of them a wave finds the n_topth largest of
-// its lanes' largest (each lane has one that reaches it, so n_top keys do): what is below is not among the most
-// likely. The few runs of 16 that reach it are read again, four lanes a run, and the keys that reach it
-// go to a list in LDS. A list that is full is cut to its n_top largest, found by counting for each key how
-// many are larger, and the threshold goes up to the last of them.
+// largest of each thread's 16 logits at a time, no more. Every kLpRounds of them a wave ranks a few of
+// its lanes' largest; the n_topth of these is a threshold, as n_top keys reach it: what is below is not
+// among the most likely. The few runs of 16 that reach it are read again, four lanes a run (a single round's are
+// still in registers), and the keys that reach it go to a list in LDS. In the end, or when it is full, a
+// list is cut to its n_top largest, found by counting for each key how many are larger.
+//
+// A row of many logits is split over workgroups. A wave of each leaves its n_top largest in order, and the first
+// wave of the last workgroup to arrive takes from the lists' fronts what may be among the row's.
+//
+// Bound by memory where there are rows enough: 500 rows of 151936 (304 MB) 50 us (6.0 TB/s, a part of them from the
+// Infinity Cache), with the 20 most likely 67 (4.5); few rows by instructions in turn: one row of 151936 with 5
+// tokens takes 9.5 us, 3.5 of which an empty launch takes, 1 the pass, 2 the choices of the splits, 1.5 sums and
+// their way to the last workgroup, 1.5 its choice. (A choice of single keys as they came, with comparisons of integers:
+// 11.9, 64 rows of 32003 with 20 tokens 17 and not 13.8.)
 #pragma once
 
 #include <float.h>
@@ -35,18 +44,39 @@ struct LogprobArgs {
     int64_t n_token;
     int n_top, n_split;
     int64_t per_split;  // granules of 16 bytes of a split
-    uint8_t *part;      // [row][split]: maximum, sums, keys
+    uint8_t *part;      // of each row: [split] maximum and sums, [split][wave][n_top] keys
     uint32_t *cnt;      // of each row: splits that have arrived, zero between launches
 };
 
 constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
+constexpr int kLpMostSplits = 64;  // of a row, where tokens are chosen
 constexpr int kLpMostTop = 64;  // keys that a wave can choose with a lane each
-constexpr int kLpList = 192;
+constexpr int kLpList = 384;
 constexpr int kLpGroup = 4;     // 16-byte loads of a thread at a time
 constexpr int kLpRounds = 8;    // of them between choices
 
-// bytes of a split's part
-__host__ __device__ inline int64_t lp_part_bytes(int n_top) { return 32 + (int64_t)(n_top + 1) / 2 * 16; }
+// bytes of a row's part
+__host__ __device__ inline int64_t lp_part_bytes(int n_top, int n_split) { return (int64_t)n_split * (32 + kLpWaves * n_top * 8); }
+
+// x of another lane: 1 .. 32 lanes away, once all lanes between have the same
+template <int D>
+__device__ inline uint32_t lp_other(uint32_t x) {
+    if constexpr (D >= 16) {  // (one of the two is this lane's: the sum of both, less it)
+        const auto r = D == 16 ? __builtin_amdgcn_permlane16_swap(x, x, false, false) : __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return (uint32_t)r[0] ^ (uint32_t)r[1] ^ x;
+    } else {
+        constexpr int ctrl = D == 1 ? 0xb1 : D == 2 ? 0x4e : D == 4 ? 0x141 : 0x140;
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true);
+    }
+}
+template <int D>
+__device__ inline uint64_t lp_other(uint64_t x) {
+    return (uint64_t)lp_other<D>((uint32_t)(x >> 32)) << 32 | lp_other<D>((uint32_t)x);
+}
+template <int D>
+__device__ inline double lp_other(double x) { return __builtin_bit_cast(double, lp_other<D>(__builtin_bit_cast(uint64_t, x))); }
+template <int D>
+__device__ inline float lp_other(float x) { return __builtin_bit_cast(float, lp_other<D>(__builtin_bit_cast(uint32_t, x))); }
 
 struct LpSums {
     float m;
@@ -62,40 +92,69 @@ struct LpSums {
         l *= f;
         m = to;
     }
-    __device__ void add(LpSums o) {
-        const float to = fmaxf(m, o.m);
+    template <int D, int N>
+    __device__ void largest(float &to) const {
+        to = fmaxf(to, lp_other<D>(to));
+        if constexpr (2 * D < N) largest<2 * D, N>(to);
+    }
+    template <int D, int N>
+    __device__ void sum() {
+        l += lp_other<D>(l);
+        t += lp_other<D>(t);
+        if constexpr (2 * D < N) sum<2 * D, N>();
+    }
+    // of N lanes in a row, the same bits in each of them
+    template <int N>
+    __device__ void join() {
+        float to = m;
+        largest<1, N>(to);
         raise(to);
-        o.raise(to);
-        l += o.l;
-        t += o.t;
+        sum<1, N>();
     }
 };
 
-// NaN counts as -inf, -0 as 0
-__device__ inline uint64_t lp_key(float x, uint32_t index) {
+// a number that grows with x; NaN counts as -inf, -0 as 0
+__device__ inline uint32_t lp_order(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x == x ? x + 0.0f : -INFINITY);
-    return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xffffffffu - index);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+constexpr uint32_t kLpNone = 0x007fffffu;  // of -inf
+// (63 bits, of which the first 11 are never all set: as f64 numbers keys are finite and in the same order, and
+// those are compared faster)
+__device__ inline uint64_t lp_pair(uint32_t order, uint32_t index) { return (uint64_t)order << 31 | (0x7fffffffu - index); }
+__device__ inline bool lp_above(uint64_t a, uint64_t b) { return __builtin_bit_cast(double, a) > __builtin_bit_cast(double, b); }
+__device__ inline uint64_t lp_key(float x, uint32_t index) { return lp_pair(lp_order(x), index); }
 __device__ inline float lp_value(uint64_t key) {
-    const uint32_t b = (uint32_t)(key >> 32);
+    const uint32_t b = (uint32_t)(key >> 31);
     return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
-__device__ inline int32_t lp_index(uint64_t key) { return (int32_t)(0xffffffffu - (uint32_t)key); }
+__device__ inline int32_t lp_index(uint64_t key) { return 0x7fffffff - (int32_t)(key & 0x7fffffff); }
 
-// how many of n keys in LDS are larger (n is padded to even with zeros)
+typedef uint32_t lp_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t lp_u2 __attribute__((ext_vector_type(2)));
+
+// how many of n keys in LDS are larger (n is padded to a multiple of eight with zeros, by lp_pad)
 __device__ inline int lp_larger(const uint64_t *keys, int n, uint64_t key) {
     int k = 0;
-#pragma unroll 8
-    for (int i = 0; i < n; i += 2) {
-        const ulonglong2 o = *(const ulonglong2 *)(keys + i);
-        k += (o.x > key) + (o.y > key);
+#pragma unroll 1
+    for (int i = 0; i < n; i += 8) {
+        ulonglong2 o[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = *(const ulonglong2 *)(keys + i + 2 * e);
+#pragma unroll
+        for (int e = 0; e < 4; e++) k += lp_above(o[e].x, key) + lp_above(o[e].y, key);
     }
     return k;
 }
+__device__ inline void lp_pad(uint64_t *keys, int n) {
+    const int lane = threadIdx.x & 63;
+    if (lane < (-n & 7)) keys[n + lane] = 0;
+}
 
 // A wave's choice of the n_top largest of the keys it is shown.
+// it runs, so that there is one take of four keys a lane, not one of each key: 13 KB of code, not 67.)
 struct LpChoice {
-    uint64_t *list;  // of the wave, in LDS: kLpList and 64 more
+    uint64_t *list;  // of the wave, in LDS: kLpList keys and 128 more
     int n_top, count = 0;
     uint64_t least = 1;  // keys below it are not among the largest (0 is no key)
 
@@ -105,69 +164,99 @@ struct LpChoice {
     // cuts the list to its n_top largest, in order
     __device__ void cut() {
         const int lane = threadIdx.x & 63;
-        uint64_t own[kLpList / 64];
-        int rank[kLpList / 64];
-        if (lane == 0) list[count] = 0;
+        uint64_t *to = list + kLpList;
+        lp_pad(list, count);
         fence();
-#pragma unroll
-        for (int i = 0; i < kLpList / 64; i++) {
-            const int at = lane + 64 * i;
-            own[i] = at < count ? list[at] : 0;
-            rank[i] = own[i] ? lp_larger(list, count, own[i]) : n_top;
+#pragma unroll 1
+        for (int at = lane; at < count; at += 64) {
+            const uint64_t key = list[at];
+            const int rank = lp_larger(list, count, key);
+            if (rank < n_top) to[rank] = key;
         }
         fence();
-#pragma unroll
-        for (int i = 0; i < kLpList / 64; i++)
-            if (rank[i] < n_top) list[rank[i]] = own[i];
+        count = min(count, n_top);
+        if (lane < count) list[lane] = to[lane];
         fence();
-        if (count >= n_top) {
-            count = n_top;
-            const uint64_t last = list[n_top - 1];
-            least = last > least ? last : least;
-        }
+        if (count == n_top) least = max(least, list[n_top - 1]);
     }
-    // raises the threshold to the n_topth largest of a key of each lane, that is reached by one of its keys
-    __device__ void limit(uint64_t key) {
-        const int lane = threadIdx.x & 63;
-        if (__popcll(__ballot(key >= least)) < n_top) return;
+    // raises the threshold by two keys of each lane (or 0), each reached by one of its own: to the logit of the
+    // n_topth largest, or, if many reach that, as of equal logits, to that key. How many keys are ranked goes by
+    // how many are wanted: the 5th of 16 is reached by 6 keys on average (16 log 16 / 11), the 20th of 64 by
+    // 24, the 64th of 128 by 89 (of 64 by 300).
+    __device__ void limit(uint64_t a, uint64_t b) {
+        const int lane = threadIdx.x & 63, shift = n_top <= 8 ? 2 : 0;
+        const bool two = n_top > 32;
+        if (!two) a = max(a, b), b = 0;
+        if (shift) {
+            a = max(a, lp_other<1>(a));
+            a = max(a, lp_other<2>(a));
+        }
+        const bool first = !(lane & ((1 << shift) - 1));
+        if (__popcll(__ballot(first && a >= least)) + __popcll(__ballot(b >= least)) < n_top) return;
+        const int n = two ? 128 : 64 >> shift;
         uint64_t *all = list + kLpList;
-        all[lane] = key;
+        uint32_t *order = (uint32_t *)all;
+        const uint32_t a_high = (uint32_t)(a >> 32), b_high = (uint32_t)(b >> 32);
+        if (first) order[lane >> shift] = a_high;
+        if (two) order[64 + lane] = b_high;
         fence();
-        const int rank = lp_larger(all, 64, key);
-        const uint64_t last = __ballot(key && rank == n_top - 1);
-        if (last) {
-            const int from = __ffsll((unsigned long long)last) - 1;
-            const uint64_t k = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), from) << 32 |
-                               (uint32_t)__builtin_amdgcn_readlane((int)key, from);
-            least = k > least ? k : least;
+        int over_a = 0, over_b = two ? 0 : n_top;  // how many are larger
+#pragma unroll 4
+        for (int i = 0; i < n; i += 4) {
+            const lp_u4 o = *(const lp_u4 *)(order + i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) over_a += o[e] > a_high;
+            if (two)
+#pragma unroll
+                for (int e = 0; e < 4; e++) over_b += o[e] > b_high;
         }
         fence();
+        const bool many = __popcll(__ballot(first && over_a < n_top)) + __popcll(__ballot(over_b < n_top)) > n_top + 8;
+        if (many) {
+            if (first) all[lane >> shift] = a;
+            if (two) all[64 + lane] = b;
+            fence();
+            over_a = lp_larger(all, n, a);
+            if (two) over_b = lp_larger(all, n, b);
+            fence();
+        }
+        int rank = n_top - 1;
+        uint64_t in_a, in_b;
+        while (in_a = __ballot(over_a == rank), in_b = __ballot(over_b == rank), !(in_a | in_b) && rank > 0) rank--;
+        const int from = __ffsll((unsigned long long)(in_a ? in_a : in_b)) - 1;
+        const uint64_t key = in_a ? a : b;
+        const uint64_t k = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), from) << 32 |
+                           (many ? (uint32_t)__builtin_amdgcn_readlane((int)key, from) : 0u);
+        least = k > least ? k : least;
     }
-    // a key a lane, 0 for none
-    __device__ void take(uint64_t key) {
-        uint64_t takes = __ballot(key >= least);
-        if (!takes) return;
-        if (count + __popcll(takes) > kLpList - 1) {
-            cut();
-            takes = __ballot(key >= least);
-        }
-        if (key >= least) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(takes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)takes, 0))] = key;
-        count += __popcll(takes);
+    // a key a lane, where it reaches the threshold
+    __device__ void add(uint64_t key) {
+        const uint64_t here = __ballot(key >= least);
+        if (key >= least) list[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(here >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)here, 0))] = key;
+        count += __popcll(here);
+    }
+    // four keys a lane, 0 for none; whether any was taken
+    __device__ bool take(const uint64_t (&key)[4]) {
+        static_assert(kLpMostTop + 256 <= kLpList && kLpList % 8 == 0, "");
+        int more = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) more += __popcll(__ballot(key[e] >= least));
+        if (!more) return false;
+        if (count + more > kLpList) cut();
+#pragma unroll
+        for (int e = 0; e < 4; e++) add(key[e]);
         fence();
+        return true;
     }
 };
-
-typedef uint32_t lp_u4 __attribute__((ext_vector_type(4)));
-typedef uint32_t lp_u2 __attribute__((ext_vector_type(2)));
 
 // One workgroup: a split of a row, per_split granules of 16 bytes (the first and the last of a row
 // may be parts: rows begin at any f32). The last of a row's workgroups to arrive joins the
 // splits in their order.
 template <bool TOP>
 __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs A) {
-    __shared__ __attribute__((aligned(16))) uint64_t lists[TOP ? kLpWaves : 1][TOP ? kLpList + 64 : 1];
-    __shared__ float largest[TOP ? kLpWaves : 1][TOP ? kLpRounds : 1][64];  // of a thread's 16 logits; then runs to read again
-    __shared__ uint64_t chosen[kLpMostTop];
+    __shared__ __attribute__((aligned(16))) uint64_t lists[TOP ? kLpWaves : 1][TOP ? kLpList + 128 : 1];
+    __shared__ uint32_t largest[TOP ? kLpWaves : 1][TOP ? kLpRounds : 1][64];  // of a thread's 16 logits; then runs to read again
     __shared__ int counts[kLpWaves];
     __shared__ LpSums sums[kLpWaves];
     __shared__ uint32_t last;
@@ -212,35 +301,48 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs A) {
                 t = fmaf(p, fmaxf(d, -1e4f), t);  // (where p is zero d may be infinite)
             }
             S.t += (double)t;
-            if constexpr (TOP) largest[wave][r][lane] = most;
+            if constexpr (TOP) largest[wave][r][lane] = lp_order(most);
         }
         if constexpr (!TOP) continue;
-        if (rounds == 1) {  // they are still here
-            uint64_t key[4 * kLpGroup], low = 0;
-#pragma unroll
-            for (int e = 0; e < 4 * kLpGroup; e++) {
-                key[e] = key_at(v[e], first + e / 4 * kStep + 4 * tid + e % 4);
-                low = key[e] > low ? key[e] : low;
-            }
-            C.limit(low);
-#pragma unroll
-            for (int e = 0; e < 4 * kLpGroup; e++) C.take(key[e]);
-            continue;
-        }
         // runs of 16, by the bounds of their largest key: its place is between the run's first and last
+        // (where it is -inf all are, and the first has the largest key)
         LpChoice::fence();
         const uint32_t mine = first + 4 * tid;
-        uint64_t low = 0;
-        for (int r = 0; r < rounds; r++) {
-            const uint32_t p = mine + r * kRound;
-            const uint64_t k = p < p1 ? lp_key(largest[wave][r][lane], p + 3 * kStep + 3) : 0;
-            low = k > low ? k : low;
+        uint64_t low[2] = {0, 0};
+        auto bound = [&](uint32_t o, uint32_t p, uint32_t to) { return p >= p1 ? 0 : lp_pair(o, o > kLpNone ? p + to : p > skew ? p - skew : 0); };
+        if (rounds == 1) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                float most = v[8 * k];
+#pragma unroll
+                for (int e = 1; e < 8; e++) most = fmaxf(most, v[8 * k + e]);
+                low[k] = bound(lp_order(most), mine + 2 * k * kStep, kStep + 3);
+            }
+        } else {
+            for (int r = 0; r < rounds; r++) {
+                const uint64_t k = bound(largest[wave][r][lane], mine + r * kRound, 3 * kStep + 3);
+                if (r & 1) low[1] = max(low[1], k);
+                else low[0] = max(low[0], k);
+            }
         }
-        C.limit(low);
+        C.limit(low[0], low[1]);
+        if (rounds == 1 && (uint32_t)(C.least >> 31) > kLpNone) {  // they are still here
+            const float border = lp_value(C.least);
+            int more = 0;
+#pragma unroll
+            for (int e = 0; e < 4 * kLpGroup; e++) more += __popcll(__ballot(v[e] >= border));
+            if (C.count + more <= kLpList) {
+#pragma unroll
+                for (int e = 0; e < 4 * kLpGroup; e++)
+                    if (__any(v[e] >= border)) C.add(v[e] >= border ? lp_key(v[e], mine + e / 4 * kStep + e % 4 - skew) : 0);
+                LpChoice::fence();
+                continue;
+            }
+        }
         uint32_t reach = 0;
         for (int r = 0; r < rounds; r++) {
             const uint32_t p = mine + r * kRound;
-            if (p < p1 && lp_key(largest[wave][r][lane], p > skew ? p - skew : 0) >= C.least) reach |= 1u << r;
+            if (p < p1 && lp_pair(largest[wave][r][lane], p > skew ? p - skew : 0) >= C.least) reach |= 1u << r;
         }
         LpChoice::fence();
         uint16_t *runs = (uint16_t *)largest[wave];
@@ -256,58 +358,34 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs A) {
             const uint32_t p = j < n ? first + (run >> 6) * kRound + (lane & 3) * kStep + 4 * (wave * 64 + (run & 63)) : p1;
             float v[4];
             load4(p, v);
-#pragma unroll
-            for (int e = 0; e < 4; e++) C.take(key_at(v[e], p + e));
+            const uint64_t key[4] = {key_at(v[0], p), key_at(v[1], p + 1), key_at(v[2], p + 2), key_at(v[3], p + 3)};
+            C.take(key);
         }
         LpChoice::fence();
     }
-    // the workgroup's sums and choice
-    auto join = [&]() {
-        for (int d = 1; d < 64; d <<= 1) {
-            LpSums o;
-            o.m = __shfl_xor(S.m, d);
-            o.l = __shfl_xor(S.l, d);
-            o.t = __shfl_xor(S.t, d);
-            S.add(o);
-        }
-        if (lane == 0) sums[wave] = S;
-        if constexpr (TOP) {
-            if (C.count > 64) C.cut();
-            if (lane == 0) {
-                counts[wave] = C.count;
-                C.list[C.count] = 0;
-            }
-            if (tid < A.n_top) chosen[tid] = 0;
-        }
-        __syncthreads();
-        S = sums[0];
-#pragma unroll
-        for (int w = 1; w < kLpWaves; w++) S.add(sums[w]);
-        if constexpr (TOP) {
-            if (lane < C.count) {
-                const uint64_t key = C.list[lane];
-                int rank = 0;
-#pragma unroll
-                for (int w = 0; w < kLpWaves; w++) rank += lp_larger(lists[w], counts[w], key);
-                if (rank < A.n_top) chosen[rank] = key;
-            }
-        }
-        __syncthreads();
-    };
-    join();
+    // the wave's sums and choice; of several splits, those of all of them
+    if constexpr (TOP)
+        if (A.n_split > 1 || C.count > A.n_top) C.cut();
     if (A.n_split > 1) {
-        const int64_t bytes = lp_part_bytes(A.n_top);
-        const __amdgpu_buffer_rsrc_t part = __builtin_amdgcn_make_buffer_rsrc(A.part + row * A.n_split * bytes, (short)0,
-                                                                              (int)(A.n_split * bytes), 0x00020000);
-        const uint32_t to = split * (uint32_t)bytes;
+        const int64_t bytes = lp_part_bytes(A.n_top, A.n_split);
+        const __amdgpu_buffer_rsrc_t part = __builtin_amdgcn_make_buffer_rsrc(A.part + row * bytes, (short)0, (int)bytes, 0x00020000);
+        if constexpr (TOP)
+            if (lane < A.n_top) {
+                const uint64_t key = lane < C.count ? C.list[lane] : 0;
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(lp_u2, key), part,
+                                                      A.n_split * 32 + ((split * kLpWaves + wave) * A.n_top + lane) * 8, 0, 16);
+            }
+        S.join<64>();
+        if (lane == 0) sums[wave] = S;
+        __syncthreads();
+        S = sums[lane & (kLpWaves - 1)];
+        S.join<kLpWaves>();
         if (tid == 0) {
             const double two[2] = {S.l, S.t};
             const lp_u4 first = {__builtin_bit_cast(uint32_t, S.m), 0, 0, 0};
-            __builtin_amdgcn_raw_buffer_store_b128(first, part, (int)to, 0, 16);
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(lp_u4, two), part, (int)to + 16, 0, 16);
+            __builtin_amdgcn_raw_buffer_store_b128(first, part, split * 32, 0, 16);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(lp_u4, two), part, split * 32 + 16, 0, 16);
         }
-        if constexpr (TOP)
-            if (tid < A.n_top) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(lp_u2, chosen[tid]), part, (int)to + 32 + 8 * tid, 0, 16);
         // (the order that agent.h describes)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -316,42 +394,56 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs A) {
         __syncthreads();
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         if (!last) return;
+        if (tid == 0) __hip_atomic_store(A.cnt + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         S = LpSums::none();
-        C.count = 0;
-        C.least = 1;
-        for (int k = tid; k < A.n_split; k += kLpThreads) {
-            LpSums o;
-            const lp_u4 a = __builtin_amdgcn_raw_buffer_load_b128(part, (int)(k * bytes), 0, 16);
-            const lp_u4 b = __builtin_amdgcn_raw_buffer_load_b128(part, (int)(k * bytes) + 16, 0, 16);
-            o.m = __builtin_bit_cast(float, a.x);
-            o.l = __builtin_bit_cast(double, (uint64_t)b.y << 32 | b.x);
-            o.t = __builtin_bit_cast(double, (uint64_t)b.w << 32 | b.z);
-            S.add(o);
+        if (tid < A.n_split) {  // (at most kLpThreads)
+            const lp_u4 a = __builtin_amdgcn_raw_buffer_load_b128(part, tid * 32, 0, 16);
+            const lp_u4 b = __builtin_amdgcn_raw_buffer_load_b128(part, tid * 32 + 16, 0, 16);
+            S.m = __builtin_bit_cast(float, a.x);
+            S.l = __builtin_bit_cast(double, (uint64_t)b.y << 32 | b.x);
+            S.t = __builtin_bit_cast(double, (uint64_t)b.w << 32 | b.z);
         }
         if constexpr (TOP) {
-            for (int k0 = 0; k0 < A.n_split * A.n_top; k0 += 4 * kLpThreads) {
+            C.count = 0;
+            C.least = 1;
+            // Lists in order: a list a lane, two or four, or, of few, a list to `lanes` lanes, four keys a lane
+            // at a time from the lists' largest on, until none is among the largest.
+            const int n = A.n_split * kLpWaves, ranks = n <= 64 ? 4 : n <= 128 ? 2 : 1;
+            static_assert(kLpMostSplits * kLpWaves <= 256, "");
+            int lanes = 1;
+            while (2 * lanes * n <= 64) lanes *= 2;
+            for (int r = lane % lanes; wave == 0; r += ranks * lanes) {
                 uint64_t key[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int i = k0 + e * kLpThreads + tid;
+                    const int list = lane / lanes + e / ranks * 64, rank = r + e % ranks * lanes;
                     key[e] = 0;
-                    if (i < A.n_split * A.n_top) {
-                        const lp_u2 w = __builtin_amdgcn_raw_buffer_load_b64(part, (int)(i / A.n_top * bytes + 32 + i % A.n_top * 8), 0, 16);
-                        key[e] = (uint64_t)w.y << 32 | w.x;
-                    }
+                    if (list < n && rank < A.n_top)
+                        key[e] = __builtin_bit_cast(uint64_t, __builtin_amdgcn_raw_buffer_load_b64(part, A.n_split * 32 + (list * A.n_top + rank) * 8, 0, 16));
                 }
-                uint64_t low = key[0];
-#pragma unroll
-                for (int e = 1; e < 4; e++) low = key[e] > low ? key[e] : low;
-                C.limit(low);
-#pragma unroll
-                for (int e = 0; e < 4; e++) C.take(key[e]);
+                if (r < lanes) C.limit(max(key[0], key[2]), max(key[1], key[3]));
+                if (!C.take(key)) break;
             }
         }
+    } else if constexpr (TOP) {
+        if (lane == 0) counts[wave] = C.count;
         __syncthreads();
-        join();
-        if (tid == 0) __hip_atomic_store(A.cnt + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (wave == 0) {
+            uint64_t key[4];
+#pragma unroll
+            for (int w = 0; w < kLpWaves; w++) key[w] = lane < counts[w] ? lists[w][lane] : 0;
+            C.count = 0;
+            LpChoice::fence();
+            C.limit(max(key[0], key[1]), max(key[2], key[3]));
+            C.take(key);
+        }
     }
+    S.join<64>();
+    __syncthreads();
+    if (lane == 0) sums[wave] = S;
+    __syncthreads();
+    S = sums[lane & (kLpWaves - 1)];
+    S.join<kLpWaves>();
     // S.l is zero where no logit is above -inf: then there is no token to choose
     const bool none = S.l == 0.0;
     const double log_l = none ? 0.0 : log(S.l);
@@ -363,10 +455,13 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs A) {
         }
     if (A.entropy && tid == 0) A.entropy[row] = none ? 0.0f : (float)(log_l - S.t / S.l);
     if constexpr (TOP)
-        if (tid < A.n_top) {
-            const uint64_t key = chosen[tid];
-            A.top_id[row * A.n_top + tid] = lp_index(key);
-            A.top_logprob[row * A.n_top + tid] = logprob(lp_value(key));
+        if (wave == 0) {
+            C.cut();
+            if (lane < A.n_top) {
+                const uint64_t key = C.list[lane];
+                A.top_id[row * A.n_top + lane] = lp_index(key);
+                A.top_logprob[row * A.n_top + lane] = logprob(lp_value(key));
+            }
         }
 }
 

@@ -9,11 +9,11 @@ using namespace sihip;
 
 namespace {
 
-// Checks, and the splits of a row: until the device has two workgroups a CU, or one where no
-// tokens are chosen, and none shorter than one round of loads. Each split ends with reductions and
-// a choice, in turn, that no loads cover. us with 1 / 2 / 4 / 8 a CU: 500 rows of 151936, 20 tokens
-// 77 / 73 / 86 / 87, none 51 / 52 / 56 / 60; 64 of 151936, 20 tokens 25 / 21 / 26 / 43; 64 of 32003, 20 tokens
-// 15 / 17 / 17 / 17, most of them masked 23 / 18 / 18 / 18, none 8 / 9 / 9 / 9.
+// Checks, and the splits of a row: until the device has two workgroups a CU, and none shorter than one round of
+// loads. Each split ends with reductions and a choice, in turn, that no loads cover. us with 1 / 2 / 4 /
+// 8 a CU: 500 rows of 151936, no tokens chosen 53 / 50 / 53 / 54, 20 tokens 80 / 67 / 82 / 73; 64 of 151936 14 / 12 / 14 / 22 and
+// 23 / 19 / 22 / 35; 200 of 151936 24 / 24 / 26 / 27 and 40 / 36 / 36 / 44; 64 of 32003, which have 8 splits at
+// most, 7.3 / 7.9 / 7.8 / 7.6 and 13.1 / 13.8 / 13.8 / 13.9.
 int plan_logprobs(sihip_ctx *ctx, const sihip_logprobs *a, LogprobArgs &A, size_t &part_bytes) {
     const char *fn = "logprobs_dev";
     if (!ctx || !a) return set_err(ctx, SIHIP_EINVAL, "%s: NULL argument", fn);
@@ -43,11 +43,11 @@ int plan_logprobs(sihip_ctx *ctx, const sihip_logprobs *a, LogprobArgs &A, size_
     A.top_id = a->top_id;
     A.top_logprob = a->top_logprob;
     const int64_t granules = (A.n + 6) / 4, round = kLpThreads * kLpGroup;  // (a row may begin inside one)
-    const int64_t want = ((A.n_top ? 2 : 1) * ctx->n_cu + a->n_rows - 1) / a->n_rows, most = (granules + round - 1) / round;
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>({want, most, 256}));
-    A.per_split = ((granules + n - 1) / n + kLpThreads - 1) / kLpThreads * kLpThreads;
+    const int64_t want = (2 * ctx->n_cu + a->n_rows - 1) / a->n_rows, most = (granules + round - 1) / round;
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>({want, most, A.n_top ? kLpMostSplits : kLpThreads}));
+    A.per_split = ((granules + n - 1) / n + 3) / 4 * 4;  // (whole 64 bytes, of splits of one length)
     A.n_split = (int)((granules + A.per_split - 1) / A.per_split);
-    if (A.n_split > 1) part_bytes = (size_t)a->n_rows * A.n_split * lp_part_bytes(A.n_top);
+    if (A.n_split > 1) part_bytes = (size_t)a->n_rows * lp_part_bytes(A.n_top, A.n_split);
     return SIHIP_OK;
 }
 

@@ -94,7 +94,7 @@ def tokens(rng, rows, n, given=2):
 
 
 @pytest.mark.parametrize("rows,n", [(1, 1), (1, 2), (3, 5), (2, 63), (5, 64), (1, 4096), (2, 4097), (7, 1000), (1, 32003), (64, 2049),
-                                    (1, 151936), (2, 262147), (300, 4099), (2100, 517)])
+                                    (1, 100003), (1, 151936), (2, 262147), (40, 5000), (300, 4099), (2100, 517)])
 @pytest.mark.parametrize("n_top", [0, 1, 5, 20, 64])
 def test_rows(dev, rows, n, n_top):
     rng = np.random.default_rng(rows + n)

@@ -144,7 +144,7 @@ for rows_, n in ((1, 1), (1, 4000), (1, 151936), (64, 32003), (500, 151936), (20
 dev.logprobs_dev(lp(n_top=0))
 result = launched()
 """)
-    assert [g[:2] for g in got] == [["logprobs_kernel<true>", g] for g in (1, 1, 38, 512, 1000, 2048, 256)] + [["logprobs_kernel<false>", 6]]
+    assert [g[:2] for g in got] == [["logprobs_kernel<true>", g] for g in (1, 1, 38, 512, 1000, 2048, 64)] + [["logprobs_kernel<false>", 6]]
 
 
 def test_a_failed_launch_is_reported():
