@@ -79,6 +79,11 @@ __device__ inline float ap4_bf16(uint32_t x, int high) { return __builtin_bit_ca
 // NK slices of 4 KD: 16 bytes, or 8 for heads up to 64. Row m of key tile t is token TT m + t, so
 // that a lane's TT subs are neighbours, and its scores, of tokens 4 TT g .., are
 // i-major: token TT i + t of them is register (t, i).
+//
+// Bound by its vector instructions: codes to f16, twice a byte of the cache, and subs for the pairs of a
+// word. 16 requests of 4 tokens over up to 8192 keys (32 heads of 128 on 8) 35 us, where its 55 MB would take 12; 4096 rows of 16 heads of
+// 256, for which there is no large block, 770 (its doubled products 222); a prompt of 509 tokens, 14 heads of 64 on 2, 11.6, of
+// which an empty launch takes 3.5 and two chunks a wave, in turn, most of the rest.
 template <int KD, int NK, int ND, int TT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A) {
     constexpr int CH = 16 * TT, SEG = 4 * TT, KW = KD / 8, VW = SEG / 8;
@@ -341,6 +346,12 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
 // sums of values likewise: weights times subs are a column's operand, and of its sums the dims of its
 // group are used. No code is multiplied by a sub: the subs of a token and its group are two numbers of a
 // lane where the other kernel has eight, and their products with codes.
+//
+// Bound by memory and vector instructions at once: of a chunk's 660 instructions 290 make codes f16, the others are
+// scores, weights and splits, of which NG columns have the same (vector pipes busy for two thirds of the time,
+// matrix ones a fifth). 64 single tokens over up to 8192 keys, 32 heads of 128 on 8, 66-72 us (224 MB, 3.1-3.4 TB/s), 94 by
+// the kernel above; one over 131072 42 (147 MB, 3.5 TB/s) and 63; 16 over up to 16000, 16 heads of 256 on 8, 78. Which of both runs
+// is a matter of the columns: more rows do not fit.
 // Codes alone, in units of 2^-10: of a nibble n 2^-24 or n 2^-20 (ap4_cvt) one packed FMA with
 // constants.
 constexpr float kAp4Code = 0x1p10f;
@@ -621,15 +632,25 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
 
 // ---- many rows ---------------------------------------------------------------------
 //
-// attnp_tiles_kernel (attnp.h) over 4-bit values: the codes of a 64-key chunk become f16 numbers
-// once, code * sub, on their way into LDS; the scales of its keys and values lie there beside
-// them, as f32. A unit of 16 values is 8 bytes here.
 // x of another lane of the row of 16
 template <int CTRL>
 __device__ inline float ap4_from(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
 
+// attnp_tiles_kernel (attnp.h) over 4-bit values: the codes of a 64-key chunk become f16 numbers
+// once, code * sub, on their way into LDS; the scales of its keys and values lie there beside
+// them, as f32. A unit of 16 values is 8 bytes here.
+//
+// A wave has 32 rows. The scores of half a chunk are computed beside the weights of the half before, the products with
+// values follow; two barriers a chunk. The queries' lower halves are read from LDS for each half: in
+// registers they would leave none for the next scores.
+//
+// Bound by the vector step: its pipes are busy for half of the time and the matrix ones for a third, and a wave
+// overlaps little of its own (two waves a SIMD are all that the registers allow). 3 prompts of up to 4096 tokens behind up to 1000, 40
+// heads of 128 on 8, slopes and prefixes, 800 us: 366 TFLOP/s, twice that with the second halves, against the
+// 1177 of a large f16 product; 4096 rows of 32 heads of 128 319, of 64 222. Four waves a block for heads up to 64
+// (with eight 252), eight for wider ones (with four, of whose blocks LDS holds one, 497).
 constexpr int ap4_tile_waves(int hd) { return hd <= 64 ? 4 : 8; }
 
 template <int NS, int WAVES = ap4_tile_waves(16 * NS)>

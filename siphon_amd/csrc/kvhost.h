@@ -145,6 +145,11 @@ constexpr int kApFewRows = 64;
 //   14 heads of 64 on 2: 1200 27 / 33, 4096 133 / 124; 32 on 8: 4096 239 / 171
 //   wider than 128 the large blocks' sums would leave one wave a SIMD: 16 heads of
 //     256, 4096 rows 467, 627 in a build that had them
+// and over 4 bits:
+//   32 heads of 128: 1500 rows 102 / 111, 1800 136 / 132, 2048 158 / 144, 3000 298 / 202; 190 behind 8000 keys 120 /
+//     125, 256 behind 8000 123 / 96, 64 behind 30000 133 / 87; window of 512, 2048 rows 81 / 66; 200 prompts of up to
+//     256 312 / 385, 50 of up to 512 192 / 217, 8 of up to 1024 106 / 91; heads of 96: 1300 84 / 79, 2048 156 / 128
+//   heads of 64: 32 on 8: 2048 105 / 107, 3000 199 / 159
 int attn_waves(const sihip_ctx *ctx, const AttnPArgs &A, int waves, int64_t rows, int64_t all_rows) {
     if (A.C.hd > 128) return 0;
     if (ctx->opt.attnp_large >= 0) return ctx->opt.attnp_large ? waves : 0;
