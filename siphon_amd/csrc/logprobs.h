@@ -309,7 +309,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobArgs A) {
         LpChoice::fence();
         const uint32_t mine = first + 4 * tid;
         uint64_t low[2] = {0, 0};
-        auto bound = [&](uint32_t o, uint32_t p, uint32_t to) { return p >= p1 ? 0 : lp_pair(o, o > kLpNone ? p + to : p > skew ? p - skew : 0); };
+        auto bound = [&](uint32_t o, uint32_t p, uint32_t to) { return p >= p1 ? 0 : lp_pair(o, o > kLpNone ? min(p + to, 0x7fffffffu) : p > skew ? p - skew : 0); };
         if (rounds == 1) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {

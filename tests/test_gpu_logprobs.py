@@ -195,6 +195,43 @@ def test_rows_past_32_bits(dev):
         big.free()
 
 
+@pytest.mark.parametrize("n_top", [0, 5, 64])
+def test_the_longest_row(dev, n_top):
+    """2^31 - 1 logits, of which the last few are not all alike."""
+    rng = np.random.default_rng(9)
+    n, piece, far = 2 ** 31 - 1, 1 << 26, 3000
+    fill, tail = np.full(piece, -5, np.float32), logits(rng, 1, far)
+    tail[0, -1] = tail.max() + 1
+    big = dev.alloc(4 * n)
+    try:
+        for at in range(0, n, piece):
+            dev._check(dev.L.sihip_memcpy_htod(dev.ctx, big.ptr + 4 * at, fill.ctypes.data, 4 * min(piece, n - at)))
+        dev._check(dev.L.sihip_memcpy_htod(dev.ctx, big.ptr + 4 * (n - far), tail.ctypes.data, tail.nbytes))
+        token = np.array([[0, n - 1, n - far, -1]])
+        with ko.OnDevice(dev, **buffers(tail, token, n_top)) as d:
+            dev.logprobs_dev(arguments(d, tail, token, n_top, logits=big.ptr, ld=n, n_vocab=n))
+            dev.synchronize()
+            y = tail[0].astype(np.float64)
+            m, e = y.max(), np.exp(y - y.max())
+            rest = (n - far) * np.exp(-5 - m)
+            l = rest + e.sum()
+            spread = ((m - y) * e).sum() / l + rest / l * (m + 5)
+            lp = lambda x: x - m - np.log(l)
+            # a thread's maximum may be raised at each of its runs of the tail
+            bound = (2.0 ** -22 + 3 * spread * 2.0 ** -24) * 66
+            got = d.get("lp")[0]
+            assert got[3] == 55
+            for g, x in zip(got, (-5.0, y[-1], y[0])):
+                assert abs(g - lp(x)) <= bound + 2.0 ** -24 * abs(lp(x))
+            assert abs(d.get("h")[0] - (np.log(l) + spread)) <= bound * (2 + spread) + 2.0 ** -20 * spread
+            if n_top:
+                order = np.argsort(-y, kind="stable")[:n_top]
+                assert np.array_equal(d.get("ti")[0], n - far + order)
+                assert (np.abs(d.get("tl")[0] - lp(y[order])) <= bound + 2.0 ** -24 * np.abs(lp(y[order]))).all()
+    finally:
+        big.free()
+
+
 def test_streams_workspaces_and_graphs(dev):
     """Two calls at once with workspaces of their own; captured ones replayed with other
     logits and eager calls between."""
