@@ -72,6 +72,11 @@ __device__ inline void ap4_subs(uint32_t x, uint32_t y, Ap4Sub (&s)[4]) {
 // a bfloat16 in the low or high half of x
 __device__ inline float ap4_bf16(uint32_t x, int high) { return __builtin_bit_cast(float, high ? x & 0xffff0000u : x << 16); }
 
+// Chunk u of u0 .. u1 - 1, the nearest first. With slopes scores rise towards a row's own position, and in
+// the other order nearly every chunk would move the maximum and the sums with it: 3 prompts of up to 4096, 40 heads, 810
+// us and 680 this way; 64 single tokens over up to 8192 73 and 68. Without them both orders take the same.
+__device__ inline int ap4_chunk(const Sight &S, int u0, int u1, int u) { return ap_chunk(S, u0 + u1 - 1 - u); }
+
 // ---- few rows ----------------------------------------------------------------------
 //
 // attnp_rows_kernel (attnp.h) over 4-bit values: 16 rows of one request and KV head, one split of
@@ -88,7 +93,7 @@ template <int KD, int NK, int ND, int TT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A) {
     constexpr int CH = 16 * TT, SEG = 4 * TT, KW = KD / 8, VW = SEG / 8;
     constexpr uint32_t kAll = (1u << SEG) - 1;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
     int r, h, tile, split, per;
     int64_t piece;
@@ -101,13 +106,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
     const Sight S = ap_sight(A, r, s, t0, t1);
     const int n_split = ap_splits(A, S.n, per);
     if (split >= n_split) return;
-    const int u0 = (int)((int64_t)S.n * split / n_split), u1 = (int)((int64_t)S.n * (split + 1) / n_split);
+    const int u0 = __builtin_amdgcn_readfirstlane((int)((int64_t)S.n * split / n_split));
+    const int u1 = __builtin_amdgcn_readfirstlane((int)((int64_t)S.n * (split + 1) / n_split));
+    auto chunk_of = [&](int u) { return ap4_chunk(S, u0, u1, u); };
 
     // table entries of this lane's key rows, and of its values and scores: loaded a chunk ahead,
     // between its keys and its values, and looked at when they are used (a wait for a load is one for
     // all loads before it)
     const int last_block = max(S.keys - 1, 0) >> shift, n_pages = (int)A.C.n_pages;
-    auto first_of = [&](int u, int seg) { return ap_chunk(S, u) * CH + seg * SEG; };
+    auto first_of = [&](int u, int seg) { return chunk_of(u) * CH + seg * SEG; };
     auto entry_of = [&](int u, int seg) { return table[min(first_of(u, seg) >> shift, last_block)]; };
     auto page_of = [&](int u, int seg, int entry) { return first_of(u, seg) < S.keys && entry >= 0 && entry < n_pages ? entry : -1; };
     int u = u0 + wave, ek = 0, ev = 0, pv = 0;
@@ -138,7 +145,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
     uint32_t kr[TT][NK][KW], vr[ND][VW];
     uint32_t ksub[NK], vsub[ND / 2][SEG / 4], kd[SEG / 2], vd[SEG / 2];
     auto load_keys = [&](int u) {
-        const int at = ap_chunk(S, u) * CH & (B - 1), pk = page_of(u, col >> 2, ek);
+        const int at = chunk_of(u) * CH & (B - 1), pk = page_of(u, col >> 2, ek);
         pv = page_of(u, g, ev);
         const int64_t ph = (int64_t)max(pk, 0) * A.C.n_kv + h, ps = (int64_t)max(pv, 0) * A.C.n_kv + h;
         const uint8_t *kp = kb + (ph * head_bytes + at * row_bytes);
@@ -168,7 +175,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
         }
     };
     auto load_values = [&](int u) {
-        const int at = ap_chunk(S, u) * CH & (B - 1);
+        const int at = chunk_of(u) * CH & (B - 1);
         const int64_t ph = (int64_t)max(pv, 0) * A.C.n_kv + h;
         const uint8_t *vp = vb + (ph * head_bytes + at / 2);
         const int8_t *sp = A.vsub + ((ph * groups) << shift) + at + vt;
@@ -239,7 +246,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = ap_f4{0, 0, 0, 0};
     for (; u < u1; u += WAVES) {
-        const int next = min(u + WAVES, u1 - 1), c = ap_chunk(S, u);
+        const int next = min(u + WAVES, u1 - 1), c = chunk_of(u);
         ap_f4 sc[TT];
 #pragma unroll
         for (int t = 0; t < TT; t++) sc[t] = ap_f4{0, 0, 0, 0};
@@ -390,7 +397,7 @@ template <int KD, int NK, int ND, int TT, int WAVES, int NG>
 __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args A) {
     constexpr int CH = 16 * TT, SEG = 4 * TT, KW = KD / 8, VW = SEG / 8, RB = 16 / NG;
     constexpr uint32_t kAll = (1u << SEG) - 1;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, group = col / RB;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, group = col / RB;
     const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
     int r, h, tile, split, per;
     int64_t piece;
@@ -402,13 +409,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
     const Sight S = ap_sight(A, r, s, 0, n_tok - 1);
     const int n_split = ap_splits(A, S.n, per);
     if (split >= n_split) return;
-    const int u0 = (int)((int64_t)S.n * split / n_split), u1 = (int)((int64_t)S.n * (split + 1) / n_split);
+    const int u0 = __builtin_amdgcn_readfirstlane((int)((int64_t)S.n * split / n_split));
+    const int u1 = __builtin_amdgcn_readfirstlane((int)((int64_t)S.n * (split + 1) / n_split));
+    auto chunk_of = [&](int u) { return ap4_chunk(S, u0, u1, u); };
 
     // table entries of this lane's key rows, and of its values and scores: loaded a chunk ahead,
     // between its keys and its values, and looked at when they are used (a wait for a load is one for
     // all loads before it)
     const int last_block = max(S.keys - 1, 0) >> shift, n_pages = (int)A.C.n_pages;
-    auto first_of = [&](int u, int seg) { return ap_chunk(S, u) * CH + seg * SEG; };
+    auto first_of = [&](int u, int seg) { return chunk_of(u) * CH + seg * SEG; };
     auto entry_of = [&](int u, int seg) { return table[min(first_of(u, seg) >> shift, last_block)]; };
     auto page_of = [&](int u, int seg, int entry) { return first_of(u, seg) < S.keys && entry >= 0 && entry < n_pages ? entry : -1; };
     int u = u0 + wave, ek = 0, ev = 0, pv = 0;
@@ -450,7 +459,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
         }
     };
     auto load_keys = [&](int u) {
-        const int at = ap_chunk(S, u) * CH & (B - 1), pk = page_of(u, col >> 2, ek);
+        const int at = chunk_of(u) * CH & (B - 1), pk = page_of(u, col >> 2, ek);
         pv = page_of(u, g, ev);
         const int64_t ph = (int64_t)max(pk, 0) * A.C.n_kv + h, ps = (int64_t)max(pv, 0) * A.C.n_kv + h;
         const uint8_t *kp = kb + (ph * head_bytes + at * row_bytes);
@@ -478,7 +487,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
         }
     };
     auto load_values = [&](int u) {
-        const int at = ap_chunk(S, u) * CH & (B - 1);
+        const int at = chunk_of(u) * CH & (B - 1);
         const int64_t ph = (int64_t)max(pv, 0) * A.C.n_kv + h;
         const uint8_t *vp = vb + (ph * head_bytes + at / 2);
 #pragma unroll
@@ -537,7 +546,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = ap_f4{0, 0, 0, 0};
     for (; u < u1; u += WAVES) {
-        const int next = min(u + WAVES, u1 - 1), c = ap_chunk(S, u);
+        const int next = min(u + WAVES, u1 - 1), c = chunk_of(u);
         ap_f4 sc[TT];
 #pragma unroll
         for (int t = 0; t < TT; t++) sc[t] = ap_f4{0, 0, 0, 0};
@@ -648,7 +657,7 @@ __device__ inline float ap4_from(float x) {
 //
 // Bound by the vector step: its pipes are busy for half of the time and the matrix ones for a third, and a wave
 // overlaps little of its own (two waves a SIMD are all that the registers allow). 3 prompts of up to 4096 tokens behind up to 1000, 40
-// heads of 128 on 8, slopes and prefixes, 800 us: 366 TFLOP/s, twice that with the second halves, against the
+// heads of 128 on 8, slopes and prefixes, 685 us: 427 TFLOP/s, twice that with the second halves, against the
 // 1177 of a large f16 product; 4096 rows of 32 heads of 128 319, of 64 222. Four waves a block for heads up to 64
 // (with eight 252), eight for wider ones (with four, of whose blocks LDS holds one, 497).
 constexpr int ap4_tile_waves(int hd) { return hd <= 64 ? 4 : 8; }
@@ -677,7 +686,9 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
     const Sight S = ap_sight(A, r, s, tile * kApTileRows / A.G, min((tile * kApTileRows + kApTileRows - 1) / A.G, n_tok - 1));
     const int n_split = ap_splits(A, S.n, A.per_split);
     if (split >= n_split) return;
-    const int u0 = (int)((int64_t)S.n * split / n_split), u1 = (int)((int64_t)S.n * (split + 1) / n_split);
+    const int u0 = __builtin_amdgcn_readfirstlane((int)((int64_t)S.n * split / n_split));
+    const int u1 = __builtin_amdgcn_readfirstlane((int)((int64_t)S.n * (split + 1) / n_split));
+    auto chunk_of = [&](int u) { return ap4_chunk(S, u0, u1, u); };
 
     // the wave's rows and this lane's
     const int row0 = tile * kApTileRows + wave * 32;
@@ -717,13 +728,13 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
     }
     const uint32_t soff = (uint32_t)(h << shift) + (scaled & (B - 1));
     auto load_entries = [&](int u) {
-        const int j0 = ap_chunk(S, u) * 64;
+        const int j0 = chunk_of(u) * 64;
 #pragma unroll
         for (int i = 0; i < NU; i++) ek[i] = entry_of(j0 + unit(i) / NS);
         ev = entry_of(j0 + seg);
     };
     auto load_keys = [&](int u) {
-        const int j0 = ap_chunk(S, u) * 64, at = j0 & (B - 1);
+        const int j0 = chunk_of(u) * 64, at = j0 & (B - 1);
 #pragma unroll
         for (int i = 0; i < NU; i++) {
             const uint64_t pg = (uint32_t)max(page_of(j0 + unit(i) / NS, ek[i]), 0);
@@ -738,7 +749,7 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
         if (tid < 128) scale = (tid < 64 ? A.kd : A.vd)[(uint64_t)(uint32_t)max(vpg, 0) * page_scales + at + soff];
     };
     auto load_values = [&](int u) {
-        const int at = ap_chunk(S, u) * 64 & (B - 1);
+        const int at = chunk_of(u) * 64 & (B - 1);
         const uint64_t pg = (uint32_t)max(vpg, 0);
 #pragma unroll
         for (int i = 0; i < NU; i++) {
@@ -850,7 +861,7 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
         scores(sc, 0, 0);
     }
     for (int u = u0; u < u1; u++) {
-        const int buf = (u - u0) & 1, j0 = ap_chunk(S, u) * 64;
+        const int buf = (u - u0) & 1, j0 = chunk_of(u) * 64;
         const bool whole = ap_whole(A, W, j0, 64);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
