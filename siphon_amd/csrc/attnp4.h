@@ -354,7 +354,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
 // group are used. No code is multiplied by a sub: the subs of a token and its group are two numbers of a
 // lane where the other kernel has eight, and their products with codes.
 //
-// Bound by memory and vector instructions at once: of a chunk's 660 instructions 290 make codes f16, the others are
+// Bound by memory and vector instructions at once: of a chunk's 640 instructions 290 make codes f16, the others are
 // scores, weights and splits, of which NG columns have the same (vector pipes busy for two thirds of the time,
 // matrix ones a fifth). 64 single tokens over up to 8192 keys, 32 heads of 128 on 8, 66-72 us (224 MB, 3.1-3.4 TB/s), 94 by
 // the kernel above; one over 131072 42 (147 MB, 3.5 TB/s) and 63; 16 over up to 16000, 16 heads of 256 on 8, 78. Which of both runs
@@ -655,7 +655,7 @@ __device__ inline float ap4_from(float x) {
 // values follow; two barriers a chunk. The queries' lower halves are read from LDS for each half: in
 // registers they would leave none for the next scores.
 //
-// Bound by the vector step: its pipes are busy for half of the time and the matrix ones for a third, and a wave
+// Bound by the vector step: its pipes are busy for more than half of the time and the matrix ones for 42%, and a wave
 // overlaps little of its own (two waves a SIMD are all that the registers allow). 3 prompts of up to 4096 tokens behind up to 1000, 40
 // heads of 128 on 8, slopes and prefixes, 685 us: 427 TFLOP/s, twice that with the second halves, against the
 // 1177 of a large f16 product; 4096 rows of 32 heads of 128 319, of 64 222. Four waves a block for heads up to 64
