@@ -78,6 +78,9 @@ int check_batch(sihip_ctx *ctx, const char *fn, const sihip_kv_batch *b, int64_t
     return SIHIP_OK;
 }
 
+// Rotated queries of more than twice what the L2s hold are written past them.
+constexpr int64_t kPastBytes = 64 << 20;
+
 // The new rows of a step for a cache of n_kv heads of hd dims. Without tokens
 // (R.max_q 0) arrays may be missing.
 int check_rows(sihip_ctx *ctx, const char *fn, const sihip_kv_rows *a, const BatchArgs &R, int n_kv, int hd, RopeArgs &P,
@@ -113,7 +116,8 @@ int check_rows(sihip_ctx *ctx, const char *fn, const sihip_kv_rows *a, const Bat
             return set_err(ctx, SIHIP_EINVAL, "%s: in place, ldq %lld and ldq_out %lld must be equal", fn, (long long)a->ldq,
                            (long long)a->ldq_out);
         Q = {a->q, a->q_out, a->ldq, a->ldq_out, (int)(a->n_head / n_kv),
-             aligned(a->q, 16) && aligned(a->q_out, 16) && a->ldq % 4 == 0 && a->ldq_out % 4 == 0};
+             aligned(a->q, 16) && aligned(a->q_out, 16) && a->ldq % 4 == 0 && a->ldq_out % 4 == 0,
+             R.n_tok * wide * 4 > kPastBytes};
     }
     if (R.max_q > 0 && (!a->k || !a->v || !aligned(a->k, 4) || !aligned(a->v, 4)))
         return set_err(ctx, SIHIP_EINVAL, "%s: k and v must be f32 arrays", fn);

@@ -29,6 +29,7 @@ struct RopeQueries {
     int64_t ldq, ldo;
     int G;      // query heads of a KV head
     bool wide;  // rows of q and out and their heads are 16-byte aligned
+    bool past;  // out is more than the L2s hold: written past them
 };
 
 __device__ inline float2 rope_pair(float a, float b, float c, float s) {
@@ -86,12 +87,21 @@ __device__ inline float4 rope_load4(const RopeArgs &P, const float *x, const flo
     return float4{v[0], v[1], v[2], v[3]};
 }
 
+typedef float rope_f4 __attribute__((ext_vector_type(4)));
+template <bool PAST>
+__device__ inline void rope_store4(float *to, float4 v) {
+    if constexpr (PAST) __builtin_nontemporal_store(rope_f4{v.x, v.y, v.z, v.w}, (rope_f4 *)to);
+    else *(float4 *)to = v;
+}
+
 // The rows q0 + t0 .. q0 + t1 - 1 of a request whose row 0 is at position p0, of the
 // query heads of KV head h, by a workgroup of THREADS: a thread takes four pairs (or
 // eight dims that are not rotated) at a time, reads both of each pair and writes
-// both, so that out may be q.
-template <int THREADS>
-__device__ inline void rope_queries(const RopeArgs &P, const RopeQueries &Q, int hd, int h, int64_t q0, int p0, int t0, int t1) {
+// both, so that out may be q. What the L2s cannot hold is written past them: queries of 111 MB, with the append of their
+// keys and values and its read-back, 73 us and 89 the other way, 78 MB 60 / 65, 65 MB 47 / 50; 49 MB 79 / 78, 34 MB
+// 24 / 25 alone over 8 bits and 23 / 22 over 4.
+template <int THREADS, bool PAST>
+__device__ inline void rope_queries_to(const RopeArgs &P, const RopeQueries &Q, int hd, int h, int64_t q0, int p0, int t0, int t1) {
     const int turns = (P.pairs + 3) / 4, rest = (hd - 2 * P.pairs + 7) / 8, per_head = turns + rest;
     const int n = (t1 - t0) * Q.G * per_head;
     const bool fours = Q.wide && P.fours;
@@ -103,8 +113,8 @@ __device__ inline void rope_queries(const RopeArgs &P, const RopeQueries &Q, int
             const int d0 = 2 * P.pairs + 8 * (it - turns);
             if (fours) {  // (2 pairs is a multiple of 8, so d0 is; hd of 16)
                 const float4 a = *(const float4 *)(x + d0), b = *(const float4 *)(x + d0 + 4);
-                *(float4 *)(to + d0) = a;
-                *(float4 *)(to + d0 + 4) = b;
+                rope_store4<PAST>(to + d0, a);
+                rope_store4<PAST>(to + d0 + 4, b);
             } else {
                 for (int d = d0; d < min(d0 + 8, hd); d++) to[d] = x[d];
             }
@@ -112,19 +122,24 @@ __device__ inline void rope_queries(const RopeArgs &P, const RopeQueries &Q, int
         }
         const float *cs = P.table + (int64_t)(p0 + t) * (2 * P.pairs) + 8 * it;
         if (fours) {
-            const float4 t0 = *(const float4 *)cs, t1 = *(const float4 *)(cs + 4);
-            const int at = P.neighbours ? 8 * it : 4 * it, next = P.neighbours ? at + 4 : at + P.pairs;
+            // (neighbours past the L2s: two times two pairs, so that a wave's lanes write whole lines at a time)
+            const bool four = P.neighbours && !PAST;
+            const int at = four ? 8 * it : 4 * it, next = four ? at + 4 : at + P.pairs;
+            const float *c0 = cs, *c1 = cs + 4;
+            if constexpr (PAST)
+                if (P.neighbours) c0 = cs - at, c1 = c0 + P.pairs;
+            const float4 t0 = *(const float4 *)c0, t1 = *(const float4 *)c1;
             const float4 a = *(const float4 *)(x + at), b = *(const float4 *)(x + next);
             if (P.neighbours) {
                 const float2 r0 = rope_pair(a.x, a.y, t0.x, t0.y), r1 = rope_pair(a.z, a.w, t0.z, t0.w);
                 const float2 r2 = rope_pair(b.x, b.y, t1.x, t1.y), r3 = rope_pair(b.z, b.w, t1.z, t1.w);
-                *(float4 *)(to + at) = float4{r0.x, r0.y, r1.x, r1.y};
-                *(float4 *)(to + next) = float4{r2.x, r2.y, r3.x, r3.y};
+                rope_store4<PAST>(to + at, float4{r0.x, r0.y, r1.x, r1.y});
+                rope_store4<PAST>(to + next, float4{r2.x, r2.y, r3.x, r3.y});
             } else {
                 const float2 r0 = rope_pair(a.x, b.x, t0.x, t0.y), r1 = rope_pair(a.y, b.y, t0.z, t0.w);
                 const float2 r2 = rope_pair(a.z, b.z, t1.x, t1.y), r3 = rope_pair(a.w, b.w, t1.z, t1.w);
-                *(float4 *)(to + at) = float4{r0.x, r1.x, r2.x, r3.x};
-                *(float4 *)(to + next) = float4{r0.y, r1.y, r2.y, r3.y};
+                rope_store4<PAST>(to + at, float4{r0.x, r1.x, r2.x, r3.x});
+                rope_store4<PAST>(to + next, float4{r0.y, r1.y, r2.y, r3.y});
             }
             continue;
         }
@@ -135,6 +150,12 @@ __device__ inline void rope_queries(const RopeArgs &P, const RopeQueries &Q, int
             to[b] = r.y;
         }
     }
+}
+
+template <int THREADS>
+__device__ inline void rope_queries(const RopeArgs &P, const RopeQueries &Q, int hd, int h, int64_t q0, int p0, int t0, int t1) {
+    if (Q.past) rope_queries_to<THREADS, true>(P, Q, hd, h, q0, p0, t0, t1);
+    else rope_queries_to<THREADS, false>(P, Q, hd, h, q0, p0, t0, t1);
 }
 
 }  // namespace sihip

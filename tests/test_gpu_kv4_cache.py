@@ -38,7 +38,7 @@ class Append:
     """One append of a batch, and everything it may and may not write."""
 
     def __init__(self, dev, cache, pages, q_start, kv_len, k, v, q=None, rope=None, neighbours=False, gap=4, shift=4, in_place=False,
-                 max_q=None, max_kv=None, stream=None):
+                 max_q=None, max_kv=None, stream=None, n_tok=None):
         n, width = len(k), cache.n_kv * cache.hd
         heads = 0 if q is None else q.shape[1]
         ld, ldq = width + gap, heads * cache.hd + gap
@@ -51,7 +51,7 @@ class Append:
             arrays["qo"] = np.full_like(arrays["q"], 77.0)
         with ko.OnDevice(dev, **arrays) as d:
             c = (k4 if four else ko).put_cache(d, cache)
-            b = ko.put_batch(d, pages, q_start, kv_len, n, max_q=max_q, max_kv=max_kv)
+            b = ko.put_batch(d, pages, q_start, kv_len, n_tok or n, max_q=max_q, max_kv=max_kv)
             rows = sa.KvRows(k=d.ptr("nk") + 4 * shift, v=d.ptr("nv") + 4 * shift, ldk=ld, ldv=ld)
             if q is not None:
                 rows.q, rows.ldq, rows.ldq_out, rows.n_head = d.ptr("q") + 4 * shift, ldq, ldq, heads
@@ -122,6 +122,24 @@ def test_rotated_append(dev, bits_, neighbours, hd, dim, aligned):
     rope = k4.table(int(kv_len.max()) + 3, dim)
     got = Append(dev, cache, pages, q_start, kv_len, k, v, q, rope, neighbours, *((4, 4) if aligned else (3, 1)), in_place=not aligned)
     pos = positions(q_start, kv_len, n)
+    cache.append(pages, q_start, kv_len, k4.rotate(k, pos, rope, neighbours), v)
+    check(got, cache)
+    assert same(got.q, k4.rotate(q, pos, rope, neighbours))
+
+
+@pytest.mark.parametrize("bits_", [4, 8])
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("hd,dim", ROPES)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rotated_queries_of_large_steps(dev, bits_, neighbours, hd, dim, in_place):
+    """A step of so many rows, as far as the host's bound says, that queries are written past the caches."""
+    rng = np.random.default_rng(hd + dim + bits_)
+    cache, pages, q_start, kv_len = make(bits_, rng, [0, 40, 15], [50, 1, 33], 16, 2, hd)
+    k, v, q = (step_rows(rng, 84, h, hd) for h in (2, 2, 6))
+    rope = k4.table(int(kv_len.max()), dim)
+    got = Append(dev, cache, pages, q_start, kv_len, k, v, q, rope, neighbours, in_place=in_place, max_q=60,
+                 n_tok=(64 << 20) // (4 * 6 * hd) + 1)
+    pos = positions(q_start, kv_len, 84)
     cache.append(pages, q_start, kv_len, k4.rotate(k, pos, rope, neighbours), v)
     check(got, cache)
     assert same(got.q, k4.rotate(q, pos, rope, neighbours))
