@@ -188,7 +188,7 @@ __device__ inline uint32_t kv4_codes(const float *v, const Kv4Step &q) {
 // from where a thread takes four dims of eight tokens, turns them round and writes a
 // word a dim. Words that hold other tokens as well keep those.
 //
-// Bound by memory: 5 prompt chunks of up to 2047 tokens, 40 heads of 128 on 8, rotated, 288 MB in 70.5 us (4.1 TB/s; the
+// Bound by memory: 5 prompt chunks of up to 2047 tokens, 40 heads of 128 on 8, rotated, 288 MB in 58.4 us (4.9 TB/s; the
 // queries are four fifths of it), 26.8 without queries, where four rows a wave at a time are quantized in about 100 instructions each: divisions
 // and rounding proofs only next to a border. One token each for 64 requests 6.2 us, of which an empty launch takes 3.5.
 __global__ __launch_bounds__(k4Threads) void kv4_append_kernel(Append4Args A) {

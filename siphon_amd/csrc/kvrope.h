@@ -2,7 +2,7 @@
 // way (rope.h): kv_append_kernel (kvcache.h) on rotated keys, and in the same
 // launch the step's queries.
 //
-// Bound by memory: 5 prompt chunks of up to 2047 tokens, 40 heads of 128 on 8, 293 MB in 70 us (4.2 TB/s; the queries are
+// Bound by memory: 5 prompt chunks of up to 2047 tokens, 40 heads of 128 on 8, 293 MB in 59 us (4.9 TB/s; the queries are
 // four fifths of it, 27 us without them); one token each for 64 requests 7 us, of which an empty launch takes
 // 3.5. Queries are a layer of workgroups of their own, a page's tokens and a KV head each, because keys and values
 // need the whole page's maximum first, and they nothing.
