@@ -310,14 +310,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
             for (int d = 0; d < ND; d++) o[d] *= ao;
         }
         // weights, and their products with the values' scales
-        float z[SEG], most = 0.0f;
+        float z[SEG], most = 0.0f, few = 0.0f;
 #pragma unroll
         for (int i = 0; i < SEG; i++) {
             const float x = __builtin_amdgcn_exp2f(fmaf(w[i], f, -R.m));
-            R.l += x;
+            few += x;
             z[i] = x * vs[i];
             most = fmaxf(most, z[i]);
         }
+        R.l += few;
         if (__any(most > 16.0f * R.ref)) {
             const float ao = R.refer(1.0f, ap_max_quarters(most));
 #pragma unroll
@@ -607,14 +608,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
             for (int d = 0; d < ND; d++) o[d] *= ao;
         }
         // weights, and their products with the values' scales
-        float z[SEG], most = 0.0f;
+        float z[SEG], most = 0.0f, few = 0.0f;
 #pragma unroll
         for (int i = 0; i < SEG; i++) {
             const float x = __builtin_amdgcn_exp2f(fmaf(w[i], f, -R.m));
-            R.l += x;
+            few += x;
             z[i] = x * vs[i];
             most = fmaxf(most, fabsf(z[i]));
         }
+        R.l += few;
         if (__any(most > 16.0f * R.ref)) {
             const float ao = R.refer(1.0f, ap_max_quarters(most));
 #pragma unroll
@@ -920,13 +922,15 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
                 // the next half's scores (behind the last chunk: of what is there, for nobody) beside the weights
                 ap_f16 next;
                 scores(next, i == 0 ? buf : buf ^ 1, i ^ 1);
-                float z[16];
+                // (16 weights are added first: a sum of thousands, one by one, is off by more than the products)
+                float z[16], l16 = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const float w = __builtin_amdgcn_exp2f(fmaf(sc[e], f, -R.m));
-                    R.l += w;
+                    l16 += w;
                     z[e] = w * vd[e];
                 }
+                R.l += l16;
                 ap_h8 ph[2], pl[2];
 #pragma unroll
                 for (int e = 0; e < 2; e++) ap_split8w(z + 8 * e, R.over, ph[e], pl[e]);
