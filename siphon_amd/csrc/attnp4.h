@@ -675,7 +675,7 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
     __shared__ uint4 q_lds[WAVES][NS][64];  // the lower halves of each wave's queries
     __shared__ __attribute__((aligned(16))) float s_lds[2][2][64];  // scales of keys and values
     __shared__ __attribute__((aligned(16))) float m_lds[2][4];  // the largest scale of a segment of 16 values, -1 without a page
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
     const int h = blockIdx.x % A.C.n_kv, split = blockIdx.y;
     const int64_t place = blockIdx.x / A.C.n_kv;
