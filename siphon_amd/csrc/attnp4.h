@@ -659,8 +659,8 @@ __device__ inline float ap4_from(float x) {
 //
 // Bound by the vector step: its pipes are busy for more than half of the time and the matrix ones for 42%, and a wave
 // overlaps little of its own (two waves a SIMD are all that the registers allow). 3 prompts of up to 4096 tokens behind up to 1000, 40
-// heads of 128 on 8, slopes and prefixes, 685 us: 427 TFLOP/s, twice that with the second halves, against the
-// 1177 of a large f16 product; 4096 rows of 32 heads of 128 319, of 64 222. Four waves a block for heads up to 64
+// heads of 128 on 8, slopes and prefixes, 670 us: 437 TFLOP/s, twice that with the second halves, against the
+// 1177 of a large f16 product; 4096 rows of 32 heads of 128 322, of 64 219. Four waves a block for heads up to 64
 // (with eight 252), eight for wider ones (with four, of whose blocks LDS holds one, 497).
 constexpr int ap4_tile_waves(int hd) { return hd <= 64 ? 4 : 8; }
 
