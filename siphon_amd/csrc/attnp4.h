@@ -719,6 +719,7 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
     uint32_t kr[NU][2], ksub[NU], vr[NU][2], vsub[NU][2], scale;
     int ek[NU], ev, vpg = -1;  // entries; the page of this thread's values and scale
     bool seen = false;         // some row may see the key of `scale`
+    const int seen_to = min(S.keys, max(S.p_hi + 1, S.prefix));
 #pragma unroll
     for (int i = 0; i < NU; i++) {
         const int key = unit(i) / NS, d = unit(i) % NS * 16 < hd ? unit(i) % NS * 16 : 0;
@@ -745,9 +746,10 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
             ksub[i] = *(const uint8_t *)(A.ksub + (pg * page_subs + at + ksoff[i]));
         }
         vpg = page_of(j0 + seg, ev);
-        // (what no row sees may have any scale, and counts as zero)
+        // (what no row sees may have any scale, and counts as zero: also new tokens behind the block's last row, which
+        // nothing has written where they are past max_q)
         const int j = j0 + scaled;
-        seen = vpg >= 0 && j < S.keys && (!A.window || j > S.p_lo - A.window || j < S.prefix);
+        seen = vpg >= 0 && j < seen_to && (!A.window || j > S.p_lo - A.window || j < S.prefix);
         if (tid < 128) scale = (tid < 64 ? A.kd : A.vd)[(uint64_t)(uint32_t)max(vpg, 0) * page_scales + at + soff];
     };
     auto load_values = [&](int u) {
