@@ -293,6 +293,17 @@ struct Running {
     }
 };
 
+// The unit of a piece's sums, `unit` times the reference, at its end, where weights (relative to 2^m, with the total l) times
+// values are made numbers of f32. Sums of many large values can pass the largest of those where their mean does not: m + 64
+// with l and the sums times 2^-64 stand for the same, and are joined with other pieces as any.
+__device__ inline float ap_unit(const Running &R, float unit, float &m, float &l) {
+    const bool large = R.ref > 0x1p60f;
+    const float down = large ? 0x1p-64f : 1.0f;
+    m = large ? R.m + 64.0f : R.m;
+    l *= down;
+    return R.ref * down * unit;
+}
+
 // ---- few rows ----------------------------------------------------------------------
 //
 // One workgroup: 16 rows of one request and KV head, one split of its
@@ -510,16 +521,16 @@ __device__ __forceinline__ bool ap_rows_place(const AttnPArgs &A, int &r, int &h
 
 // The end of a 16-row block's piece: its waves' sums joined through LDS, then whole
 // rows to out, or a part for ap_join_rows. o: sums of 16-dim tiles, dims 16 d + 4 (lane / 16) ..
-// of the column lane % 16.
+// of the column lane % 16, in units of `unit` times the reference.
 template <int ND, int WAVES, int RB = 16>
-__device__ __forceinline__ void ap_rows_end(const AttnPArgs &A, const Span &s, const Running &R, const ap_f4 (&o)[ND], int h, int tile,
-                                            int n_rows, int64_t piece, int split, int n_split, int tok, int head) {
+__device__ __forceinline__ void ap_rows_end(const AttnPArgs &A, const Span &s, const Running &R, const ap_f4 (&o)[ND], float unit, int h,
+                                            int tile, int n_rows, int64_t piece, int split, int n_split, int tok, int head) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4, hd = A.C.hd;
     // all lanes of a column hold the same m and parts of l
-    float m = R.m, l = R.l;
+    float m, l = R.l;
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    const float back = R.ref * (1.0f / kApUnit);
+    const float back = ap_unit(R, unit, m, l);
     const int rows = min(16, n_rows - tile * 16);
     const __amdgpu_buffer_rsrc_t part = ap_pieces(A, piece, 1);
     if constexpr (WAVES == 1) {
@@ -779,7 +790,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp_rows_kernel(AttnPArgs A) 
         pv = page_of(min(next + WAVES, u1 - 1), g);
     }
 
-    ap_rows_end<ND, WAVES>(A, s, R, o, h, tile, n_rows, piece, split, n_split, tok, head);
+    ap_rows_end<ND, WAVES>(A, s, R, o, 1.0f / kApUnit, h, tile, n_rows, piece, split, n_split, tok, head);
 }
 
 // ---- many rows ---------------------------------------------------------------------
@@ -1153,10 +1164,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 2) void attnp_tiles_ke
         }
     }
     if (kTurns && u0 < u1 && wave < 4) __syncthreads();
-    float m = R.m, l = R.l;
+    float m, l = R.l;
     l += __shfl_xor(l, 32);
 
-    const float back = R.ref * (1.0f / kApUnit);
+    const float back = ap_unit(R, 1.0f / kApUnit, m, l);
     if (row0 + col < n_rows) {
         // four dims in a row a register group: 32 d + 8 a + 4 half ..
         if (n_split == 1) {

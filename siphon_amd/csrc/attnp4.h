@@ -343,8 +343,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
         }
         load_values(next);
     }
-    R.ref *= kAp4Unit;  // (of the sums, here on)
-    ap_rows_end<ND, WAVES>(A, s, R, o, h, tile, n_rows, piece, split, n_split, tok, head);
+    ap_rows_end<ND, WAVES>(A, s, R, o, kAp4Unit / kApUnit, h, tile, n_rows, piece, split, n_split, tok, head);
 }
 
 // The same for so few rows that the 16 columns of a tile can be NG groups of 32 dims times RB =
@@ -637,8 +636,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
             }
         load_values(next);
     }
-    R.ref *= kAp4Code;  // (of the sums, here on)
-    ap_rows_end<ND, WAVES, RB>(A, s, R, o, h, tile, n_rows, piece, split, n_split, tok, head);
+    ap_rows_end<ND, WAVES, RB>(A, s, R, o, kAp4Code / kApUnit, h, tile, n_rows, piece, split, n_split, tok, head);
 }
 
 // ---- many rows ---------------------------------------------------------------------
@@ -960,10 +958,10 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
             __syncthreads();
         }
     }
-    float m = R.m, l = R.l;
+    float m, l = R.l;
     l += __shfl_xor(l, 32);
 
-    const float back = R.ref * (kAp4Unit / kApUnit);
+    const float back = ap_unit(R, kAp4Unit / kApUnit, m, l);
     if (row0 + col < n_rows) {
         // four dims in a row a register group: 32 d + 8 a + 4 half ..
         if (n_split == 1) {
