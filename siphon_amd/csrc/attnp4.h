@@ -26,7 +26,8 @@ typedef uint32_t ap_u4 __attribute__((ext_vector_type(4)));
 // Products are in units of 2^-16: a nibble n where it lies in a half word, at bit 0 or 4, is the
 // f16 number n 2^-24 or n 2^-20 (subnormal, which costs the packed FMA nothing). Elements 0, 1
 // and 4, 5 of a word are at bit 0 of their halves (the latter after a shift by 8), 2, 3 and 6, 7 at bit 4.
-constexpr float kAp4Unit = 0x1p16f;
+constexpr int kAp4Bits = 16;
+constexpr float kAp4Unit = 1 << kAp4Bits;
 
 // subs of a pair of elements: times 2^8 or 2^4, which any byte allows (2^9 times -128, of memory
 // that was never written, would be infinite), and -8 sub 2^-16
@@ -71,6 +72,20 @@ __device__ inline void ap4_subs(uint32_t x, uint32_t y, Ap4Sub (&s)[4]) {
 
 // a bfloat16 in the low or high half of x
 __device__ inline float ap4_bf16(uint32_t x, int high) { return __builtin_bit_cast(float, high ? x & 0xffff0000u : x << 16); }
+
+// What turns a row's sums of products, in units of 2^-e times its queries' power of two, into scores in log2 units (f) or
+// the argument of the tanh (fc). Of large queries f can pass the largest number where scores do not, as keys are small: from 2^100
+// on it is 2^64 less, true is returned, and sums times a key's scale are multiplied by that first (ap4_raise). f is above zero: it
+// leaves -inf as it is.
+__device__ inline bool ap4_factors(const AttnPArgs &A, int e, float &f, float &fc) {
+    const bool large = e + __builtin_amdgcn_frexp_expf(A.scale2) > 100;
+    if (large) e -= 64;
+    f = fminf(fmaxf(ldexpf(A.scale2, e), 0x1p-149f), FLT_MAX);
+    fc = fminf(ldexpf(A.cap_in, e), FLT_MAX);
+    return large;
+}
+// (a choice for each number, not of a factor, which would be held in a register throughout)
+__device__ inline float ap4_raise(float x, bool large) { return large ? x * 0x1p64f : x; }
 
 // Chunk u of u0 .. u1 - 1, the nearest first. With slopes scores rise towards a row's own position, and in
 // the other order nearly every chunk would move the maximum and the sums with it: 3 prompts of up to 4096, 40 heads, 810
@@ -215,6 +230,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
     // the query, while the first keys are on their way
     ap_h8 qh[NK][KW], ql[NK][KW];
     float f_row, fc_row;
+    bool large;
     {
         // (no scale: zeros, so that a score is zero whatever the key)
         const float sign = A.scale2 > 0.0f ? A.sign : 0.0f;
@@ -237,10 +253,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
                 for (int j = 0; j < 8; j++) x[e][y][j] = ldexpf(x[e][y][j], e2);
                 ap_split8(x[e][y], qh[e][y], ql[e][y]);
             }
-        f_row = ldexpf(kAp4Unit, -e2);
-        fc_row = fminf(f_row * A.cap_in, FLT_MAX);
-        f_row = fmaxf(f_row * A.scale2, FLT_MIN);  // above zero: it leaves -inf as it is
+        large = ap4_factors(A, kAp4Bits - e2, f_row, fc_row);
     }
+    const bool any_large = __any(large);
     Running R;
     ap_f4 o[ND];
 #pragma unroll
@@ -280,6 +295,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
         const bool here = pv >= 0;
         load_keys(next);
         load_entries(min(next + WAVES, u1 - 1));
+        if (any_large) {
+#pragma unroll
+            for (int i = 0; i < SEG; i++) w[i] = ap4_raise(w[i], large);
+        }
         if (A.cap != 0.0f) {
 #pragma unroll
             for (int i = 0; i < SEG; i++) w[i] = ap_capped(A, w[i] * f, w[i] * fc_row);
@@ -361,7 +380,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
 // is a matter of the columns: more rows do not fit.
 // Codes alone, in units of 2^-10: of a nibble n 2^-24 or n 2^-20 (ap4_cvt) one packed FMA with
 // constants.
-constexpr float kAp4Code = 0x1p10f;
+constexpr int kAp4CodeBits = 10;
+constexpr float kAp4Code = 1 << kAp4CodeBits;
 
 __device__ inline ap_h8 ap4_codes(uint32_t w) {
     const _Float16 f = (_Float16)0x1p14f, g = (_Float16)0x1p10f, off = (_Float16)-0x1p-7f;
@@ -515,6 +535,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
     // the query, while the first keys are on their way
     ap_h8 qh[NK][KW], ql[NK][KW];
     float f_row, fc_row;
+    bool large;
     {
         // (no scale: zeros, so that a score is zero whatever the key)
         const float sign = A.scale2 > 0.0f ? A.sign : 0.0f;
@@ -537,10 +558,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
                 for (int j = 0; j < 8; j++) x[e][y][j] = dim_of(e) / 32 == group ? ldexpf(x[e][y][j], e2) : 0.0f;
                 ap_split8(x[e][y], qh[e][y], ql[e][y]);
             }
-        f_row = ldexpf(kAp4Code, -e2);
-        fc_row = fminf(f_row * A.cap_in, FLT_MAX);
-        f_row = fmaxf(f_row * A.scale2, FLT_MIN);  // above zero: it leaves -inf as it is
+        large = ap4_factors(A, kAp4CodeBits - e2, f_row, fc_row);
     }
+    const bool any_large = __any(large);
     Running R;
     ap_f4 o[ND];
 #pragma unroll
@@ -577,6 +597,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
         const bool here = pv >= 0;
         load_keys(next);
         load_entries(min(next + WAVES, u1 - 1));
+        if (any_large) {
+#pragma unroll
+            for (int i = 0; i < SEG; i++) w[i] = ap4_raise(w[i], large);
+        }
         if (A.cap != 0.0f) {
 #pragma unroll
             for (int i = 0; i < SEG; i++) w[i] = ap_capped(A, w[i] * f, w[i] * fc_row);
@@ -825,10 +849,11 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
             ap_split8(x[c], qh[c], lo);
             q_lds[wave][c][lane] = __builtin_bit_cast(uint4, lo);
         }
-        f_row = ldexpf(kAp4Unit, -e2);
-        fc_row = fminf(f_row * A.cap_in, FLT_MAX);
-        f_row = fmaxf(f_row * A.scale2, FLT_MIN);  // above zero: it leaves -inf as it is
+        if (ap4_factors(A, kAp4Bits - e2, f_row, fc_row)) f_row = -f_row;
     }
+    // (large rows have the sign of f_row, taken off for each half: a register or a mask of their own spills others of heads of
+    // 64, 4096 rows 232 us and not 220)
+    const bool any_large = __any(f_row < 0.0f), capped_or_large = any_large || A.cap != 0.0f;
     ap_f16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++)
@@ -873,15 +898,24 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
                 const float vmax = i == 0 ? (half ? vm.y : vm.x) : (half ? vm.w : vm.z);
                 const float *kd = &s_lds[buf][0][32 * i + 16 * half], *vd = &s_lds[buf][1][32 * i + 16 * half];
                 float f = f_row;
+                asm("" : "+v"(f));
+                const bool large = f < 0.0f;
+                f = fabsf(f);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const float4 d = ((const float4 *)kd)[e];
                     sc[4 * e] *= d.x, sc[4 * e + 1] *= d.y, sc[4 * e + 2] *= d.z, sc[4 * e + 3] *= d.w;
                 }
-                if (A.cap != 0.0f) {
+                if (capped_or_large) {
+                    if (any_large) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) sc[e] = ap_capped(A, sc[e] * f, sc[e] * fc_row);
-                    f = 1.0f;
+                        for (int e = 0; e < 16; e++) sc[e] = ap4_raise(sc[e], large);
+                    }
+                    if (A.cap != 0.0f) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) sc[e] = ap_capped(A, sc[e] * f, sc[e] * fc_row);
+                        f = 1.0f;
+                    }
                 }
                 const int j1 = j0 + 32 * i + 16 * half;
                 if (A.slopes) {

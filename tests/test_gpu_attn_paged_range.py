@@ -46,3 +46,29 @@ def test_large_values(dev, option, bits, kernel, hd, block, log2, row_waves, spl
     q = queries(rng, sum(adds), group * n_kv, hd, 2.0)
     got = attend(bits, dev, cache, pages, q_start, kv_len, q, 1 / np.sqrt(hd))
     ks.check(got, cache, pages, q_start, kv_len, q, 1 / np.sqrt(hd))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("hd,block", [(128, 16), (64, 64), (96, 32), (256, 32)])
+@pytest.mark.parametrize("log2_q,log2_k,change", [
+    (110, -90, "none"), (118, -98, "none"), (124, -98, "slopes"), (126.5, -98, "none"), (126.5, -98, "cap"), (126.5, -60, "none"),
+    (-10, 80, "none"), (-60, 60, "none")])
+def test_sizes_of_queries_and_keys(dev, option, bits, kernel, hd, block, log2_q, log2_k, change):
+    """Queries and keys of any size whose scores are of ordinary size, among them the largest that sums of products can have:
+    keys whose dims all have the largest magnitude and the queries' signs."""
+    group, (lengths, adds), large = KERNELS[kernel]
+    option("ATTNP_LARGE", large)
+    rng = np.random.default_rng(hd + int(log2_q))
+    n, n_kv = sum(lengths) + sum(adds), 2
+    u = rng.choice([-1, 1], (n_kv, hd))
+    k = rng.uniform(-1, 1, (n, n_kv, hd)) * u
+    k[::3] = rng.choice([-1, 1], (len(k[::3]), 1, 1)) * u
+    v = rng.standard_normal((n, n_kv, hd))
+    cache, pages, q_start, kv_len = filled(bits, lengths, adds, block, (k * 2.0 ** log2_k).astype(np.float32), v.astype(np.float32), rng)
+    q = np.repeat(u, group, 0)[None] * rng.uniform(0.7, 1.3, (sum(adds), group * n_kv, hd))
+    q = (q * 2.0 ** log2_q).astype(np.float32)
+    kq = 20 / hd * 2.0 ** -(log2_q + log2_k)
+    o = dict(none={}, cap=dict(cap=10.0), slopes=dict(slopes=2.0 ** -np.arange(group * n_kv, dtype=np.float32)))[change]
+    got = attend(bits, dev, cache, pages, q_start, kv_len, q, kq, **dict(o))
+    ks.check(got, cache, pages, q_start, kv_len, q, float(np.float32(kq)), **o)
