@@ -10,6 +10,8 @@
 // value's before they are split.
 #pragma once
 
+#include <limits.h>
+
 #include "attnp.h"
 #include "kvcache4.h"
 
@@ -73,19 +75,19 @@ __device__ inline void ap4_subs(uint32_t x, uint32_t y, Ap4Sub (&s)[4]) {
 // a bfloat16 in the low or high half of x
 __device__ inline float ap4_bf16(uint32_t x, int high) { return __builtin_bit_cast(float, high ? x & 0xffff0000u : x << 16); }
 
-// What turns a row's sums of products, in units of 2^-e times its queries' power of two, into scores in log2 units (f) or
-// the argument of the tanh (fc). Of large queries f can pass the largest number where scores do not, as keys are small: from 2^100
-// on it is 2^64 less, true is returned, and sums times a key's scale are multiplied by that first (ap4_raise). f is above zero: it
-// leaves -inf as it is.
-__device__ inline bool ap4_factors(const AttnPArgs &A, int e, float &f, float &fc) {
-    const bool large = e + __builtin_amdgcn_frexp_expf(A.scale2) > 100;
-    if (large) e -= 64;
+// What turns a row's sums of products times a key's scale, in units of 2^-e times its queries' power of two, into scores in
+// log2 units (f) or the argument of the tanh (fc). Of large queries f can pass the largest number where scores do not, as keys
+// are small; of small ones the sums times a large key's scale can. Where f passes 2^100, or is below 2^least, it is 2^64 less or
+// more, and sums are multiplied by what is returned first. (Scores that pass 2^68 on the way have no weights in f32.) f is
+// above zero: it leaves -inf as it is.
+__device__ inline float ap4_factors(const AttnPArgs &A, int e, int least, float &f, float &fc) {
+    const int size = e + __builtin_amdgcn_frexp_expf(A.scale2);
+    const bool large = size > 100, small = size < least;
+    e += large ? -64 : small ? 64 : 0;
     f = fminf(fmaxf(ldexpf(A.scale2, e), 0x1p-149f), FLT_MAX);
     fc = fminf(ldexpf(A.cap_in, e), FLT_MAX);
-    return large;
+    return large ? 0x1p64f : small ? 0x1p-64f : 1.0f;
 }
-// (a choice for each number, not of a factor, which would be held in a register throughout)
-__device__ inline float ap4_raise(float x, bool large) { return large ? x * 0x1p64f : x; }
 
 // Chunk u of u0 .. u1 - 1, the nearest first. With slopes scores rise towards a row's own position, and in
 // the other order nearly every chunk would move the maximum and the sums with it: 3 prompts of up to 4096, 40 heads, 810
@@ -229,8 +231,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
 
     // the query, while the first keys are on their way
     ap_h8 qh[NK][KW], ql[NK][KW];
-    float f_row, fc_row;
-    bool large;
+    float f_row, fc_row, turn;
     {
         // (no scale: zeros, so that a score is zero whatever the key)
         const float sign = A.scale2 > 0.0f ? A.sign : 0.0f;
@@ -253,9 +254,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
                 for (int j = 0; j < 8; j++) x[e][y][j] = ldexpf(x[e][y][j], e2);
                 ap_split8(x[e][y], qh[e][y], ql[e][y]);
             }
-        large = ap4_factors(A, kAp4Bits - e2, f_row, fc_row);
+        turn = ap4_factors(A, kAp4Bits - e2, -60, f_row, fc_row);
     }
-    const bool any_large = __any(large);
+    const bool turned = __any(turn != 1.0f);
     Running R;
     ap_f4 o[ND];
 #pragma unroll
@@ -284,6 +285,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
                     for (int i = 0; i < 2; i++) sc[t + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], ql[e][y], sc[t + i], 0, 0, 0);
                 }
             }
+        if (turned) {
+#pragma unroll
+            for (int t = 0; t < TT; t++) sc[t] *= turn;
+        }
         // key i of this lane: j0 + i; its score in log2 units is w[i] * f
         const int j0 = c * CH + g * SEG;
         float w[SEG], vs[SEG], f = f_row;
@@ -295,10 +300,6 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
         const bool here = pv >= 0;
         load_keys(next);
         load_entries(min(next + WAVES, u1 - 1));
-        if (any_large) {
-#pragma unroll
-            for (int i = 0; i < SEG; i++) w[i] = ap4_raise(w[i], large);
-        }
         if (A.cap != 0.0f) {
 #pragma unroll
             for (int i = 0; i < SEG; i++) w[i] = ap_capped(A, w[i] * f, w[i] * fc_row);
@@ -534,8 +535,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
 
     // the query, while the first keys are on their way
     ap_h8 qh[NK][KW], ql[NK][KW];
-    float f_row, fc_row;
-    bool large;
+    float f_row, fc_row, turn;
     {
         // (no scale: zeros, so that a score is zero whatever the key)
         const float sign = A.scale2 > 0.0f ? A.sign : 0.0f;
@@ -558,9 +558,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
                 for (int j = 0; j < 8; j++) x[e][y][j] = dim_of(e) / 32 == group ? ldexpf(x[e][y][j], e2) : 0.0f;
                 ap_split8(x[e][y], qh[e][y], ql[e][y]);
             }
-        large = ap4_factors(A, kAp4CodeBits - e2, f_row, fc_row);
+        turn = ap4_factors(A, kAp4CodeBits - e2, -60, f_row, fc_row);
     }
-    const bool any_large = __any(large);
+    const bool turned = __any(turn != 1.0f);
     Running R;
     ap_f4 o[ND];
 #pragma unroll
@@ -585,6 +585,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
 #pragma unroll
                     for (int i = 0; i < 2; i++) sc[t + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], ql[e][y], sc[t + i], 0, 0, 0);
                 }
+        if (turned) {
+#pragma unroll
+            for (int t = 0; t < TT; t++) sc[t] *= turn;
+        }
         // key i of this lane: j0 + i; its score in log2 units is w[i] * f
         const int j0 = c * CH + g * SEG;
         float w[SEG], vs[SEG], f = f_row;
@@ -597,10 +601,6 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
         const bool here = pv >= 0;
         load_keys(next);
         load_entries(min(next + WAVES, u1 - 1));
-        if (any_large) {
-#pragma unroll
-            for (int i = 0; i < SEG; i++) w[i] = ap4_raise(w[i], large);
-        }
         if (A.cap != 0.0f) {
 #pragma unroll
             for (int i = 0; i < SEG; i++) w[i] = ap_capped(A, w[i] * f, w[i] * fc_row);
@@ -695,7 +695,11 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
     __shared__ uint4 k_lds[2][64][KC];
     __shared__ uint4 v_lds[2][ND * 32][8];
     __shared__ uint4 q_lds[WAVES][NS][64];  // the lower halves of each wave's queries
-    __shared__ __attribute__((aligned(16))) float s_lds[2][2][64];  // scales of keys and values
+    // scales of keys, times 2^-12, and values: a sum of 256 products of 2^14 and 1016 2^-16 times 2^116, the largest scale, is then a
+    // number, and of the smallest one, 2^-110, no bits are lost
+    __shared__ __attribute__((aligned(16))) float s_lds[2][2][64];
+    constexpr int kScaleBits = 12;
+    constexpr float kScaleUnit = 1.0f / (1 << kScaleBits);
     __shared__ __attribute__((aligned(16))) float m_lds[2][4];  // the largest scale of a segment of 16 values, -1 without a page
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int hd = A.C.hd, shift = A.C.shift, B = 1 << shift;
@@ -799,7 +803,7 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
         }
         if (tid < 128) {
             const float x = seen ? ap4_bf16(scale, 0) : 0.0f;
-            s_lds[buf][tid >> 6][scaled] = x;
+            s_lds[buf][tid >> 6][scaled] = tid < 64 ? x * kScaleUnit : x;
             // the segment's 16 values are those of the lanes that differ in bits 0, 3, 4 and 5
             float most = fmaxf(x, ap4_from<0xb1>(x));
             most = fmaxf(most, ap4_from<0x128>(most));
@@ -849,11 +853,11 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
             ap_split8(x[c], qh[c], lo);
             q_lds[wave][c][lane] = __builtin_bit_cast(uint4, lo);
         }
-        if (ap4_factors(A, kAp4Bits - e2, f_row, fc_row)) f_row = -f_row;
+        if (ap4_factors(A, kAp4Bits + kScaleBits - e2, INT_MIN, f_row, fc_row) != 1.0f) f_row = -f_row;
     }
-    // (large rows have the sign of f_row, taken off for each half: a register or a mask of their own spills others of heads of
-    // 64, 4096 rows 232 us and not 220)
-    const bool any_large = __any(f_row < 0.0f), capped_or_large = any_large || A.cap != 0.0f;
+    // (large rows have the sign of f_row, taken off for each half: a mask of their own, or one more branch, makes heads of 64 spill,
+    // 4096 rows 225 us and not 214)
+    const bool capped_or_large = __any(f_row < 0.0f) || A.cap != 0.0f;
     ap_f16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++)
@@ -907,9 +911,9 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
                     sc[4 * e] *= d.x, sc[4 * e + 1] *= d.y, sc[4 * e + 2] *= d.z, sc[4 * e + 3] *= d.w;
                 }
                 if (capped_or_large) {
-                    if (any_large) {
+                    if (__any(large)) {
 #pragma unroll
-                        for (int e = 0; e < 16; e++) sc[e] = ap4_raise(sc[e], large);
+                        for (int e = 0; e < 16; e++) sc[e] = large ? sc[e] * 0x1p64f : sc[e];
                     }
                     if (A.cap != 0.0f) {
 #pragma unroll

@@ -59,7 +59,7 @@ def test_sizes_of_queries_and_keys(dev, option, bits, kernel, hd, block, log2_q,
     keys whose dims all have the largest magnitude and the queries' signs."""
     group, (lengths, adds), large = KERNELS[kernel]
     option("ATTNP_LARGE", large)
-    rng = np.random.default_rng(hd + int(log2_q))
+    rng = np.random.default_rng(hd + int(log2_q) % 256)
     n, n_kv = sum(lengths) + sum(adds), 2
     u = rng.choice([-1, 1], (n_kv, hd))
     k = rng.uniform(-1, 1, (n, n_kv, hd)) * u
@@ -72,3 +72,12 @@ def test_sizes_of_queries_and_keys(dev, option, bits, kernel, hd, block, log2_q,
     o = dict(none={}, cap=dict(cap=10.0), slopes=dict(slopes=2.0 ** -np.arange(group * n_kv, dtype=np.float32)))[change]
     got = attend(bits, dev, cache, pages, q_start, kv_len, q, kq, **dict(o))
     ks.check(got, cache, pages, q_start, kv_len, q, float(np.float32(kq)), **o)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("hd,block", [(128, 16), (64, 64), (96, 32), (256, 32)])
+@pytest.mark.parametrize("log2_q,log2_k,change", [(-10, 126, "none"), (-60, 117, "none"), (-100, 122, "slopes"), (-120, 126, "cap"),
+                                                  (-124, 126, "none")])
+def test_the_largest_keys(dev, option, kernel, hd, block, log2_q, log2_k, change):
+    """The same with keys up to the largest that 4 bits hold."""
+    test_sizes_of_queries_and_keys(dev, option, 4, kernel, hd, block, log2_q, log2_k, change)
