@@ -95,17 +95,18 @@ class Cache:
             return (np.zeros((self.n_kv, 0, self.hd)),) * 2
         return np.concatenate(k, 1)[:, :n], np.concatenate(v, 1)[:, :n]
 
-    def append(self, table, q_start, kv_len, k, v):
+    def append(self, table, q_start, kv_len, k, v, max_q=2 ** 31, max_kv=2 ** 31):
         """The step's rows [token, head, dim] into the pages."""
         for r, end in enumerate(int(x) for x in kv_len):
             q0, q1 = int(q_start[r]), int(q_start[r + 1])
             start = end - (q1 - q0)
-            for b in range(start // self.block, blocks_of(end, self.block) if q1 > q0 else 0):
+            end = min(start + min(q1 - q0, max_q), max_kv)  # of what is written
+            for b in range(start // self.block, blocks_of(end, self.block) if end > start else 0):
                 p, first = int(table[r, b]), max(start - b * self.block, 0)
                 if not 0 <= p < self.n_pages:
                     continue
                 t0 = q0 + b * self.block + first - start
-                t1 = min(q1, q0 + (b + 1) * self.block - start)
+                t1 = q0 + min(end, (b + 1) * self.block) - start
                 for h in range(self.n_kv):
                     got, s = append_page(self.k[p, h], self.ks[p, h], k[t0:t1, h], first)
                     self.k[p, h], self.ks[p, h] = got.astype(np.int8), s
