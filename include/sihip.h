@@ -332,8 +332,8 @@ int sihip_kv_read_dev(sihip_ctx *ctx, const sihip_kv_cache *cache, const int64_t
  * behind the last token are left as they were. Products are of f32 accuracy:
  * a value of q counts to 2^-22 of itself (2^-38 of its row's largest where that
  * is more), a key's probability times its value scale to 2^-22 of that (2^-34
- * of the row's largest such product), and probabilities below 2^-126 of the
- * row's largest are zero. Sums are f32; results do not depend on the order in
+ * of the row's largest such product, and 2^-134), and probabilities below 2^-126 of the
+ * row's largest are zero. Scores are to be below 2^29 in magnitude. Sums are f32; results do not depend on the order in
  * which workgroups run.
  * workspace: NULL, or device memory of sihip_attn_paged_workspace bytes
  * (16-byte aligned) of its own for calls that may overlap other work of the
@@ -426,7 +426,8 @@ int sihip_kv4_read_dev(sihip_ctx *ctx, const sihip_kv4_cache *cache, const int64
 
 /* Attention over it: sihip_attn_paged_dev in every respect, of the same accuracy (a
  * key's probability times its value scale counts to 2^-22 of that, 2^-34 of the row's
- * largest such product), and with the same workspace rules. */
+ * largest such product, and 2^-134), and with the same workspace rules. Queries, keys and values may be
+ * of any size that f32 and the cache hold. */
 int sihip_attn_paged4_dev(sihip_ctx *ctx, const sihip_kv4_cache *cache, const sihip_kv_batch *batch,
                           const sihip_attn_paged *args, void *stream);
 int sihip_attn_paged4_workspace(sihip_ctx *ctx, const sihip_kv4_cache *cache,
@@ -434,7 +435,7 @@ int sihip_attn_paged4_workspace(sihip_ctx *ctx, const sihip_kv4_cache *cache,
                                 uint64_t *bytes);
 
 /* ---- log probabilities -----------------------------------------------------
- * Of n_rows rows of n_vocab logits (f32, row i at i * ld), as sihip_gemm_dev of the head
+ * Of n_rows (less than 2^24) rows of n_vocab logits (f32, row i at i * ld), as sihip_gemm_dev of the head
  * leaves them, with log p_j = x_j - log sum e^x:
  *   logprob   f32 [n_rows][n_token], of the tokens token[n_rows][n_token]; an entry whose
  *             token is outside 0 .. n_vocab - 1 is left as it was

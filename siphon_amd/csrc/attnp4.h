@@ -366,21 +366,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_rows_kernel(Attn4Args A)
     ap_rows_end<ND, WAVES>(A, s, R, o, kAp4Unit / kApUnit, h, tile, n_rows, piece, split, n_split, tok, head);
 }
 
-// The same for so few rows that the 16 columns of a tile can be NG groups of 32 dims times RB =
-// 16 / NG rows: column group * RB + row. A column's query values are those of its group alone, so that
-// a tile's score is the group's part of it, and a part is multiplied by the group's sub of its
-// token where the key's scale is, in f32; the parts of a row are then added over its columns. The
-// sums of values likewise: weights times subs are a column's operand, and of its sums the dims of its
-// group are used. No code is multiplied by a sub: the subs of a token and its group are two numbers of a
-// lane where the other kernel has eight, and their products with codes.
-//
-// Bound by memory and vector instructions at once: of a chunk's 640 instructions 290 make codes f16, the others are
-// scores, weights and splits, of which NG columns have the same (vector pipes busy for two thirds of the time,
-// matrix ones a fifth). 64 single tokens over up to 8192 keys, 32 heads of 128 on 8, 66-72 us (224 MB, 3.1-3.4 TB/s), 94 by
-// the kernel above; one over 131072 42 (147 MB, 3.5 TB/s) and 63; 16 over up to 16000, 16 heads of 256 on 8, 78. Which of both runs
-// is a matter of the columns: more rows do not fit.
 // Codes alone, in units of 2^-10: of a nibble n 2^-24 or n 2^-20 (ap4_cvt) one packed FMA with
-// constants.
+// constants. (In units of 2^-24 they would need no factor at bit 0. But they are subnormal then, and the matrix cores add products
+// of such numbers with fewer bits: results were off by 10^-5.)
 constexpr int kAp4CodeBits = 10;
 constexpr float kAp4Code = 1 << kAp4CodeBits;
 
@@ -414,6 +402,20 @@ __device__ inline void ap4_over_groups(float (&x)[N]) {
     if constexpr (NG >= 8) add(std::integral_constant<int, 0x122>());  // 2
 }
 
+// The same for so few rows that the 16 columns of a tile can be NG groups of 32 dims times RB =
+// 16 / NG rows: column group * RB + row. A column's query values are those of its group alone, so that
+// a tile's score is the group's part of it, and a part is multiplied by the group's sub of its
+// token where the key's scale is, in f32; the parts of a row are then added over its columns. The
+// sums of values likewise: weights times subs are a column's operand, and of its sums the dims of its
+// group are used. No code is multiplied by a sub: the subs of a token and its group are two numbers of a
+// lane where the other kernel has eight, and their products with codes.
+//
+// Bound by memory and vector instructions at once: of a chunk's 640 instructions 290 make codes f16, the others are
+// scores, weights and splits, of which NG columns have the same (vector pipes busy for two thirds of the time,
+// matrix ones a fifth). 64 single tokens over up to 8192 keys, 32 heads of 128 on 8, 65 us in a loop (224 MB, 3.4 TB/s), 70 by
+// the kernel above; one over 131072 41 (147 MB, 3.6 TB/s) and 44; 16 over up to 16000, 16 heads of 256 on 8, 77 and 92; 64 over
+// up to 8192, 32 heads of 96, 56 and 61. Which of both runs is a matter of the columns: more rows do not fit (5 to 8 heads of
+// 128 on each of 8 take 70 to 72 with the kernel above).
 template <int KD, int NK, int ND, int TT, int WAVES, int NG>
 __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args A) {
     constexpr int CH = 16 * TT, SEG = 4 * TT, KW = KD / 8, VW = SEG / 8, RB = 16 / NG;
@@ -665,12 +667,6 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attnp4_groups_kernel(Attn4Args 
 
 // ---- many rows ---------------------------------------------------------------------
 //
-// x of another lane of the row of 16
-template <int CTRL>
-__device__ inline float ap4_from(float x) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
-}
-
 // attnp_tiles_kernel (attnp.h) over 4-bit values: the codes of a 64-key chunk become f16 numbers
 // once, code * sub, on their way into LDS; the scales of its keys and values lie there beside
 // them, as f32. A unit of 16 values is 8 bytes here.
@@ -679,11 +675,12 @@ __device__ inline float ap4_from(float x) {
 // values follow; two barriers a chunk. The queries' lower halves are read from LDS for each half: in
 // registers they would leave none for the next scores.
 //
-// Bound by the vector step: its pipes are busy for more than half of the time and the matrix ones for 42%, and a wave
-// overlaps little of its own (two waves a SIMD are all that the registers allow). 3 prompts of up to 4096 tokens behind up to 1000, 40
-// heads of 128 on 8, slopes and prefixes, 670 us: 437 TFLOP/s, twice that with the second halves, against the
-// 1177 of a large f16 product; 4096 rows of 32 heads of 128 322, of 64 219. Four waves a block for heads up to 64
-// (with eight 252), eight for wider ones (with four, of whose blocks LDS holds one, 497).
+// Bound by the vector step: vector instructions take 50% of the cycles (exponentials, four times as long, counted once) and
+// products 42%, and a wave overlaps little of its own (two waves a SIMD are all that the registers allow). 3 prompts of up to 4096
+// tokens behind up to 1000, 40 heads of 128 on 8, slopes and prefixes, 660-690 us: 425-445 TFLOP/s, twice that with the second
+// halves, against the 1177 of a large f16 product; 4096 rows of 32 heads of 128 320-330, of 64 212-220. Four waves a block for
+// heads up to 64 (with eight 252), eight for wider ones (with four, of whose blocks LDS holds one, 497). Waves without rows,
+// chunks that a wave's rows do not see and what follows the last chunk take their turn with the others: nothing is skipped.
 constexpr int ap4_tile_waves(int hd) { return hd <= 64 ? 4 : 8; }
 
 template <int NS, int WAVES = ap4_tile_waves(16 * NS)>
@@ -805,8 +802,8 @@ __global__ __launch_bounds__(64 * WAVES, NS == 4 ? 3 : 2) void attnp4_tiles_kern
             const float x = seen ? ap4_bf16(scale, 0) : 0.0f;
             s_lds[buf][tid >> 6][scaled] = tid < 64 ? x * kScaleUnit : x;
             // the segment's 16 values are those of the lanes that differ in bits 0, 3, 4 and 5
-            float most = fmaxf(x, ap4_from<0xb1>(x));
-            most = fmaxf(most, ap4_from<0x128>(most));
+            float most = fmaxf(x, kv4_from<0xb1>(x));
+            most = fmaxf(most, kv4_from<0x128>(most));
             most = ap_max_quarters(most);
             if (tid >= 64 && tid < 72) m_lds[buf][tid >> 1 & 3] = vpg >= 0 ? most : -1.0f;
         }

@@ -78,7 +78,10 @@ int check_batch(sihip_ctx *ctx, const char *fn, const sihip_kv_batch *b, int64_t
     return SIHIP_OK;
 }
 
-// Rotated queries of more than twice what the L2s hold are written past them.
+// Rotated queries of more than twice what the L2s hold are written past them. By the step's room, which the host knows: a step of
+// fewer rows loses nothing by it. us of an append and the attention that reads its queries next, through / past the L2s, 32 heads of
+// 128 on 8, over 4 and 8 bits: a row 16.3 / 16.5 and 15.7 / 15.9; 64 single tokens behind 600 keys 26.5 / 26.0 and 25.9 /
+// 25.6, behind 8191 71.9 / 71.8 and 99.1 / 98.4; 1008 rows 75.1 / 74.5 and 63.9 / 63.3.
 constexpr int64_t kPastBytes = 64 << 20;
 
 // The new rows of a step for a cache of n_kv heads of hd dims. Without tokens
@@ -148,11 +151,12 @@ constexpr int kApFewRows = 64;
 //     to 512 184 / 205, 8 of up to 1024 128 / 125
 //   14 heads of 64 on 2: 1200 27 / 33, 4096 133 / 124; 32 on 8: 4096 239 / 171
 //   wider than 128 the large blocks' sums would leave one wave a SIMD: 16 heads of
-//     256, 4096 rows 467, 627 in a build that had them
-// and over 4 bits:
+//     256, 4096 rows 467, 627 in a build that had them (over 4 bits 770, and none was built)
+// and over 4 bits (one threshold for both: of these it has the slower side for 2048 rows with the window, and for 1300 of
+// heads of 96):
 //   32 heads of 128: 1500 rows 102 / 111, 1800 136 / 132, 2048 158 / 144, 3000 298 / 202; 190 behind 8000 keys 120 /
-//     125, 256 behind 8000 123 / 96, 64 behind 30000 133 / 87; window of 512, 2048 rows 81 / 66; 200 prompts of up to
-//     256 312 / 385, 50 of up to 512 192 / 217, 8 of up to 1024 106 / 91; heads of 96: 1300 84 / 79, 2048 156 / 128
+//     125, 256 behind 8000 123 / 96, 64 behind 30000 133 / 87; window of 512, 2048 rows 82 / 67; 200 prompts of up to
+//     256 312 / 385, 50 of up to 512 192 / 217, 8 of up to 1024 106 / 91; heads of 96: 1300 85 / 80, 2048 156 / 128
 //   heads of 64: 32 on 8: 2048 105 / 107, 3000 199 / 159
 int attn_waves(const sihip_ctx *ctx, const AttnPArgs &A, int waves, int64_t rows, int64_t all_rows) {
     if (A.C.hd > 128) return 0;

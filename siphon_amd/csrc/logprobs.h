@@ -19,8 +19,8 @@
 // A row of many logits is split over workgroups. A wave of each leaves its n_top largest in order, and the first
 // wave of the last workgroup to arrive takes from the lists' fronts what may be among the row's.
 //
-// Bound by memory where there are rows enough: 500 rows of 151936 (304 MB) 50 us (6.0 TB/s, a part of them from the
-// Infinity Cache), with the 20 most likely 67 (4.5); few rows by instructions in turn: one row of 151936 with 5
+// Bound by memory where there are rows enough: 500 rows of 151936 (304 MB) 50-53 us (5.8-6.0 TB/s, a part of them from the
+// Infinity Cache), with the 20 most likely 67-72 (4.2-4.5), with 64 105; few rows by instructions in turn: one row of 151936 with 5
 // tokens takes 9.5 us, 3.5 of which an empty launch takes, 1 the pass, 2 the choices of the splits, 1.5 sums and
 // their way to the last workgroup, 1.5 its choice. (A choice of single keys as they came, with comparisons of integers:
 // 11.9, 64 rows of 32003 with 20 tokens 17 and not 13.8.)
@@ -152,7 +152,6 @@ __device__ inline void lp_pad(uint64_t *keys, int n) {
 }
 
 // A wave's choice of the n_top largest of the keys it is shown.
-// it runs, so that there is one take of four keys a lane, not one of each key: 13 KB of code, not 67.)
 struct LpChoice {
     uint64_t *list;  // of the wave, in LDS: kLpList keys and 128 more
     int n_top, count = 0;
